@@ -85,6 +85,38 @@ class DualDesc(C.Structure):
   ]
 
 
+class BlockQuantDesc(C.Structure):
+  """aqtb200_block_quant_desc."""
+  _fields_ = [
+      ('x', View), ('qdtype', C.c_int32), ('po2_scale', C.c_int32),
+      ('square', C.c_int32), ('sizes_int64', C.c_int32),
+      ('q_row', C.c_void_p), ('ld_row', C.c_int64), ('scale_row', C.c_void_p),
+      ('q_col', C.c_void_p), ('ld_col', C.c_int64), ('scale_col', C.c_void_p),
+      ('group_sizes', C.c_void_p), ('groups', C.c_int64),
+  ]
+
+
+class GroupedGemmDesc(C.Structure):
+  """aqtb200_grouped_gemm_desc."""
+  _fields_ = [
+      ('contract_groups', C.c_int32), ('a_dtype', C.c_int32),
+      ('b_dtype', C.c_int32), ('out_dtype', C.c_int32),
+      ('r', C.c_int64), ('t', C.c_int64), ('k', C.c_int64), ('rows', C.c_int64),
+      ('a', C.c_void_p), ('a_ld', C.c_int64), ('a_group_stride', C.c_int64),
+      ('b', C.c_void_p), ('b_ld', C.c_int64),
+      ('a_mn_major', C.c_int32), ('b_mn_major', C.c_int32),
+      ('a_scale_square', C.c_int32), ('sizes_int64', C.c_int32),
+      ('a_scale', C.c_void_p), ('a_scale_group_stride', C.c_int64),
+      ('a_scale_k_stride', C.c_int64), ('a_scale_r_stride', C.c_int64),
+      ('b_scale', C.c_void_p), ('b_scale_k_stride', C.c_int64),
+      ('group_sizes', C.c_void_p), ('groups', C.c_int64),
+      ('out', C.c_void_p), ('out_ld', C.c_int64), ('out_group_stride', C.c_int64),
+      ('workspace', C.c_void_p), ('workspace_bytes', C.c_size_t),
+  ]
+
+
+MAX_GROUPS = 1024  # AQTB200_MAX_GROUPS
+
 # name -> (restype, argtypes); every symbol include/aqt_b200.h declares.
 MAX_RANKS = 8
 
@@ -138,6 +170,14 @@ SYMBOLS = {
         C.POINTER(DgRawDesc), C.c_void_p]),
     'aqtb200_dot_general_raw_exchange': (C.c_int, [
         C.POINTER(DgRawDesc), C.POINTER(ExchangeDesc), C.c_void_p, C.c_void_p]),
+    'aqtb200_block_quantize': (C.c_int, [
+        C.POINTER(BlockQuantDesc), C.c_void_p]),
+    'aqtb200_grouped_gemm_workspace_bytes': (C.c_size_t, [
+        C.POINTER(GroupedGemmDesc)]),
+    'aqtb200_grouped_gemm': (C.c_int, [
+        C.POINTER(GroupedGemmDesc), C.c_void_p, C.c_void_p]),
+    'aqtb200_pack_bf16': (C.c_int, [
+        C.POINTER(View), C.c_void_p, C.c_int64, C.c_void_p]),
     'aqtb200_dequantize': (C.c_int, [
         C.POINTER(View), C.POINTER(View), C.c_int32, C.c_void_p, C.c_void_p]),
     'aqtb200_set_device': (C.c_int, [C.c_int]),

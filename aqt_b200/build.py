@@ -13,9 +13,11 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 LIB = os.path.join(HERE, 'libaqt_b200.so')
-SOURCES = ['quantize.cu', 'gemm.cu', 'noise.cu', 'runtime.cu', 'api.cu',
+SOURCES = ['quantize.cu', 'gemm.cu', 'block_quantize.cu', 'grouped_gemm.cu',
+           'noise.cu', 'runtime.cu', 'api.cu',
            'xla_ffi.cc']
 HEADERS = [os.path.join(CSRC, 'common.cuh'),
+           os.path.join(CSRC, 'tcgen05.cuh'), os.path.join(CSRC, 'groups.cuh'),
            os.path.join(HERE, '..', 'include', 'aqt_b200.h')]
 NVCC_FLAGS = [
     '-gencode', 'arch=compute_100a,code=sm_100a', '-O3', '-lineinfo',

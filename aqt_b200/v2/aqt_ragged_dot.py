@@ -1,0 +1,188 @@
+"""Products of consecutive row groups with a matrix each: a mixture of experts.
+
+    out[i] = lhs[i] . rhs[e(i)]         lhs [M, K], rhs [G, K, N], group_sizes [G]
+
+e(i) is the group row i falls into when the groups, `group_sizes[e]` rows each,
+lie one after the other. The reference swaps lax.ragged_dot into its quantized
+dot_general for this, forward only (aqt/jax/v2/aqt_ragged_dot.py:23-86); here
+the gradients exist too:
+
+    dlhs[i] = g[i] . rhs[e(i)]^T        drhs[e] = sum_{i in e} lhs[i]^T g[i]
+
+    y = ragged_dot(x, w, sizes)                                  # bf16
+    y = ragged_dot(x, w, sizes, cfg=block_scaled.dot_general_make())   # fp8
+    y = ragged_dot(x, block_quantize(w, 1, square=True), sizes, cfg=...)  # serving
+
+group_sizes (int32 or int64) lives on the device and is never read by the host.
+Rows behind the last group give zeros and take no part in drhs; an empty group
+has a zero drhs. Sizes are made safe on the device: a negative one counts as
+zero, and the running sum is cut at M.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from aqt_b200 import block_engine as be
+from aqt_b200.v2 import aqt_tensor
+from aqt_b200.v2 import block_scaled
+
+
+def ragged_dot(lhs, rhs, group_sizes, cfg=None, preferred_element_type=None):
+  """lhs [M, K] times rhs [G, K, N], rows grouped by group_sizes [G].
+
+  cfg None: bfloat16 operands, f32 sums. cfg a BlockScaledDotGeneral: float32 or
+  bfloat16 operands in block-scaled fp8; rhs may then be a QTensor of 128 x 128
+  blocks contracted over axis 1 (serving, without gradient). The result has
+  lhs's dtype, or preferred_element_type (float32, bfloat16); without cfg a
+  float32 cotangent is rounded to bfloat16, the type of the products.
+  """
+  out_dtype = _check(lhs, rhs, group_sizes, cfg, preferred_element_type)
+  if isinstance(rhs, aqt_tensor.QTensor):
+    if torch.is_grad_enabled() and lhs.requires_grad:
+      raise NotImplementedError(
+          'a product with frozen weights has no gradient; pass float weights')
+  elif torch.is_grad_enabled() and (lhs.requires_grad or rhs.requires_grad):
+    return _RaggedDot.apply(lhs, rhs, group_sizes, cfg, out_dtype)
+  return _forward(lhs, rhs, group_sizes, cfg, out_dtype, (False, False))[0]
+
+
+def ragged_dot_vjp(lhs, rhs, group_sizes, cfg=None, preferred_element_type=None):
+  """(out, backprop) of ragged_dot with backprop(g) -> (dlhs, drhs)."""
+  if isinstance(rhs, aqt_tensor.QTensor):
+    raise NotImplementedError(
+        'a product with frozen weights has no gradient; pass float weights')
+  out_dtype = _check(lhs, rhs, group_sizes, cfg, preferred_element_type)
+  out, step = _forward(lhs.detach(), rhs.detach(), group_sizes, cfg, out_dtype,
+                       (True, True))
+  return out, lambda g: _backward(step, g, (True, True))
+
+
+def _check(lhs, rhs, group_sizes, cfg, preferred):
+  q = isinstance(rhs, aqt_tensor.QTensor)
+  if cfg is not None and not isinstance(cfg, block_scaled.BlockScaledDotGeneral):
+    raise NotImplementedError(
+        'cfg is None (bfloat16) or block_scaled.dot_general_make(...)')
+  if q and cfg is None:
+    raise ValueError('a frozen rhs needs cfg=block_scaled.dot_general_make(...)')
+  floats = be._FLOATS if cfg is not None else (torch.bfloat16,)  # pylint: disable=protected-access
+  be.check_operand(lhs, 'lhs', floats)
+  w = rhs.qvalue if q else rhs
+  be.check_operand(w, 'rhs', be._FP8 if q else floats)  # pylint: disable=protected-access
+  if not q and lhs.dtype != rhs.dtype:
+    raise TypeError(f'Unmatched lhs and rhs dtype: {lhs.dtype} vs {rhs.dtype}')
+  if lhs.ndim != 2 or w.ndim != 3:
+    raise ValueError('ragged_dot takes lhs [M, K] and rhs [G, K, N] (got '
+                     f'{tuple(lhs.shape)}, {tuple(w.shape)})')
+  if lhs.shape[1] != w.shape[1]:
+    raise ValueError(f'contracted extents differ: lhs {tuple(lhs.shape)}, rhs '
+                     f'{tuple(w.shape)}')
+  be.check_group_sizes(group_sizes, w.shape[0])
+  be.check_same_device(lhs, w, group_sizes)
+  return block_scaled._out_dtype(preferred, lhs)  # pylint: disable=protected-access
+
+
+class _Step:
+  __slots__ = ('cfg', 'lhs', 'rhs', 'sizes', 'keep', 'lhs_dtype', 'rhs_dtype',
+               'shape')
+
+
+def _forward(lhs, rhs, sizes, cfg, out_dtype, grads):
+  need_l, need_r = grads
+  with be.on_device_of(lhs):
+    step = None
+    if need_l or need_r:
+      step = _Step()
+      step.cfg, step.sizes = cfg, sizes
+      step.lhs_dtype, step.rhs_dtype = lhs.dtype, rhs.dtype
+      step.shape = (*lhs.shape, rhs.shape[2])
+      step.keep = None
+    if cfg is None:
+      out = be.bf16_rows(lhs, rhs, 1, sizes, out_dtype)
+      if step is not None:
+        step.lhs = lhs if need_r else None
+        step.rhs = rhs if need_l else None
+      return out, step
+    if isinstance(rhs, aqt_tensor.QTensor):
+      a, a_scale, a_dtype = block_scaled._frozen_operand(rhs, -2)  # pylint: disable=protected-access
+    else:
+      w = be.quantize(rhs, cfg.fwd_dtype, row=need_l, col=True, square=True,
+                      po2=cfg.po2_scale)
+      a, a_scale, a_dtype = block_scaled._kept_major(w, -2)  # pylint: disable=protected-access
+    l = be.quantize(lhs, cfg.fwd_dtype, row=True, col=need_r, po2=cfg.po2_scale,
+                    group_sizes=sizes if need_r else None)
+    out = be.fp8_rows(l.row, l.row_scale, lhs.shape[0], a, a_dtype, a_scale,
+                      a.shape[-2], lhs.shape[1], cfg.fwd_dtype, out_dtype, sizes)
+    if step is not None:
+      if need_r:
+        l.row = l.row_scale = None
+      step.lhs = l if need_r else None
+      step.rhs = w if need_l else None
+      step.keep = be.Residuals(
+          (l.tensors() if need_r else []) + (w.tensors() if need_l else []), lhs)
+    return out, step
+
+
+def _backward(step, g, grads):
+  need_l, need_r = grads
+  cfg, sizes = step.cfg, step.sizes
+  m, k, n = step.shape
+  if tuple(g.shape) != (m, n):
+    raise ValueError(f'the cotangent has shape {tuple(g.shape)}, the result '
+                     f'{(m, n)}')
+  dlhs = drhs = None
+  if cfg is None:
+    if g.dtype != torch.bfloat16:
+      g = g.to(torch.bfloat16)
+    with be.on_device_of(g):
+      if need_l:
+        dlhs = be.bf16_rows(g, step.rhs, 2, sizes, step.lhs_dtype)
+      if need_r:
+        drhs = be.bf16_contract_rows(step.lhs, g, sizes, step.rhs_dtype)
+    return dlhs, drhs
+  be.check_operand(g, 'the cotangent')
+  step.keep.about_to_use()
+  with be.on_device_of(g):
+    q = be.quantize(g, cfg.bwd_dtype, row=need_l, col=need_r, po2=cfg.po2_scale,
+                    group_sizes=sizes if need_r else None)
+    if need_l:
+      a, a_scale, a_dtype = block_scaled._kept_major(step.rhs, -1)  # pylint: disable=protected-access
+      dlhs = be.fp8_rows(q.row, q.row_scale, m, a, a_dtype, a_scale, k, n,
+                         cfg.bwd_dtype, step.lhs_dtype, sizes)
+    if need_r:
+      l = step.lhs
+      drhs = be.fp8_contract_rows(
+          l.col, l.col_scale, k, q.col, q.col_scale, n, l.col.shape[1], m,
+          cfg.bwd_dtype, cfg.fwd_dtype, step.rhs_dtype, sizes)
+  return dlhs, drhs
+
+
+class _RaggedDot(torch.autograd.Function):
+
+  @staticmethod
+  def forward(ctx, lhs, rhs, sizes, cfg, out_dtype):
+    out, step = _forward(lhs.detach(), rhs.detach(), sizes, cfg, out_dtype,
+                         ctx.needs_input_grad[:2])
+    if cfg is None:
+      # operands themselves: saved the way torch watches for writes into them
+      ctx.save_for_backward(sizes, step.lhs if step.lhs is None else lhs,
+                            step.rhs if step.rhs is None else rhs)
+      step.lhs = step.rhs = None
+    else:
+      ctx.save_for_backward(sizes)
+    step.sizes = None
+    ctx.step = step
+    return out
+
+  @staticmethod
+  def backward(ctx, g):
+    step = ctx.step
+    step.sizes = ctx.saved_tensors[0]
+    if step.cfg is None:
+      _, lhs, rhs = ctx.saved_tensors
+      step.lhs = None if lhs is None else lhs.detach()
+      step.rhs = None if rhs is None else rhs.detach()
+    dlhs, drhs = _backward(step, g, ctx.needs_input_grad[:2])
+    if step.cfg is None:
+      step.lhs = step.rhs = None
+    return dlhs, drhs, None, None, None

@@ -554,6 +554,115 @@ int aqtb200_jax_noise(uint32_t key0, uint32_t key1, int64_t n, int32_t kind,
  */
 int aqtb200_mma_peak(int32_t is_int, int64_t mmas_per_sm, int32_t* status, void* stream);
 
+/*
+ * Block-scaled fp8 (sub-channel scales): one f32 scale for each block of 128
+ * elements along the contraction, or for each 128 x 128 block. The reference
+ * reaches the same arithmetic by reshaping an axis into tiles of one scale each
+ * (tiled_dot_general.py:546-568).
+ *
+ *   a = max|x| over the block        s = max((a == 0 ? 1 : a) / bound, 2^-126)
+ *   po2_scale: s rounded up to a power of two
+ *   q = fp8(clip(x * (1/s), -bound, bound))    f32 arithmetic, bound 448 | 57344
+ *
+ * x         : view; its b0 * b1 matrices are quantized one after the other, any
+ *             strides, F32 | BF16.
+ * q_row     : [b][rows][ld_row] bytes, blocks along the columns; scale_row
+ *             [b][ceil(cols/128)][rows].
+ * q_col     : [b][cols][ld_col] bytes, the transpose, blocks along the rows;
+ *             scale_col [b][ceil(rows/128)][cols].
+ *             Either may be NULL; both together take one read of x. ld_* are
+ *             multiples of 16.
+ * square    : 128 x 128 blocks in both; scale_row and / or scale_col
+ *             [b][ceil(rows/128)][ceil(cols/128)].
+ * group_sizes: optional, device pointer to `groups` int32 (int64 when
+ *             sizes_int64): rows belong to consecutive groups and blocks along
+ *             the rows start anew at each group's first row. q_col and scale_col
+ *             are then in PADDED order: a group takes ceil(size/128) blocks, its
+ *             last one filled up with zeros; ld_col >= 128 * (rows/128 +
+ *             min(groups, rows)). Negative sizes count as 0, and the running sum
+ *             is cut at `rows`. Rows behind the last group are not read and their
+ *             places in q_row and scale_row are left as they were.
+ */
+typedef struct aqtb200_block_quant_desc {
+  aqtb200_view x;
+  int32_t qdtype; /* AQTB200_E4M3 | AQTB200_E5M2 */
+  int32_t po2_scale;
+  int32_t square;
+  int32_t sizes_int64;
+  void* q_row;
+  int64_t ld_row;
+  float* scale_row;
+  void* q_col;
+  int64_t ld_col;
+  float* scale_col;
+  const void* group_sizes;
+  int64_t groups;
+} aqtb200_block_quant_desc;
+
+int aqtb200_block_quantize(const aqtb200_block_quant_desc* desc, void* stream);
+
+/*
+ * aqtb200_grouped_gemm: matrix products of consecutive row groups (one expert
+ * each; the reference's quantized lax.ragged_dot, aqt_ragged_dot.py:23-86), in
+ * bf16 or in block-scaled fp8. With group_sizes NULL there is one group: an
+ * ordinary product.
+ *
+ *   contract_groups 0: out[t][r] = sum_k b[t][k] a[g(t)][r][k]   forward, dlhs
+ *       t: the grouped rows; rows behind the last group come out as zeros.
+ *   contract_groups 1: out[g][t][r] = sum_{k in group g} b[t][k] a[r][k]   drhs
+ *       k: the grouped rows; an empty group gives zeros.
+ * fp8:  every 128 products are summed on the tensor core, times a_scale times
+ *       b_scale, and added in f32. bf16: one f32 sum.
+ *
+ * r         : extent of the output's contiguous index; t: of its row index.
+ * k         : extent of the contraction; contract_groups 1 with groups: number of
+ *             grouped rows (bf16), or of padded positions in a and b (fp8; see
+ *             aqtb200_block_quantize).
+ * a, b      : element (r, k) of group g at g*a_group_stride + r*a_ld + k, or
+ *             with a_mn_major at g*a_group_stride + k*a_ld + r (bf16 only; b
+ *             alike). 16-byte aligned, strides multiples of 16 bytes.
+ * a_scale   : fp8 only. f32 of (r, block kb) at g*a_scale_group_stride +
+ *             kb*a_scale_k_stride + (a_scale_square ? r/128 : r)*a_scale_r_stride.
+ * b_scale   : f32 of (t, kb) at kb*b_scale_k_stride + t.
+ * group_sizes, groups, sizes_int64: as for aqtb200_block_quantize; at most
+ *             AQTB200_MAX_GROUPS groups.
+ * rows      : number of grouped rows (contract_groups 1; t otherwise).
+ * workspace : contract_groups 1 in bf16 with groups: aqtb200_grouped_gemm_
+ *             workspace_bytes() bytes, 256-byte aligned; otherwise unused.
+ * out       : F32 | BF16, (t, r) at g*out_group_stride + t*out_ld + r.
+ * status    : as for aqtb200_gemm_dequant.
+ */
+#define AQTB200_MAX_GROUPS 1024
+typedef struct aqtb200_grouped_gemm_desc {
+  int32_t contract_groups, a_dtype, b_dtype, out_dtype;
+  int64_t r, t, k, rows;
+  const void* a;
+  int64_t a_ld, a_group_stride;
+  const void* b;
+  int64_t b_ld;
+  int32_t a_mn_major, b_mn_major, a_scale_square, sizes_int64;
+  const float* a_scale;
+  int64_t a_scale_group_stride, a_scale_k_stride, a_scale_r_stride;
+  const float* b_scale;
+  int64_t b_scale_k_stride;
+  const void* group_sizes;
+  int64_t groups;
+  void* out;
+  int64_t out_ld, out_group_stride;
+  void* workspace;
+  size_t workspace_bytes;
+} aqtb200_grouped_gemm_desc;
+
+size_t aqtb200_grouped_gemm_workspace_bytes(const aqtb200_grouped_gemm_desc* desc);
+int aqtb200_grouped_gemm(const aqtb200_grouped_gemm_desc* desc, int32_t* status, void* stream);
+
+/*
+ * aqtb200_pack_bf16: out[b][rows][ld] = x[b][rows][cols] (bf16, any strides; b =
+ * b0 * b1), columns from `cols` to `ld` zero: brings an operand whose strides a
+ * tensor map cannot describe into a layout aqtb200_grouped_gemm takes.
+ */
+int aqtb200_pack_bf16(const aqtb200_view* x, void* out, int64_t ld, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

@@ -1,0 +1,376 @@
+"""Products grouped by expert on the GPU against the definition in 64 bits."""
+
+import numpy as np
+import pytest
+import torch
+
+from aqt_b200 import engine
+from aqt_b200.v2 import aqt_ragged_dot as rd
+from aqt_b200.v2 import block_scaled as bs
+from tests import block_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+
+
+def _data(shape, dtype, seed, scale=1.0):
+  rng = np.random.default_rng(seed)
+  return torch.from_numpy((rng.standard_normal(shape) * scale).astype(
+      np.float32)).to(dtype).cuda()
+
+
+def _f32(t):
+  return t.float().cpu().numpy()
+
+
+def _done():
+  torch.cuda.synchronize()
+  engine.check_status()
+
+
+def _sizes(values, dtype=torch.int32):
+  return torch.tensor(values, dtype=dtype, device='cuda')
+
+
+def _want(x, w, g, sizes, q, po2=False, fwd='e4m3', bwd='e5m2'):
+  x, w, g = (np.asarray(v, np.float64) for v in (x, w, g))
+  if not q:
+    pairs = (x, w, g, x, g)
+  else:
+    f = lambda v, br, bc, b: ref.fake(v, br, bc, b, po2)
+    xt, gt = np.zeros_like(x), np.zeros_like(g)
+    for a, b in ref.spans(sizes, len(x)):
+      if b > a:  # blocks along the rows start at each group's first row
+        xt[a:b], gt[a:b] = f(x[a:b], 128, 1, fwd), f(g[a:b], 128, 1, bwd)
+    pairs = (f(x, 1, 128, fwd), np.stack([f(m, 128, 128, fwd) for m in w]),
+             f(g, 1, 128, bwd), xt, gt)
+  xr, wq, gr, xt, gt = pairs
+  k, n = w.shape[1:]
+  out = (*ref.ragged(xr, wq, sizes), k)
+  dl = (*ref.ragged(gr, wq.transpose(0, 2, 1), sizes), n)
+  dr = (*ref.ragged_drhs(xt, gt, sizes, len(w)), len(x))
+  return out, dl, dr
+
+
+def _check(got, want, half, what):
+  value, mag, k = want
+  ref.assert_close(_f32(got).astype(np.float64), value, mag, k, half, what)
+
+
+# rows, K, N, group sizes
+CASES = [
+    (1, 64, 64, [1]),
+    (1, 64, 72, [0, 1, 0]),
+    (5, 8, 8, [0, 0, 0]),                       # every row behind the last group
+    (40, 200, 136, [40]),
+    (300, 264, 520, [1, 0, 63, 64, 65, 100]),   # seven rows left over
+    (300, 129, 77, [128, 129, 43]),             # odd strides
+    (513, 384, 256, [256, 257]),
+    (700, 136, 264, [0, 700, 0]),
+    (90, 72, 96, [30] * 40),                    # more than there are rows
+    (90, 72, 96, [-5, 40, -1, 60]),             # negative sizes, cut at the end
+    (70, 64, 64, [2] * 35),
+]
+
+
+@pytest.mark.parametrize('m,k,n,sizes', CASES)
+@pytest.mark.parametrize('q', [False, True])
+@pytest.mark.parametrize('index', [torch.int32, torch.int64])
+def test_step_matches_definition(m, k, n, sizes, q, index):
+  x, w, g = (_data((m, k), torch.bfloat16, 1), _data(
+      (len(sizes), k, n), torch.bfloat16, 2, 0.1), _data((m, n), torch.bfloat16, 3))
+  cfg = bs.dot_general_make() if q else None
+  out, bp = rd.ragged_dot_vjp(x, w, _sizes(sizes, index), cfg=cfg)
+  dl, dr = bp(g)
+  _done()
+  want = _want(_f32(x), _f32(w), _f32(g), sizes, q)
+  for name, got, wt in zip(('out', 'dlhs', 'drhs'), (out, dl, dr), want):
+    assert got.dtype == torch.bfloat16
+    _check(got, wt, 2.0 ** -8, name)
+  left = max(b for _, b in ref.spans(sizes, m))
+  assert not out[left:].any() and not dl[left:].any()
+
+
+@pytest.mark.parametrize('m,k,n,sizes', CASES)
+def test_float32_operands_and_results(m, k, n, sizes):
+  x, w, g = (_data((m, k), torch.float32, 4), _data(
+      (len(sizes), k, n), torch.float32, 5, 0.1), _data((m, n), torch.float32, 6))
+  cfg = bs.dot_general_make('e4m3', 'e4m3', po2_scale=True)
+  out, bp = rd.ragged_dot_vjp(x, w, _sizes(sizes), cfg=cfg)
+  dl, dr = bp(g)
+  _done()
+  for got, wt in zip((out, dl, dr), _want(_f32(x), _f32(w), _f32(g), sizes, True,
+                                          True, 'e4m3', 'e4m3')):
+    assert got.dtype == torch.float32
+    _check(got, wt, 2.0 ** -24, '')
+  xb, wb = x.bfloat16(), w.bfloat16()
+  out = rd.ragged_dot(xb, wb, _sizes(sizes), preferred_element_type=torch.float32)
+  _done()
+  assert out.dtype == torch.float32
+  _check(out, _want(_f32(xb), _f32(wb), _f32(g), sizes, False)[0], 2.0 ** -24, '')
+
+
+@pytest.mark.parametrize('m,k,n,sizes', CASES)
+def test_frozen_weights(m, k, n, sizes):
+  x, w, g = (_data((m, k), torch.bfloat16, 7), _data(
+      (len(sizes), k, n), torch.bfloat16, 8, 0.1), np.zeros((m, n)))
+  qt = bs.block_quantize(w, contract_axis=1, square=True)
+  again = bs.frozen(qt.qvalue.contiguous(), qt.scale[0].clone())
+  want = _want(_f32(x), _f32(w), g, sizes, True)[0]
+  for t in (qt, again):
+    out = rd.ragged_dot(x, t, _sizes(sizes), cfg=bs.dot_general_make())
+    _done()
+    _check(out, want, 2.0 ** -8, '')
+
+
+def test_long_decode_shares_the_contraction():
+  """One or two rows against long contractions: few tiles, so each one's
+  contraction is divided; the result must not depend on it."""
+  for m, sizes in ((1, [1]), (2, [1, 1]), (33, [33])):
+    for q in (False, True):
+      x, w = _data((m, 4104), torch.bfloat16, 9), _data(
+          (len(sizes), 4104, 264), torch.bfloat16, 10, 0.05)
+      cfg = bs.dot_general_make() if q else None
+      a = rd.ragged_dot(x, w, _sizes(sizes), cfg=cfg)
+      b = rd.ragged_dot(x, w, _sizes(sizes), cfg=cfg)
+      _done()
+      assert torch.equal(a, b)
+      _check(a, _want(_f32(x), _f32(w), np.zeros((m, 264)), sizes, q)[0],
+             2.0 ** -8, '')
+
+
+def test_many_groups():
+  g = 1024
+  rng = np.random.default_rng(11)
+  sizes = rng.integers(0, 3, g)
+  m = int(sizes.sum()) + 4
+  x, w = _data((m, 64), torch.bfloat16, 12), _data((g, 64, 32), torch.bfloat16, 13)
+  ct = _data((m, 32), torch.bfloat16, 14)
+  for q in (False, True):
+    out, bp = rd.ragged_dot_vjp(x, w, _sizes(sizes),
+                                cfg=bs.dot_general_make() if q else None)
+    dl, dr = bp(ct)
+    _done()
+    for got, wt in zip((out, dl, dr), _want(_f32(x), _f32(w), _f32(ct), sizes, q)):
+      _check(got, wt, 2.0 ** -8, '')
+
+
+@pytest.mark.parametrize('q', [False, True])
+@pytest.mark.parametrize('bad', [float('nan'), float('inf')])
+def test_groups_do_not_mix(q, bad):
+  """What lies in other groups' rows, or behind the last group, reaches nothing."""
+  m, k, n, sizes = 200, 136, 72, [30, 0, 70, 50]
+  x, w, g = (_data((m, k), torch.bfloat16, 15), _data(
+      (4, k, n), torch.bfloat16, 16), _data((m, n), torch.bfloat16, 17))
+  cfg = bs.dot_general_make() if q else None
+
+  def step():
+    out, bp = rd.ragged_dot_vjp(x, w, _sizes(sizes), cfg=cfg)
+    return (out, *bp(g))
+
+  out, dl, dr = step()
+  x[150:] = bad
+  g[150:] = bad
+  x[30, 5] = bad   # first row of the third group
+  g[99, 7] = bad   # its last row
+  out2, dl2, dr2 = step()
+  _done()
+  keep = [i for i in range(200) if not 30 <= i < 100]
+  assert torch.equal(out[keep], out2[keep]) and torch.equal(dl[keep], dl2[keep])
+  assert not out2[150:].any() and not dl2[150:].any()
+  for e in (0, 1, 3):
+    assert torch.equal(dr[e], dr2[e]), e
+  assert not torch.isfinite(out2[30]).any()
+  assert not torch.isfinite(dr2[2, 5]).any()
+
+
+@pytest.mark.parametrize('q', [False, True])
+def test_any_strides(q):
+  m, k, n, sizes = 150, 72, 88, [50, 60, 30]
+  x, w, g = (_data((m, k), torch.bfloat16, 18), _data(
+      (3, k, n), torch.bfloat16, 19), _data((m, n), torch.bfloat16, 20))
+  cfg = bs.dot_general_make() if q else None
+
+  def step(a, b, c):
+    out, bp = rd.ragged_dot_vjp(a, b, _sizes(sizes), cfg=cfg)
+    return (out, *bp(c))
+
+  want = step(x, w, g)
+
+  def off(t):
+    wide = torch.zeros(*t.shape[:-1], t.shape[-1] + 9, dtype=t.dtype,
+                       device=t.device)
+    wide[..., 1:1 + t.shape[-1]] = t
+    return wide[..., 1:1 + t.shape[-1]]
+
+  flip = lambda t: t.transpose(-1, -2).contiguous().transpose(-1, -2)
+  every = torch.zeros(6, k, n, dtype=w.dtype, device='cuda')
+  every[::2] = w
+  for a, b, c in ((off(x), off(w), off(g)), (flip(x), flip(w), flip(g)),
+                  (x, every[::2], g), (x[:, :], w, g)):
+    got = step(a, b, c)
+    _done()
+    for s, t in zip(got, want):
+      assert torch.equal(s, t)
+
+
+def test_broadcast_weights():
+  """One matrix for every group (stride 0): gradients come per group."""
+  m, k, n, sizes = 60, 64, 48, [20, 10, 30]
+  x, one, g = (_data((m, k), torch.bfloat16, 21), _data(
+      (k, n), torch.bfloat16, 22), _data((m, n), torch.bfloat16, 23))
+  for q in (False, True):
+    cfg = bs.dot_general_make() if q else None
+    leaf = one.clone().requires_grad_()
+    out = rd.ragged_dot(x, leaf.expand(3, k, n), _sizes(sizes), cfg=cfg)
+    out.backward(g)
+    _, bp = rd.ragged_dot_vjp(x, one.expand(3, k, n).contiguous(), _sizes(sizes),
+                              cfg=cfg)
+    want = bp(g)[1].sum(0)
+    _done()
+    assert torch.equal(leaf.grad, want)
+
+
+def test_autograd_matches_vjp():
+  m, k, n, sizes = 100, 72, 64, [40, 0, 55]
+  x, w, g = (_data((m, k), torch.bfloat16, 24), _data(
+      (3, k, n), torch.bfloat16, 25), _data((m, n), torch.bfloat16, 26))
+  for q in (False, True):
+    cfg = bs.dot_general_make() if q else None
+    out, bp = rd.ragged_dot_vjp(x, w, _sizes(sizes), cfg=cfg)
+    dl, dr = bp(g)
+    for need_l, need_r in ((True, True), (True, False), (False, True)):
+      a, b = x.clone().requires_grad_(need_l), w.clone().requires_grad_(need_r)
+      y = rd.ragged_dot(a, b, _sizes(sizes), cfg=cfg)
+      y.backward(g, retain_graph=True)
+      assert torch.equal(y, out)
+      assert torch.equal(a.grad, dl) if need_l else a.grad is None
+      assert torch.equal(b.grad, dr) if need_r else b.grad is None
+      y.backward(g)  # a second time, from the same residuals
+    _done()
+
+
+def test_gradients_against_differences():
+  rng = np.random.default_rng(27)
+  ints = lambda *s: torch.from_numpy(
+      rng.integers(-3, 4, s).astype(np.float32)).cuda()
+  sizes = [3, 0, 4]
+  x, w, g = ints(8, 16), ints(3, 16, 8), ints(8, 8)
+  out, bp = rd.ragged_dot_vjp(x.bfloat16(), w.bfloat16(), _sizes(sizes))
+  dl, dr = bp(g.bfloat16())
+  _done()
+  x64, w64, g64 = (_f32(t).astype(np.float64) for t in (x, w, g))
+  loss = lambda a, b: float((ref.ragged(a, b, sizes)[0] * g64).sum())
+  for i, j in ((0, 1), (6, 15), (7, 3)):
+    d = np.zeros_like(x64)
+    d[i, j] = 1
+    assert float(dl[i, j]) == (loss(x64 + d, w64) - loss(x64 - d, w64)) / 2
+  for e, i, j in ((0, 1, 0), (1, 2, 2), (2, 15, 7)):
+    d = np.zeros_like(w64)
+    d[e, i, j] = 1
+    assert float(dr[e, i, j]) == (loss(x64, w64 + d) - loss(x64, w64 - d)) / 2
+
+
+def test_empty_extents():
+  for q in (False, True):
+    cfg = bs.dot_general_make() if q else None
+    for m, k, n in ((0, 64, 32), (4, 0, 32), (4, 64, 0)):
+      x = torch.ones(m, k, device='cuda', dtype=torch.bfloat16)
+      w = torch.ones(2, k, n, device='cuda', dtype=torch.bfloat16)
+      out, bp = rd.ragged_dot_vjp(x, w, _sizes([m // 2, m // 2]), cfg=cfg)
+      dl, dr = bp(torch.ones(m, n, device='cuda', dtype=torch.bfloat16))
+      _done()
+      assert tuple(out.shape) == (m, n) and not out.any()
+      assert dl.shape == x.shape and not dl.any()
+      assert dr.shape == w.shape and not dr.any()
+
+
+@pytest.mark.parametrize('q', [False, True])
+def test_captured_with_other_sizes_at_replay(q):
+  """The sizes are read by the kernels: a captured step follows new ones."""
+  m, k, n = 120, 136, 72
+  x, w, g = (_data((m, k), torch.bfloat16, 28), _data(
+      (4, k, n), torch.bfloat16, 29), _data((m, n), torch.bfloat16, 30))
+  sizes = _sizes([30, 30, 30, 30])
+  cfg = bs.dot_general_make() if q else None
+
+  def step():
+    out, bp = rd.ragged_dot_vjp(x, w, sizes, cfg=cfg)
+    return (out, *bp(g))
+
+  step()
+  torch.cuda.synchronize()
+  graphs, outs = [], []
+  for _ in range(2):  # two graphs alive at once
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+      outs.append(step())
+    graphs.append(graph)
+  for values in ([0, 119, 1, 0], [64, 0, 3, 20], [1, 1, 1, 117]):
+    sizes.copy_(_sizes(values))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+      graphs[1].replay()
+    graphs[0].replay()
+    torch.cuda.current_stream().wait_stream(side)
+    want = step()
+    _done()
+    for got in outs:
+      for s, t in zip(got, want):
+        assert torch.equal(s, t)
+
+
+def test_expert_layer():
+  """Router, experts and their gradients together, as a model runs them: rows
+  sorted by expert, gate and up products, a gated product, the down product,
+  weighted and added back; against the same layer in 64 bits."""
+  tokens, d, f, e, top = 96, 128, 192, 6, 2
+  x = _data((tokens, d), torch.bfloat16, 31)
+  router = _data((d, e), torch.float32, 32, 0.2)
+  ws = [_data((e, d, f), torch.bfloat16, 33, 0.1), _data(
+      (e, d, f), torch.bfloat16, 34, 0.1), _data((e, f, d), torch.bfloat16, 35, 0.1)]
+  p, chosen = torch.softmax(x.float() @ router, -1).topk(top, -1)
+  expert = chosen.reshape(-1)
+  order = expert.argsort(stable=True)
+  sizes = torch.bincount(expert, minlength=e).to(torch.int32)
+  row = order // top
+  weight = p.reshape(-1)[order]
+  ct = _data((tokens, d), torch.float32, 36)
+
+  def layer(x, ws, product, cast):
+    rows = x[row]
+    gate, up = product(rows, ws[0]), product(rows, ws[1])
+    hidden = cast(torch.nn.functional.silu(gate.double()) * up.double())
+    down = product(hidden, ws[2]).double() * weight.double()[:, None]
+    return torch.zeros(tokens, d, dtype=torch.float64, device='cuda').index_add(
+        0, row, down)
+
+  def run(cfg, exact):
+    leaves = [t.double().requires_grad_() if exact else
+              t.clone().requires_grad_() for t in [x] + ws]
+    ends = sizes.cumsum(0).tolist()
+    if exact:
+      def product(a, w):
+        return torch.cat([a[b:c] @ w[i] for i, (b, c) in enumerate(
+            zip([0] + ends[:-1], ends))])
+      y = layer(leaves[0], leaves[1:], product, lambda t: t)
+    else:
+      y = layer(leaves[0], leaves[1:],
+                lambda a, w: rd.ragged_dot(a, w, sizes, cfg=cfg),
+                lambda t: t.bfloat16())
+    (y * ct.double()).sum().backward()
+    return [y.detach()] + [t.grad.double() for t in leaves]
+
+  want = run(None, True)
+  # relative error, in the 2-norm, of a chain of three products: bf16 rounds
+  # operands and results by 2^-8 at most, four times along the longest path and
+  # its gradient twice that; fp8 operands are off by at most 2^-4 (e4m3) or 2^-3
+  # (e5m2) each, two operands a product
+  for cfg, tol in ((None, 8 * 2.0 ** -8 * 2), (bs.dot_general_make(
+      'e4m3', 'e4m3'), 6 * 2 * 2.0 ** -4)):
+    got = run(cfg, False)
+    _done()
+    for a, b in zip(got, want):
+      assert float((a - b).norm() / b.norm()) < tol
