@@ -11,14 +11,15 @@
 // decode batch streams its weights at memory speed. Each tile issues MMAs only
 // as wide as the rows it has (a multiple of 32).
 //
-// Persistent kernel, one CTA pair (cta_group::2) per two SMs, 12 warps a CTA:
+// Persistent kernel, one CTA pair (cta_group::2) per two SMs, 12 or 20 warps a CTA:
 //   warp 0      TMA producer, 128-byte k-slabs, 128-byte swizzle, no multicast
 //   warp 1      MMA issuer (even CTA)
-//   warps 4-11  epilogue: two per TMEM lane quarter, 128 columns each
+//   warp 2      scales (fp8)
+//   warps 4-    epilogue: two or four per TMEM lane quarter, up to 64 columns each
 // bf16 accumulates the whole contraction in TMEM (two 256-column accumulators:
 // the epilogue of one tile runs under the next tile's MMAs). fp8 accumulates
 // one 128-block there; the epilogue warps read it, multiply by the two scales
-// and add it to f32 registers (128 a thread) while the tensor core fills the
+// and add it to f32 registers (64 a thread) while the tensor core fills the
 // other accumulator.
 //
 // Group sizes stay on the device: every CTA scans them once (prefix sums in
@@ -36,18 +37,25 @@ namespace aqtb200 {
 
 int sm_count();
 
-constexpr int GG_EPI = 8;
-constexpr int GG_COLS = 128;                 // columns an epilogue warp holds
-constexpr int GG_THREADS = 32 * (4 + GG_EPI);  // whole warpgroups, for the register split
-// Registers: 384 threads start with 168 each (64512). The first warpgroup keeps
-// 88 of them and the two epilogue warpgroups, whose threads hold 128 sums, take
-// 208: 128 * 88 + 256 * 208 = 64512.
-#define GG_REGS_FEW "88"
-#define GG_REGS_MANY "208"
+// Epilogue warps: SLICES for each TMEM lane quarter, COLS columns each; a tile is
+// up to SLICES * COLS columns wide. Four more warps carry the other roles.
+// Registers (setmaxnreg): the first warpgroup gives up what the epilogue takes.
+//   2 slices: 384 threads start with 168: 128 *  88 + 256 * 208 = 64512
+//   3 slices: 512 threads start with 128: 128 *  56 + 384 * 152 = 65536
+//   4 slices: 640 threads start with  96: 128 *  32 + 512 * 112 = 61440 (fp8)
+//                                         128 *  64 + 512 * 104 = 61440 (bf16)
+constexpr int gg_threads(int slices) { return 128 * (1 + slices); }
 constexpr int GG_A_STAGE = 128 * 128;        // this CTA's 128 rows of A, 128 bytes of k
-constexpr int GG_MAX_STAGES = 10;
+constexpr int GG_KS = 2;                     // k-slabs a stage of the ring holds
+constexpr int GG_MAX_STAGES = 5;
 constexpr int GG_RING = 192 * 1024;          // bytes of the operand ring
-constexpr int GG_F_BYTES = GG_EPI * GG_COLS * 4;  // scale factors, one a column and warp
+// Scales travel in batches of GG_BATCH slabs: one barrier round for four of them.
+constexpr int GG_BATCH = 4;
+constexpr int GG_SLOTS = 2;                  // batches on their way or in use
+constexpr int GG_SLOT = 256 + 128;           // floats a slab: 256 columns, this CTA's 128 rows
+constexpr int GG_SCALE_BYTES = GG_SLOTS * GG_BATCH * GG_SLOT * 4;
+constexpr int GG_STAGE_OUT = 512;            // a warp's staging: 8 columns by 32 rows of bf16
+constexpr size_t GG_SMEM = GG_RING + GG_SCALE_BYTES + 16 * GG_STAGE_OUT + 1024;
 constexpr int GG_MAX_SEG = AQTB200_MAX_GROUPS + 1;
 constexpr int GG_TAIL = 64;                  // k-slab of bf16 elements
 
@@ -55,6 +63,9 @@ struct GGParams {
   int mode;  // 0: t is grouped; 1: the contraction is grouped
   int nt;    // columns of a full tile
   int stages, b_stage;
+  // TMEM: two halves of 256 columns, handed over one at a time; each holds
+  // `half_kb` accumulators `buf_cols` columns apart (fp8: of consecutive slabs)
+  int half_kb, buf_cols;
   int split;           // CTA pairs of a cluster that share one tile's contraction
   int a_mn, b_mn, bk;  // bk: elements of k per slab
   uint32_t idesc;      // without the column count
@@ -68,6 +79,7 @@ struct GGParams {
   int64_t sb_k;
   void* out;
   int out_f32;
+  int out_staged;  // bf16 rows of whole 16-byte pieces
   int64_t o_ld, o_g;
   int32_t* status;
 };
@@ -85,21 +97,47 @@ __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr, uint32_t lbo) {
   return d;
 }
 
-__device__ __forceinline__ void gg_mma(bool fp8, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                       uint32_t idesc, uint32_t accumulate) {
-  if (fp8) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-  } else {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-        : "memory");
-  }
+// The four MMAs of one 128-byte slab, issued by the elected lane. The whole warp
+// runs this, so that descriptors stay in uniform registers: issued from a
+// one-lane branch each MMA took about 70 clocks of moves, and the issuing thread
+// was what bounded every fp8 product.
+#define GG_MMA4(KIND)                                                                       \
+  asm volatile(                                                                             \
+      "{\n\t.reg .pred q, p, t;\n\t.reg .b64 a, b;\n\t.reg .b32 x, y;\n\t"                     \
+      "setp.ne.b32 q, %8, 0;\n\tsetp.ne.b32 p, %7, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"            \
+      "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"                                    \
+      "@q tcgen05.mma.cta_group::2.kind::" KIND " [%0], a, b, %9, p;\n\t"                   \
+      "add.u32 x, %1, %5;\n\tadd.u32 y, %3, %6;\n\t"                                        \
+      "mov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"                                      \
+      "@q tcgen05.mma.cta_group::2.kind::" KIND " [%0], a, b, %9, t;\n\t"                   \
+      "add.u32 x, x, %5;\n\tadd.u32 y, y, %6;\n\t"                                          \
+      "mov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"                                      \
+      "@q tcgen05.mma.cta_group::2.kind::" KIND " [%0], a, b, %9, t;\n\t"                   \
+      "add.u32 x, x, %5;\n\tadd.u32 y, y, %6;\n\t"                                          \
+      "mov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"                                      \
+      "@q tcgen05.mma.cta_group::2.kind::" KIND " [%0], a, b, %9, t;\n\t}" ::"r"(d_tmem),   \
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(a_step), "r"(b_step), "r"(accumulate), \
+      "r"(elected), "r"(idesc)                                                              \
+      : "memory")
+template <bool FP8>
+__device__ __forceinline__ void gg_mma4(uint32_t elected, uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi,
+                                        uint32_t b_lo, uint32_t b_hi, uint32_t a_step, uint32_t b_step,
+                                        uint32_t idesc, uint32_t accumulate) {
+  if constexpr (FP8) GG_MMA4("f8f6f4");
+  else GG_MMA4("f16");
+}
+#undef GG_MMA4
+
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t e;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(e));
+  return e;
+}
+// A wait of the whole warp with one answer for all of its lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag) ? 1 : 0) != 0;
 }
 
 __device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* tm, uint32_t leader_bar,
@@ -110,9 +148,42 @@ __device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* t
       "l"(tm), "r"(leader_bar), "r"(c0), "r"(c1), "r"(c2)
       : "memory");
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+// Two f32 multiply-adds in one instruction: (a0, a1) += (x0, x1) * (y0, y1).
+__device__ __forceinline__ void fma2(float& a0, float& a1, float x0, float x1, float y0, float y1) {
+  asm("{\n\t.reg .b64 x, y, a;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 a, {%0, %1};\n\t"
+      "fma.rn.f32x2 a, x, y, a;\n\tmov.b64 {%0, %1}, a;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "f"(x0), "f"(x1), "f"(y0), "f"(y1));
+}
+// Arrives at both CTAs of the pair once every MMA issued so far has completed.
+__device__ __forceinline__ void gg_commit(uint32_t elected, uint32_t bar, uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%0], %1;\n\t}" ::"r"(bar),
+      "h"((uint16_t)(3u << lead)), "r"(elected)
+      : "memory");
+}
+
+// 16 lanes by 32 columns of TMEM; of every 8 columns a thread gets lane / 4's
+// columns 2 (lane % 4) and the next, then the same of lane / 4 + 8.
+__device__ __forceinline__ void tc_ld_16x256(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 
@@ -179,8 +250,8 @@ __device__ __forceinline__ int share_of(int nkb, int part, int split) {
   return (int)((int64_t)nkb * part / split);
 }
 
-template <bool FP8, bool A_ROW>
-__global__ void __launch_bounds__(GG_THREADS, 1)
+template <bool FP8, bool A_ROW, int SLICES, int COLS>
+__global__ void __launch_bounds__(gg_threads(SLICES), 1)
 grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmAt, const __grid_constant__ CUtensorMap tmBt,
                     GGParams P) {
@@ -190,6 +261,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   __shared__ __align__(8) uint64_t empty_bar[GG_MAX_STAGES];  // one per CTA
   __shared__ __align__(8) uint64_t tfull_bar[2];              // one per CTA
   __shared__ __align__(8) uint64_t tempty_bar[2];             // used in the pair's even CTA
+  __shared__ __align__(8) uint64_t sfull_bar[GG_SLOTS];       // scales of a slab; one per CTA
+  __shared__ __align__(8) uint64_t sempty_bar[GG_SLOTS];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   __shared__ int nseg_s;
@@ -212,7 +285,11 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&tfull_bar[s], 1);
-      mbar_init(&tempty_bar[s], 2 * GG_EPI);
+      mbar_init(&tempty_bar[s], 2 * 4 * SLICES);
+    }
+    for (int s = 0; s < GG_SLOTS; ++s) {
+      mbar_init(&sfull_bar[s], 32);
+      mbar_init(&sempty_bar[s], 4 * SLICES);
     }
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -281,43 +358,51 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const int total = total_s;
   volatile int* abortp = &abort_flag;
   const uint32_t peer_abort = map_to_cta(smem_u32(&abort_flag), crank ^ 1u);
-  const int stage_bytes = GG_A_STAGE + P.b_stage;
+  const int slab_bytes = GG_A_STAGE + P.b_stage, stage_bytes = GG_KS * slab_bytes;
+  float* const slots = (float*)(smem + P.stages * stage_bytes);
   int fail = 0;
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 " GG_REGS_FEW ";");
+    if constexpr (SLICES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    else if constexpr (SLICES == 3) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    else if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   if (warp == 0) {
     // ---------------- TMA producer (both CTAs) ----------------
     if (lane == 0) {
       int stage = 0, cur = 0;
       uint32_t phase = 0;
       const int b_boxes = P.b_mn ? (P.nt / 2 + 63) / 64 : 1;
+      const uint32_t lbar0 = map_to_cta(smem_u32(&full_bar[0]), lead);
       for (int tile = cluster_id; tile < total && !fail; tile += num_clusters) {
         const TileAt T = gg_tile<FP8>(P, S, nseg, tile, cur);
         const int kb0 = share_of(T.nkb, part, P.split), kb1 = share_of(T.nkb, part + 1, P.split);
         const int ra = T.r0 + (int)rank * 128, tb = T.t0 + (int)rank * (T.n / 2);
         const int ga = P.mode == 0 ? T.seg : 0;
-        for (int kb = kb0; kb < kb1; ++kb) {
+        for (int ks = kb0; ks < kb1; ks += GG_KS) {
           if (!mbar_wait(&empty_bar[stage], phase ^ 1, abortp)) { fail = 1; break; }
-          const uint32_t lbar = map_to_cta(smem_u32(&full_bar[stage]), lead);
-          if (leader) mbar_expect_tx(&full_bar[stage], 2 * stage_bytes);
+          const uint32_t lbar = lbar0 + stage * 8;
+          const int ke = min(ks + GG_KS, kb1);
+          if (leader) mbar_expect_tx(&full_bar[stage], 2 * (ke - ks) * slab_bytes);
           uint8_t* sa = smem + stage * stage_bytes;
-          uint8_t* sb = sa + GG_A_STAGE;
-          if (P.mode == 1 && !FP8 && T.klen - kb * GG_TAIL < GG_TAIL && P.groups > 0) {
-            // the group ends inside this slab: its copy, filled up with zeros
-            for (int j = 0; j < 2; ++j)
-              tma_load_3d_pair(sa + j * 8192, &tmAt, lbar, ra + j * 64, 0, T.seg);
-            for (int j = 0; j < b_boxes; ++j)
-              tma_load_3d_pair(sb + j * 8192, &tmBt, lbar, tb + j * 64, 0, T.seg);
-          } else {
+          for (int kb = ks; kb < ke; ++kb, sa += slab_bytes) {
+            uint8_t* sb = sa + GG_A_STAGE;
+            if (!FP8 && P.mode == 1 && T.klen - kb * GG_TAIL < GG_TAIL && P.groups > 0) {
+              // the group ends inside this slab: its copy, filled up with zeros
+              for (int j = 0; j < 2; ++j)
+                tma_load_3d_pair(sa + j * 8192, &tmAt, lbar, ra + j * 64, 0, T.seg);
+              for (int j = 0; j < b_boxes; ++j)
+                tma_load_3d_pair(sb + j * 8192, &tmBt, lbar, tb + j * 64, 0, T.seg);
+              continue;
+            }
             const int kk = T.k0 + kb * P.bk;
-            if (P.a_mn) {
+            if (!FP8 && P.a_mn) {
               for (int j = 0; j < 2; ++j)
                 tma_load_3d_pair(sa + j * 8192, &tmA, lbar, ra + j * 64, kk, ga);
             } else {
               tma_load_3d_pair(sa, &tmA, lbar, kk, ra, ga);
             }
-            if (P.b_mn) {
+            if (!FP8 && P.b_mn) {
               for (int j = 0; j < b_boxes; ++j)
                 tma_load_3d_pair(sb + j * 8192, &tmB, lbar, tb + j * 64, kk, 0);
             } else {
@@ -336,49 +421,54 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     __syncwarp();
     if (P.split > 1) cluster_sync_all();
   } else if (warp == 1) {
-    // ---------------- MMA issuer (even CTA) ----------------
-    if (lane == 0 && leader) {
+    // ---------------- MMA issuer (even CTA, whole warp) ----------------
+    if (leader) {
       int stage = 0, cur = 0;
       uint32_t phase = 0;
-      uint32_t unit = 0;  // accumulator uses so far
-      const uint64_t a_step = P.a_mn ? 128 : 2, b_step = P.b_mn ? 128 : 2;
+      uint32_t half = 0, hphase = 0;
+      const uint32_t elected = elect_one();
+      const bool a_mn = !FP8 && P.a_mn, b_mn = !FP8 && P.b_mn;
+      const uint32_t a_step = a_mn ? 128 : 2, b_step = b_mn ? 128 : 2;
+      const uint64_t a_desc = a_mn ? smem_desc_mn(0, 8192) : make_smem_desc(0);
+      const uint64_t b_desc = b_mn ? smem_desc_mn(0, 8192) : make_smem_desc(0);
+      const uint32_t a_hi = (uint32_t)(a_desc >> 32), b_hi = (uint32_t)(b_desc >> 32);
+      // offset within this CTA: the address carries the CTA's rank above bit 18
+      const uint32_t ring = (smem_u32(smem) & 0x3FFFFu) >> 4;
+      const uint32_t a_lo0 = (uint32_t)a_desc + ring, b_lo0 = (uint32_t)b_desc + ring + (GG_A_STAGE >> 4);
+      const uint32_t empty0 = smem_u32(&empty_bar[0]);
+      const uint32_t tfull0 = smem_u32(&tfull_bar[0]);
       for (int tile = cluster_id; tile < total && !fail; tile += num_clusters) {
         const TileAt T = gg_tile<FP8>(P, S, nseg, tile, cur);
-        const int kb0 = share_of(T.nkb, part, P.split), kb1 = share_of(T.nkb, part + 1, P.split);
-        const uint32_t idesc = P.idesc | ((uint32_t)(T.n >> 3) << 17);
-        for (int kb = kb0; kb < kb1; ++kb) {
-          const uint32_t buf = unit & 1u;
-          if (FP8 || kb == kb0) {
-            if (!mbar_wait(&tempty_bar[buf], ((unit >> 1) & 1u) ^ 1u, abortp)) { fail = 2; break; }
+        const int nkb = __shfl_sync(0xffffffffu, T.nkb, 0);
+        const int kb0 = share_of(nkb, part, P.split), kb1 = share_of(nkb, part + 1, P.split);
+        const uint32_t idesc = P.idesc | ((uint32_t)(__shfl_sync(0xffffffffu, T.n, 0) >> 3) << 17);
+        int in_half = 0;  // accumulators of the current half already filled
+        for (int ks = kb0; ks < kb1; ks += GG_KS) {
+          if (!warp_wait(&full_bar[stage], phase, abortp)) { fail = 2; break; }
+          const int ke = min(ks + GG_KS, kb1);
+          uint32_t slab = (uint32_t)(stage * stage_bytes) >> 4;
+          for (int kb = ks; kb < ke; ++kb, slab += (uint32_t)slab_bytes >> 4) {
+            if (FP8 ? in_half == 0 : kb == kb0) {
+              if (!warp_wait(&tempty_bar[half], hphase ^ 1u, abortp)) { fail = 2; break; }
+            }
+            tc_fence_after();
+            gg_mma4<FP8>(elected, tmem_base + half * 256u + (FP8 ? in_half * P.buf_cols : 0),
+                         a_lo0 + slab, a_hi, b_lo0 + slab, b_hi, a_step, b_step, idesc,
+                         (!FP8 && kb > kb0) ? 1u : 0u);
+            const bool last = kb + 1 == kb1;
+            if (FP8 ? (++in_half == P.half_kb || last) : last) {
+              gg_commit(elected, tfull0 + half * 8, lead);
+              in_half = 0;
+              half ^= 1u;
+              if (half == 0) hphase ^= 1u;
+            }
           }
-          if (!mbar_wait(&full_bar[stage], phase, abortp)) { fail = 2; break; }
-          tc_fence_after();
-          const uint32_t sa = smem_u32(smem + stage * stage_bytes), sb = sa + GG_A_STAGE;
-          const uint64_t ad = P.a_mn ? smem_desc_mn(sa, 8192) : make_smem_desc(sa);
-          const uint64_t bd = P.b_mn ? smem_desc_mn(sb, 8192) : make_smem_desc(sb);
-          const uint32_t d = tmem_base + buf * 256u;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            gg_mma(FP8, d, ad + a_step * k, bd + b_step * k, idesc,
-                   (k > 0 || (!FP8 && kb > kb0)) ? 1u : 0u);
-          // delivered to both CTAs of this pair
-          asm volatile(
-              "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
-              " [%0], %1;" ::"r"(smem_u32(&empty_bar[stage])),
-              "h"((uint16_t)(3u << lead))
-              : "memory");
-          if (FP8 || kb + 1 == kb1) {
-            asm volatile(
-                "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
-                " [%0], %1;" ::"r"(smem_u32(&tfull_bar[buf])),
-                "h"((uint16_t)(3u << lead))
-                : "memory");
-            ++unit;
-          }
+          if (fail) break;
+          gg_commit(elected, empty0 + stage * 8, lead);
           if (++stage == P.stages) { stage = 0; phase ^= 1; }
         }
       }
-      if (fail) {
+      if (fail && lane == 0) {
         *abortp = 1;
         st_cluster_u32(peer_abort, 1u);
         if (P.status) atomicCAS(P.status, 0, 2);
@@ -387,38 +477,141 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     __syncwarp();
     if (P.split > 1) cluster_sync_all();
   } else {
+    // ---------------- scales, ahead of the epilogue (one warp) ----------------
+    // A load issued by the epilogue warps a slab ahead put a memory round trip on
+    // every 128-block (0.7 us a slab on the 8192 x 28672 decode, 90 us in all).
+    if (FP8 && warp == 2) {
+      int slot = 0, cur = 0;
+      uint32_t phase = 0;
+      for (int tile = cluster_id; tile < total && !fail; tile += num_clusters) {
+        const TileAt T = gg_tile<FP8>(P, S, nseg, tile, cur);
+        const int kb0 = share_of(T.nkb, part, P.split), kb1 = share_of(T.nkb, part + 1, P.split);
+        const int64_t kabs = T.k0 / 128 + kb0;
+        const int row = min(T.r0 + (int)rank * 128, P.r - 1);
+        const float* pa = P.a_scale + (P.mode == 0 ? (int64_t)T.seg * P.sa_g : 0) + kabs * P.sa_k +
+                          (int64_t)(A_ROW ? row : row >> 7) * P.sa_r;
+        const float* pb = P.b_scale + kabs * P.sb_k + T.t0;
+        const int rows = A_ROW ? min(128, P.r - row) : 1;
+        for (int kb = kb0; kb < kb1; kb += GG_BATCH) {
+          const int ok = mbar_wait(&sempty_bar[slot], phase ^ 1, abortp) ? 1 : 0;
+          if (!__all_sync(0xffffffffu, ok)) { fail = 4; break; }
+          const int m = min(GG_BATCH, kb1 - kb);
+          for (int b = 0; b < m; ++b) {
+            const uint32_t dst = smem_u32(slots + (slot * GG_BATCH + b) * GG_SLOT);
+            for (int c = lane; c < T.tvalid; c += 32)
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + c * 4), "l"(pb + c)
+                           : "memory");
+            for (int c = lane; c < rows; c += 32)
+              asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst + (256 + c) * 4),
+                           "l"(pa + c * P.sa_r)
+                           : "memory");
+            pa += P.sa_k;
+            pb += P.sb_k;
+          }
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(
+                           smem_u32(&sfull_bar[slot]))
+                       : "memory");
+          if (++slot == GG_SLOTS) { slot = 0; phase ^= 1; }
+        }
+      }
+      if (fail && lane == 0) {
+        *abortp = 1;
+        st_cluster_u32(peer_abort, 1u);
+        if (P.status) atomicCAS(P.status, 0, 4);
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    }
+    __syncwarp();
     if (P.split > 1) cluster_sync_all();
   }
   } else {
     // ---------------- epilogue (both CTAs, own 128 rows) ----------------
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 " GG_REGS_MANY ";");
+    if constexpr (SLICES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    else if constexpr (SLICES == 3) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
+    else if constexpr (FP8) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    // A warp reads its 32 rows by COLS columns with 16x256b loads: a thread then
+    // holds, of every 8 columns, two neighbouring ones in four rows,
+    //   acc[g][h][i]: column 8 g + 2 (lane % 4) + i % 2, row 16 h + lane / 4 + 8 (i / 2),
+    // so a column's scale serves four of its elements. (With one row a thread
+    // every element needs a factor of its own from shared memory, and those
+    // reads, 512 bytes to a warp each, took longer than the MMAs.)
+    constexpr int GROUPS = COLS / 8;
+    constexpr int HALF_KB = SLICES > 2 ? 1 : 128 / COLS;  // = P.half_kb
+    constexpr int LOADS = 32;                              // columns read at once
     const int quarter = warp & 3;
-    const int c0 = ((warp - 4) >> 2) * GG_COLS;  // first column of this warp
-    float* const fac = (float*)(smem + P.stages * stage_bytes) + (warp - 4) * GG_COLS;
-    uint32_t unit = 0;
-    int cur = 0;
+    const int c0 = ((warp - 4) >> 2) * COLS;  // first column of this warp
+    uint32_t half = 0, hphase = 0;
+    int slot = 0, cur = 0;
+    uint32_t sphase = 0;
     bool have = false;
-    float acc[GG_COLS];
+    float acc[GROUPS][2][4];
     const uint32_t tlane = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c0;
+    const uint32_t tempty0 = map_to_cta(smem_u32(&tempty_bar[0]), lead);
+    uint8_t* const stage_out = (uint8_t*)(slots + GG_SCALE_BYTES / 4) + (warp - 4) * GG_STAGE_OUT;
     // The place in the output is worked out anew (`again` hides that from the
     // compiler): kept across the contraction it would cost registers there.
     auto store = [&](int again) {
       asm volatile("" : "+r"(again));
       const TileAt T = gg_tile<FP8>(P, S, nseg, again, cur);
-      const int r = T.r0 + (int)rank * 128 + quarter * 32 + lane;
-      if (r < P.r) {
-        const int64_t at = (P.mode == 1 ? (int64_t)T.seg * P.o_g : 0) + (int64_t)(T.t0 + c0) * P.o_ld + r;
-        const int m = T.tvalid - c0;
-        if (P.out_f32) {
-          float* o = (float*)P.out + at;
+      const int r0 = T.r0 + (int)rank * 128 + quarter * 32;
+      const int m = T.tvalid - c0;
+      const int64_t at = (P.mode == 1 ? (int64_t)T.seg * P.o_g : 0) + (int64_t)(T.t0 + c0) * P.o_ld + r0;
+      if (P.out_staged) {
+        // bf16, aligned rows: eight columns at a time are turned round by a
+        // transposing matrix store and leave as 64-byte pieces of output rows
+        const uint32_t st = smem_u32(stage_out);
+        // 16-byte piece `lane / 8` of row `lane % 8`, XOR-ed so that pieces of
+        // neighbouring rows lie in different banks
+        const uint32_t put = st + (lane & 7) * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4);
+        const int col = lane >> 2, piece = lane & 3;
+        const uint8_t* get = stage_out + col * 64 + ((piece ^ ((col >> 1) & 3)) << 4);
+        const int left = P.r - r0 - piece * 8;
+        __nv_bfloat16* o = (__nv_bfloat16*)P.out + at + (int64_t)col * P.o_ld + piece * 8;
 #pragma unroll
-          for (int j = 0; j < GG_COLS; ++j)
-            if (j < m) o[j * P.o_ld] = acc[j];
-        } else {
-          __nv_bfloat16* o = (__nv_bfloat16*)P.out + at;
+        for (int g = 0; g < GROUPS; ++g) {
+          if (g * 8 >= m) break;
+          uint32_t w[4];
 #pragma unroll
-          for (int j = 0; j < GG_COLS; ++j)
-            if (j < m) o[j * P.o_ld] = __float2bfloat16_rn(acc[j]);
+          for (int q = 0; q < 4; ++q) {  // rows 8 q .. 8 q + 7
+            const __nv_bfloat162 v =
+                __floats2bfloat162_rn(acc[g][q >> 1][(q & 1) * 2], acc[g][q >> 1][(q & 1) * 2 + 1]);
+            w[q] = *(const uint32_t*)&v;
+          }
+          asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(put),
+                       "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                       : "memory");
+          __syncwarp();
+          const uint4 v = *(const uint4*)get;
+          __syncwarp();
+          if (g * 8 + col < m && left > 0) {
+            if (left >= 8) {
+              *(uint4*)o = v;
+            } else {
+              const uint16_t* e = (const uint16_t*)&v;
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                if (q < left) ((uint16_t*)o)[q] = e[q];
+            }
+          }
+          o += 8 * P.o_ld;
+        }
+      } else {
+        const int r = lane >> 2, c = (lane & 3) * 2;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int rr = 16 * h + r + 8 * (i >> 1), cc = 8 * g + c + (i & 1);
+              if (cc < m && r0 + rr < P.r) {
+                const int64_t x = at + (int64_t)cc * P.o_ld + rr;
+                if (P.out_f32) ((float*)P.out)[x] = acc[g][h][i];
+                else ((__nv_bfloat16*)P.out)[x] = __float2bfloat16_rn(acc[g][h][i]);
+              }
+            }
+          }
         }
       }
     };
@@ -428,73 +621,103 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       const int kb0 = share_of(T.nkb, part, P.split), kb1 = share_of(T.nkb, part + 1, P.split);
       const int cols = T.n - c0;  // this warp's columns that the MMAs write
 #pragma unroll
-      for (int j = 0; j < GG_COLS; ++j) acc[j] = 0.f;
-      const float* pa = nullptr;
-      const float* pb = nullptr;
-      if constexpr (FP8) {
-        const int64_t kabs = T.k0 / 128 + kb0;
-        const int row = min(T.r0 + (int)rank * 128 + (A_ROW ? quarter * 32 + lane : 0), P.r - 1);
-        pa = P.a_scale + (P.mode == 0 ? (int64_t)T.seg * P.sa_g : 0) + kabs * P.sa_k +
-             (int64_t)(A_ROW ? row : row >> 7) * P.sa_r;
-        pb = P.b_scale + kabs * P.sb_k + T.t0 + c0 + lane;
-      }
-      float na = 0.f, nb[4] = {0.f, 0.f, 0.f, 0.f};  // scales of the next slab
-      auto scales = [&]() {
-        const int m = T.tvalid - c0 - lane;
-        na = __ldg(pa);
+      for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) nb[q] = m > 32 * q ? __ldg(pb + 32 * q) : 0.f;
-        pa += P.sa_k;
-        pb += P.sb_k;
-      };
-      if (FP8 && kb0 < kb1) scales();
-      for (int kb = kb0; kb < kb1; kb = FP8 ? kb + 1 : kb1) {
-        const uint32_t buf = unit & 1u;
-        float fa = 1.f;
-        if constexpr (FP8) {
-          __syncwarp();
-#pragma unroll
-          for (int q = 0; q < 4; ++q) fac[lane + 32 * q] = A_ROW ? nb[q] : nb[q] * na;
-          fa = na;
-          __syncwarp();
-          if (kb + 1 < kb1) scales();
+        for (int i = 0; i < 8; ++i) acc[g][i >> 2][i & 3] = 0.f;
+      int in_batch = 0;  // slabs of the current batch of scales already used
+      for (int kb = kb0; kb < kb1;) {
+        if (FP8 && in_batch == 0) {
+          const int got = mbar_wait(&sfull_bar[slot], sphase, abortp) ? 1 : 0;
+          if (!__all_sync(0xffffffffu, got)) { fail = 3; break; }
         }
-        int ok = mbar_wait(&tfull_bar[buf], (unit >> 1) & 1u, abortp) ? 1 : 0;
+        float2 f[GROUPS];  // this thread's two column scales of every 8 columns
+        float ra[4];       // its four row scales, or the one of the whole block
+        const float* sc = slots + (slot * GG_BATCH + in_batch) * GG_SLOT;
+        auto factors = [&]() {
+          if constexpr (A_ROW) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) ra[q] = sc[256 + quarter * 32 + (lane >> 2) + 8 * q];
+          } else {
+            ra[0] = sc[256];
+          }
+#pragma unroll
+          for (int g = 0; g < GROUPS; ++g) {
+            f[g] = *(const float2*)(sc + c0 + g * 8 + (lane & 3) * 2);
+            if constexpr (!A_ROW) {
+              f[g].x *= ra[0];
+              f[g].y *= ra[0];
+            }
+          }
+        };
+        if (FP8 && HALF_KB == 1) factors();  // while the MMAs still run
+        int ok = mbar_wait(&tfull_bar[half], hphase, abortp) ? 1 : 0;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) { fail = 3; break; }
         tc_fence_after();
+        auto hand_back = [&]() {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(tempty0 + half * 8);
+        };
+        const int here = FP8 && HALF_KB > 1 ? min(HALF_KB, kb1 - kb) : 1;  // accumulators in this half
         if (cols > 0) {
-          uint32_t v[2][16];
-          tc_ld16(tlane + buf * 256u, v[0]);
+          uint32_t ta = tlane + half * 256u;
+          for (int b = 0; b < here; ++b, ta += P.buf_cols, sc += GG_SLOT) {
+            if (FP8 && HALF_KB > 1) factors();
 #pragma unroll
-          for (int c = 0; c < GG_COLS / 16; ++c) {
-            if (c * 16 >= cols) break;  // the same for the whole warp
-            tc_wait_ld();
-            if ((c + 1) * 16 < cols && c + 1 < GG_COLS / 16)
-              tc_ld16(tlane + buf * 256u + (c + 1) * 16, v[(c + 1) & 1]);
-            const uint32_t* p = v[c & 1];
-            if constexpr (FP8) {
+            for (int c = 0; c < COLS; c += LOADS) {
+              if (c >= cols) break;  // the same for the whole warp
+              uint32_t p[LOADS / 32][2][16];
 #pragma unroll
-              for (int j = 0; j < 16; j += 4) {
-                const float4 f = *(const float4*)(fac + c * 16 + j);
-                const float fs[4] = {f.x, f.y, f.z, f.w};
+              for (int q = 0; q < LOADS / 32; ++q) {
+                tc_ld_16x256(ta + c + 32 * q, p[q][0]);
+                tc_ld_16x256(ta + c + 32 * q + (16u << 16), p[q][1]);
+              }
+              tc_wait_ld();
+              if constexpr (LOADS == COLS) {
+                // everything is in registers: hand the accumulators back before
+                // the arithmetic
+                if (b + 1 == here) hand_back();
+              }
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                  const float w = __uint_as_float(p[j + q]);
-                  acc[c * 16 + j + q] = A_ROW ? fmaf(w * fs[q], fa, acc[c * 16 + j + q])
-                                              : fmaf(w, fs[q], acc[c * 16 + j + q]);
+              for (int g = 0; g < LOADS / 8; ++g) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                  for (int i = 0; i < 4; i += 2) {
+                    float* a = &acc[c / 8 + g][h][i];
+                    float x = __uint_as_float(p[g / 4][h][g % 4 * 4 + i]);
+                    float y = __uint_as_float(p[g / 4][h][g % 4 * 4 + i + 1]);
+                    if constexpr (!FP8) {
+                      a[0] = x;
+                      a[1] = y;
+                    } else {
+                      if constexpr (A_ROW) {
+                        x *= ra[h * 2 + (i >> 1)];
+                        y *= ra[h * 2 + (i >> 1)];
+                      }
+                      fma2(a[0], a[1], x, y, f[c / 8 + g].x, f[c / 8 + g].y);
+                    }
+                  }
                 }
               }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 16; ++j) acc[c * 16 + j] = __uint_as_float(p[j]);
             }
           }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(map_to_cta(smem_u32(&tempty_bar[buf]), lead));
-        ++unit;
+        if (LOADS != COLS || cols <= 0) hand_back();
+        half ^= 1u;
+        if (half == 0) hphase ^= 1u;
+        if constexpr (FP8) {
+          kb += here;
+          in_batch += here;
+          if (in_batch == GG_BATCH || kb == kb1) {
+            if (lane == 0) mbar_arrive(&sempty_bar[slot]);
+            if (++slot == GG_SLOTS) { slot = 0; sphase ^= 1u; }
+            in_batch = 0;
+          }
+        } else {
+          kb = kb1;
+        }
       }
       if (fail) break;
       if (P.split == 1) store(tile);
@@ -502,20 +725,31 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     if (P.split > 1) {
       // Parts of one tile: parts 1.. leave their sums in their own shared memory
       // (the operand ring is idle by now), part 0 adds them in part order.
-      float* mine = (float*)smem + (size_t)c0 * 128 + quarter * 32 + lane;
-      if (have && !fail && part > 0 && c0 < P.nt) {
+      float4* mine = (float4*)smem + (warp - 4) * (GROUPS * 2 * 32) + lane;
+      const bool busy = have && !fail && c0 < P.nt;
+      if (busy && part > 0) {
 #pragma unroll
-        for (int j = 0; j < GG_COLS; ++j)
-          if (c0 + j < P.nt) mine[j * 128] = acc[j];
+        for (int g = 0; g < GROUPS * 2; ++g) {
+          const float* a = acc[g >> 1][g & 1];
+          mine[g * 32] = make_float4(a[0], a[1], a[2], a[3]);
+        }
       }
       __syncwarp();
       cluster_sync_all();
-      if (have && !fail && part == 0 && c0 < P.nt) {
+      if (busy && part == 0) {
         for (int p = 1; p < P.split; ++p) {
           const uint32_t from = map_to_cta(smem_u32(mine), 2 * p + rank);
+          float4 v[GROUPS * 2];
 #pragma unroll
-          for (int j = 0; j < GG_COLS; ++j)
-            if (c0 + j < P.nt) acc[j] += ld_cluster_f32(from + j * 512);
+          for (int g = 0; g < GROUPS * 2; ++g) v[g] = ld_cluster_f32x4(from + g * 512);
+#pragma unroll
+          for (int g = 0; g < GROUPS * 2; ++g) {
+            float* a = acc[g >> 1][g & 1];
+            a[0] += v[g].x;
+            a[1] += v[g].y;
+            a[2] += v[g].z;
+            a[3] += v[g].w;
+          }
         }
         store(cluster_id);
       }
@@ -645,17 +879,18 @@ static int operand_map(CUtensorMap* tm, const void* ptr, bool fp8, int64_t inner
 
 static bool is_fp8_dtype(int dt) { return dt == AQTB200_E4M3 || dt == AQTB200_E5M2; }
 
-// Columns of a tile. A group of `len` rows costs ceil(len / nt) passes over its
-// weights, an MMA's time goes with its columns.
-static int choose_nt(int64_t len, int64_t r_tiles, bool one_group, int pairs) {
-  if (len <= 256) return (int)std::max<int64_t>(32, (len + 31) / 32 * 32);
-  if (!one_group) return 256;
-  // one group, all sizes known: the width whose waves cost least in total
-  int best = 256;
-  double least = 1e300;
-  for (int nt = 256; nt >= 160; nt -= 32) {
+// Columns of a tile, at most `most`. A group of `len` rows costs ceil(len / nt)
+// passes over its weights, an MMA's time goes with its columns, and each tile has
+// a cost of its own that goes with neither (`extra`, in columns).
+static int choose_nt(int64_t len, int64_t r_tiles, bool one_group, int pairs, int most, int extra) {
+  if (len <= most) return (int)std::max<int64_t>(32, (len + 31) / 32 * 32);
+  if (!one_group) return most;
+  // one group, all sizes known: the width whose rounds cost least in total
+  int best = most;
+  int64_t least = INT64_MAX;
+  for (int nt = most; nt >= 160; nt -= 32) {
     const int64_t tiles = r_tiles * ((len + nt - 1) / nt);
-    const double cost = (double)((tiles + pairs - 1) / pairs) * (nt + 8);
+    const int64_t cost = (tiles + pairs - 1) / pairs * (nt + extra);
     if (cost < least) { least = cost; best = nt; }
   }
   return best;
@@ -703,19 +938,30 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   P.num_kb = (int)((k + P.bk - 1) / P.bk);
   const int pairs = std::max(1, sm_count() / 2);
   const int64_t len = P.mode == 0 ? (d->t + groups - 1) / groups : d->t;
-  // uneven groups: room for one and a half times the average before a second pass
-  P.nt = choose_nt(grouped && P.mode == 0 ? len + len / 2 : len, P.r_tiles, !grouped, pairs);
+  // Row scales on both sides double the epilogue's arithmetic: its threads need
+  // more registers than a 256-column tile leaves them (8192 x 4096 x 14336 drhs,
+  // 192 columns 0.82 ms, 256 columns 0.98 ms; forward the other way round, 0.64
+  // against 0.60 ms).
+  const bool a_row = fp8 && !d->a_scale_square;
+  // Uneven groups: room for one and a half times the average before a second
+  // pass. fp8 hands over an accumulator per 128-block, bf16 one per tile.
+  P.nt = choose_nt(grouped && P.mode == 0 ? len + len / 2 : len, P.r_tiles, !grouped, pairs,
+                   a_row ? 192 : 256, fp8 ? 80 : 8);
   P.t_tiles = (int)((d->t + P.nt - 1) / P.nt);
   const uint32_t fa = fp8 ? (d->a_dtype == AQTB200_E5M2) : 1, fb = fp8 ? (d->b_dtype == AQTB200_E5M2) : 1;
   P.idesc = (1u << 4) | (fa << 7) | (fb << 10) | ((uint32_t)P.a_mn << 15) | ((uint32_t)P.b_mn << 16) |
             (16u << 24);
   P.b_stage = P.b_mn ? (P.nt / 2 + 63) / 64 * 8192 : P.nt / 2 * 128;
-  P.stages = std::min(GG_MAX_STAGES, GG_RING / (GG_A_STAGE + P.b_stage));
+  P.stages = std::min(GG_MAX_STAGES, GG_RING / (GG_KS * (GG_A_STAGE + P.b_stage)));
+  P.buf_cols = P.nt <= 64 ? 64 : P.nt <= 128 ? 128 : 256;
+  P.half_kb = 256 / P.buf_cols;
   P.a_scale = d->a_scale; P.sa_g = d->a_scale_group_stride; P.sa_k = d->a_scale_k_stride;
   P.sa_r = d->a_scale_r_stride;
   P.b_scale = d->b_scale; P.sb_k = d->b_scale_k_stride;
   P.out = d->out; P.out_f32 = d->out_dtype == AQTB200_F32;
   P.o_ld = d->out_ld; P.o_g = d->out_group_stride;
+  P.out_staged = !P.out_f32 && ((uintptr_t)d->out & 15) == 0 && d->out_ld % 8 == 0 &&
+                 (P.mode == 0 || !grouped || d->out_group_stride % 8 == 0);
   P.status = status;
 
   // Tiles, or the most there can be: groups that end inside a tile add one each.
@@ -769,13 +1015,15 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
     if (rc) return rc;
   }
 
-  const size_t smem = (size_t)P.stages * (GG_A_STAGE + P.b_stage) + GG_F_BYTES + 1024;
-  const int64_t clusters = P.split > 1 ? tiles : std::min<int64_t>(tiles, pairs);
+  const size_t smem = GG_SMEM;
+  // Whole tiles round robin: the fewest pairs that keep the number of rounds.
+  const int64_t rounds = (tiles + pairs - 1) / pairs;
+  const int64_t clusters = P.split > 1 ? tiles : grouped ? std::min<int64_t>(tiles, pairs) : (tiles + rounds - 1) / rounds;
   int dev = 0;
   AQT_CUDA_OK(cudaGetDevice(&dev));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(clusters * 2 * P.split));
-  cfg.blockDim = dim3(GG_THREADS);
+  cfg.blockDim = dim3(gg_threads(P.nt <= 128 ? 2 : a_row ? 3 : 4));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -784,20 +1032,26 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-#define AQT_GG(F, R)                                                                                  \
-  do {                                                                                                \
-    static bool attr_done[64] = {false};                                                              \
-    if (!attr_done[dev & 63]) {                                                                       \
-      AQT_CUDA_OK(cudaFuncSetAttribute(grouped_gemm_kernel<F, R>,                                     \
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize,                   \
-                                       GG_RING + GG_F_BYTES + 1024));                                 \
-      attr_done[dev & 63] = true;                                                                     \
-    }                                                                                                 \
-    AQT_CUDA_OK(cudaLaunchKernelEx(&cfg, grouped_gemm_kernel<F, R>, tmA, tmB, tmAt, tmBt, P));        \
+#define AQT_GG(F, R, S, C)                                                                        \
+  do {                                                                                           \
+    static bool attr_done[64] = {false};                                                         \
+    if (!attr_done[dev & 63]) {                                                                  \
+      AQT_CUDA_OK(cudaFuncSetAttribute(grouped_gemm_kernel<F, R, S, C>,                             \
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)GG_SMEM)); \
+      attr_done[dev & 63] = true;                                                                \
+    }                                                                                            \
+    AQT_CUDA_OK(cudaLaunchKernelEx(&cfg, grouped_gemm_kernel<F, R, S, C>, tmA, tmB, tmAt, tmBt, P)); \
   } while (0)
-  if (!fp8) AQT_GG(false, false);
-  else if (d->a_scale_square) AQT_GG(true, false);
-  else AQT_GG(true, true);
+#define AQT_GG_C(F, R, S)                   \
+  do {                                      \
+    if (P.nt <= 64) AQT_GG(F, R, 2, 32);    \
+    else if (P.nt <= 128) AQT_GG(F, R, 2, 64); \
+    else AQT_GG(F, R, S, 64);               \
+  } while (0)
+  if (!fp8) AQT_GG_C(false, false, 4);
+  else if (!a_row) AQT_GG_C(true, false, 4);
+  else AQT_GG_C(true, true, 3);
+#undef AQT_GG_C
 #undef AQT_GG
   AQT_CUDA_OK(cudaGetLastError()); count_launch();
   return 0;
