@@ -12,20 +12,21 @@ quantized operand of this library; scales with the kept index contiguous):
   Blocks(x [R, C])  row   q [R][ld], scale [C/128][R]     blocks along C
                     col   q [C][ld], scale [R/128][C]     blocks along R
                     square: both orders of q, ONE scale [R/128][C/128]
+
+The calls here are short next to their kernels' launches, so what a product
+needs between its kernels is one torch allocation, addressed by offsets, and
+operands travel as (address, stride) numbers rather than as tensor views.
 """
 
 from __future__ import annotations
 
 import contextlib
 import ctypes as C
-import dataclasses
-from typing import Any
 
 import torch
 
 from aqt_b200 import _lib
 from aqt_b200 import engine
-from aqt_b200.v2 import utils
 
 BLOCK = 128
 _FLOATS = (torch.float32, torch.bfloat16)
@@ -42,6 +43,11 @@ def fp8_dtype(bits) -> torch.dtype:
     return bits
   raise NotImplementedError(
       f'block-scaled operands are e4m3 or e5m2 (got {bits!r})')
+
+
+def tracing():
+  """Whether an engine.TracedStep is recording."""
+  return engine._tape is not None  # pylint: disable=protected-access
 
 
 def on_device_of(x):
@@ -84,151 +90,190 @@ def check_group_sizes(group_sizes, groups):
         f'between 1 and {_lib.MAX_GROUPS} groups (got {groups})')
 
 
-def _up(v, m):
-  return (v + m - 1) // m * m
+class Side:
+  """One operand of a product: values with the contraction contiguous and their
+  scales, as addresses and strides. `keep` holds the memory."""
+  __slots__ = ('ptr', 'ld', 'group', 'code', 'scale', 'scale_group', 'scale_k',
+               'scale_r', 'kept', 'keep')
+
+  def __init__(self, ptr, ld, group, code, scale, scale_group, scale_k, scale_r,
+               kept, keep):
+    self.ptr, self.ld, self.group, self.code = ptr, ld, group, code
+    self.scale, self.scale_group = scale, scale_group
+    self.scale_k, self.scale_r = scale_k, scale_r
+    self.kept, self.keep = kept, keep
 
 
-def _cdiv(a, b):
-  return -(-a // b)
+def _align(n):
+  return (n + 255) & -256
 
 
-@dataclasses.dataclass(slots=True)
-class Blocks:
-  """One operand quantized in blocks (see the module docstring)."""
-  rows: int
-  cols: int
-  dtype: torch.dtype
-  square: bool = False
-  row: Any = None
-  row_scale: Any = None
-  col: Any = None
-  col_scale: Any = None
-  groups: int = 0  # matrices [groups][...]; 0: a single one
+def quantize(x, dtype, row=True, col=False, square=False, po2=False,
+             group_sizes=None):
+  """Quantizes a matrix [R, C] or matrices [G, R, C] in blocks of 128.
 
-  def tensors(self):
-    return [t for t in (self.row, self.row_scale, self.col, self.col_scale)
-            if t is not None]
-
-
-def quantize(x, dtype, *, row=True, col=False, square=False, po2=False,
-             group_sizes=None) -> Blocks:
-  """Quantizes a matrix [R, C] or matrices [G, R, C] in blocks of 128."""
-  dev = x.device
-  batch = x.shape[0] if x.ndim == 3 else 1
-  r, c = x.shape[-2:]
-  bs = x.stride(0) if x.ndim == 3 else 0
-  rs, cs = x.stride(-2), x.stride(-1)
+  Returns (row, col) Sides: the first contracts C, the second contracts R; None
+  where not asked for.
+  """
+  code = engine._TORCH_CODE  # pylint: disable=protected-access
+  shape, strides = x.shape, x.stride()
+  if x.ndim == 3:
+    batch, r, c = shape
+    bs, rs, cs = strides
+  else:
+    r, c = shape
+    rs, cs = strides
+    batch, bs = 1, 0
   # A transposed view is read the way it lies in memory: its rows are then the
   # columns of the call, and the two outputs change places.
   swap = cs != 1 and rs == 1 and group_sizes is None
   if swap:
     r, c, rs, cs, row, col = c, r, cs, rs, col, row
-  lead = (batch,) if x.ndim == 3 else ()
-  nr, nc = _cdiv(r, BLOCK), _cdiv(c, BLOCK)
-  out = Blocks(x.shape[-2], x.shape[-1], dtype, square,
-               groups=batch if x.ndim == 3 else 0)
-  empty = engine._empty  # pylint: disable=protected-access
-  q_row = q_col = s_row = s_col = None
-  ld_row, ld_col = _up(c, 16), _up(r, 16)
+  nr, nc = -(-r // BLOCK), -(-c // BLOCK)
+  ld_row = ld_col = groups = int64 = sizes_ptr = 0
   row_blocks = nr
   if group_sizes is not None:
     # every group may end in a partial block
-    row_blocks = r // BLOCK + min(group_sizes.shape[0], r)
-    ld_col = row_blocks * BLOCK
+    groups = group_sizes.shape[0]
+    row_blocks = r // BLOCK + min(groups, r)
+    int64 = int(group_sizes.dtype == torch.int64)
+    sizes_ptr = group_sizes.data_ptr()
+  at_q_row = at_s_row = at_q_col = at_s_col = end = 0
   if row:
-    q_row = empty((*lead, r, ld_row), torch.uint8, dev)
-    if not square:
-      s_row = empty((*lead, nc, r), torch.float32, dev)
+    ld_row = (c + 15) & -16
+    end = _align(batch * r * ld_row)
+  if square:
+    at_s_row = end
+    end += _align(batch * nr * nc * 4)
+  elif row:
+    at_s_row = end
+    end += _align(batch * nc * r * 4)
   if col:
-    q_col = empty((*lead, c, ld_col), torch.uint8, dev)
+    at_q_col = end
+    ld_col = (r + 15) & -16 if group_sizes is None else row_blocks * BLOCK
+    end += _align(batch * c * ld_col)
     if not square:
-      s_col = empty((*lead, row_blocks, c), torch.float32, dev)
-  if square:
-    s_row = empty((*lead, nr, nc), torch.float32, dev)
-  ptr = lambda t: None if t is None else t.data_ptr()
+      at_s_col = end
+      end += _align(batch * row_blocks * c * 4)
+  ws = engine._empty((end,), torch.uint8, x.device)  # pylint: disable=protected-access
+  base = ws.data_ptr()
   desc = _lib.BlockQuantDesc(
-      _lib.View(x.data_ptr(), engine._TORCH_CODE[x.dtype], 0, batch, 1, r, c,  # pylint: disable=protected-access
-                bs, 0, rs, cs),
-      engine._TORCH_CODE[dtype], int(po2), int(square),  # pylint: disable=protected-access
-      int(group_sizes is not None and group_sizes.dtype == torch.int64),
-      ptr(q_row), ld_row, ptr(s_row), ptr(q_col), ld_col, ptr(s_col),
-      ptr(group_sizes), 0 if group_sizes is None else group_sizes.shape[0])
-  _lib.check(engine._call(  # pylint: disable=protected-access
+      _lib.View(x.data_ptr(), code[x.dtype], 0, batch, 1, r, c, bs, 0, rs, cs),
+      code[dtype], po2, square, int64,
+      base + at_q_row if row else None, ld_row,
+      base + at_s_row if row or square else None,
+      base + at_q_col if col else None, ld_col,
+      base + at_s_col if col and not square else None, sizes_ptr, groups)
+  _check(engine._call(  # pylint: disable=protected-access
       _lib.load().aqtb200_block_quantize, C.byref(desc), engine._stream()),  # pylint: disable=protected-access
-             'block_quantize')
+         'block_quantize')
+  q = code[dtype]
+  a = b = None
+  if row:
+    s = ((base + at_s_row, nr * nc, 1, nc) if square else
+         (base + at_s_row, nc * r, r, 1))
+    a = Side(base + at_q_row, ld_row, r * ld_row, q, *s, r, ws)
+  if col:
+    s = ((base + at_s_row, nr * nc, nc, 1) if square else
+         (base + at_s_col, row_blocks * c, c, 1))
+    b = Side(base + at_q_col, ld_col, c * ld_col, q, *s, c, ws)
+  return (b, a) if swap else (a, b)
+
+
+def quantize_tensors(x, dtype, axis, square, po2):
+  """Quantizes x for one contraction axis (-1 or -2) into tensors of their own:
+  (values of x's shape, scales as the QTensor's user sees them)."""
+  code = engine._TORCH_CODE  # pylint: disable=protected-access
+  empty = engine._empty  # pylint: disable=protected-access
+  lead, (r, c) = tuple(x.shape[:-2]), x.shape[-2:]
+  batch, bs = (lead[0], x.stride(0)) if lead else (1, 0)
+  rs, cs = x.stride(-2), x.stride(-1)
+  row = axis == -1
+  swap = cs != 1 and rs == 1
   if swap:
-    q_row, q_col = q_col, q_row
-    if square:
-      s_row = s_row.transpose(-1, -2)
-    else:
-      s_row, s_col = s_col, s_row
-  out.row, out.row_scale, out.col, out.col_scale = q_row, s_row, q_col, s_col
+    r, c, rs, cs, row = c, r, cs, rs, not row
+  nr, nc = -(-r // BLOCK), -(-c // BLOCK)
+  kept, contracted = (r, c) if row else (c, r)
+  ld = (contracted + 15) & -16
+  if ld == contracted:
+    q = view = empty((*lead, kept, ld), dtype, x.device)
+  else:
+    q = empty((*lead, kept, ld), torch.uint8, x.device)
+    view = q[..., :contracted].view(dtype)
   if square:
-    out.col_scale = s_row
-  return out
+    s = empty((*lead, nr, nc), torch.float32, x.device)
+  else:
+    s = empty((*lead, nc, r) if row else (*lead, nr, c), torch.float32, x.device)
+  qp, sp = q.data_ptr(), s.data_ptr()
+  desc = _lib.BlockQuantDesc(
+      _lib.View(x.data_ptr(), code[x.dtype], 0, batch, 1, r, c, bs, 0, rs, cs),
+      code[dtype], po2, square, 0, qp if row else None, ld,
+      sp if row or square else None, None if row else qp, ld,
+      None if row or square else sp, None, 0)
+  _check(engine._call(  # pylint: disable=protected-access
+      _lib.load().aqtb200_block_quantize, C.byref(desc), engine._stream()),  # pylint: disable=protected-access
+         'block_quantize')
+  # back to x's axes: values lie [kept][contracted], row scales [block][kept]
+  if axis == -2:
+    view = view.transpose(-1, -2)
+  if square:
+    s = s.transpose(-1, -2) if swap else s
+  elif row != swap:
+    s = s.transpose(-1, -2) if axis == -1 else s
+  else:
+    s = s if axis == -2 else s.transpose(-1, -2)
+  return view, s
+
+
+def _check(rc, what):
+  if rc:
+    _lib.check(rc, what)
 
 
 def _gemm(desc, device, what):
-  lib = _lib.load()
-  nbytes = lib.aqtb200_grouped_gemm_workspace_bytes(C.byref(desc))
-  if nbytes:
-    ws = engine._empty((nbytes,), torch.uint8, device)  # pylint: disable=protected-access
-    desc.workspace, desc.workspace_bytes = ws.data_ptr(), nbytes
-  _lib.check(engine._call(  # pylint: disable=protected-access
-      lib.aqtb200_grouped_gemm, C.byref(desc),
+  _check(engine._call(  # pylint: disable=protected-access
+      _lib.load().aqtb200_grouped_gemm, C.byref(desc),
       engine._status_buf(device).data_ptr(), engine._stream()), what)  # pylint: disable=protected-access
 
 
-def _sizes(desc, group_sizes):
-  if group_sizes is not None:
-    desc.group_sizes = group_sizes.data_ptr()
-    desc.groups = group_sizes.shape[0]
-    desc.sizes_int64 = int(group_sizes.dtype == torch.int64)
+def _sizes(group_sizes):
+  """(address, number, whether int64) for a descriptor."""
+  if group_sizes is None:
+    return None, 0, 0
+  return (group_sizes.data_ptr(), group_sizes.shape[0],
+          int(group_sizes.dtype == torch.int64))
 
 
 def _empty_out(shape, dtype, device):
   return engine._empty(shape, dtype, device)  # pylint: disable=protected-access
 
 
-def fp8_rows(tokens, tokens_scale, t, a, a_dtype, a_scale, r, k, b_dtype,
-             out_dtype, group_sizes=None):
-  """out[t][r] = sum_k b[t][k] a[g(t)][r][k], both block-scaled.
-
-  tokens: q [T][ld] with scale [k/128][T]; a: q [.., R][ld] with the square
-  scale given as a [.., R/128, k/128]-shaped view.
-  """
-  dev = tokens.device
-  out = _empty_out((t, r), out_dtype, dev)
-  code = engine._TORCH_CODE  # pylint: disable=protected-access
-  d = _lib.GroupedGemmDesc(
-      0, code[a_dtype], code[b_dtype], code[out_dtype], r, t, k, t,
-      a.data_ptr(), a.stride(-2), a.stride(0) if a.ndim == 3 else 0,
-      tokens.data_ptr(), tokens.stride(0), 0, 0, 1, 0,
-      a_scale.data_ptr(), a_scale.stride(0) if a_scale.ndim == 3 else 0,
-      a_scale.stride(-1), a_scale.stride(-2),
-      tokens_scale.data_ptr(), tokens_scale.stride(0), None, 0,
-      out.data_ptr(), r, 0, None, 0)
-  _sizes(d, group_sizes)
-  _gemm(d, dev, 'block-scaled product')
+def fp8_rows(tokens, a, k, out_dtype, device, group_sizes=None):
+  """out[t][r] = sum_k tokens[t][k] a[g(t)][r][k]; a has 128 x 128 blocks."""
+  t, r = tokens.kept, a.kept
+  out = _empty_out((t, r), out_dtype, device)
+  sizes, groups, int64 = _sizes(group_sizes)
+  _gemm(_lib.GroupedGemmDesc(
+      0, a.code, tokens.code, engine._TORCH_CODE[out_dtype], r, t, k, t,  # pylint: disable=protected-access
+      a.ptr, a.ld, a.group, tokens.ptr, tokens.ld, 0, 0, 1, int64,
+      a.scale, a.scale_group, a.scale_k, a.scale_r,
+      tokens.scale, tokens.scale_k, sizes, groups,
+      out.data_ptr(), r, 0, None, 0), device, 'block-scaled product')
   return out
 
 
-def fp8_contract_rows(b, b_scale, t, a, a_scale, r, k, rows, a_dtype, b_dtype,
-                      out_dtype, group_sizes=None):
+def fp8_contract_rows(b, a, k, rows, out_dtype, device, group_sizes=None):
   """out[g][t][r] = sum over the rows of group g: both operands are the
   transposed ("col") copies, blocks along the rows."""
-  dev = b.device
+  t, r = b.kept, a.kept
   lead = () if group_sizes is None else (group_sizes.shape[0],)
-  out = _empty_out((*lead, t, r), out_dtype, dev)
-  code = engine._TORCH_CODE  # pylint: disable=protected-access
-  d = _lib.GroupedGemmDesc(
-      1, code[a_dtype], code[b_dtype], code[out_dtype], r, t, k, rows,
-      a.data_ptr(), a.stride(0), 0, b.data_ptr(), b.stride(0), 0, 0, 0, 0,
-      a_scale.data_ptr(), 0, a_scale.stride(0), 1,
-      b_scale.data_ptr(), b_scale.stride(0), None, 0,
-      out.data_ptr(), r, t * r, None, 0)
-  _sizes(d, group_sizes)
-  _gemm(d, dev, 'block-scaled product')
+  out = _empty_out((*lead, t, r), out_dtype, device)
+  sizes, groups, int64 = _sizes(group_sizes)
+  _gemm(_lib.GroupedGemmDesc(
+      1, a.code, b.code, engine._TORCH_CODE[out_dtype], r, t, k, rows,  # pylint: disable=protected-access
+      a.ptr, a.ld, 0, b.ptr, b.ld, 0, 0, 0, int64,
+      a.scale, 0, a.scale_k, 1, b.scale, b.scale_k, sizes, groups,
+      out.data_ptr(), r, t * r, None, 0), device, 'block-scaled product')
   return out
 
 
@@ -248,7 +293,7 @@ def _fits(x, contiguous_axis, other_axis):
 
 def pack(x):
   """A copy of bf16 [.., R, C] with C contiguous and rows padded to 16 bytes."""
-  ld = _up(max(x.shape[-1], 1), 8)
+  ld = (max(x.shape[-1], 1) + 7) & -8
   batch = x.shape[0] if x.ndim == 3 else 1
   buf = _empty_out((*x.shape[:-1], ld), torch.bfloat16, x.device)
   v = _lib.View(x.data_ptr(), _lib.BF16, 0, batch, 1, x.shape[-2], x.shape[-1],
@@ -266,7 +311,7 @@ def rows_for_tma(x):
 
 def _ld(x, axis):
   """Stride of `axis`, made a valid one where the axis has a single entry."""
-  return x.stride(axis) if x.shape[axis] > 1 else _up(max(x.shape[-1], x.shape[-2]), 8)
+  return x.stride(axis) if x.shape[axis] > 1 else (max(x.shape[-1], x.shape[-2]) + 7) & -8
 
 
 def bf16_rows(tokens, a, contract_axis, group_sizes, out_dtype):
@@ -284,12 +329,12 @@ def bf16_rows(tokens, a, contract_axis, group_sizes, out_dtype):
   else:
     a = pack(a)  # its last axis is contiguous
     mn, ld = int(contract_axis == 1), a.stride(1)
-  d = _lib.GroupedGemmDesc(
+  sizes, groups, int64 = _sizes(group_sizes)
+  _gemm(_lib.GroupedGemmDesc(
       0, _lib.BF16, _lib.BF16, engine._TORCH_CODE[out_dtype], r, t, k, t,  # pylint: disable=protected-access
       a.data_ptr(), ld, a.stride(0), tokens.data_ptr(), _ld(tokens, 0), mn, 0,
-      0, 0, None, 0, 0, 0, None, 0, None, 0, out.data_ptr(), r, 0, None, 0)
-  _sizes(d, group_sizes)
-  _gemm(d, dev, 'grouped product')
+      0, int64, None, 0, 0, 0, None, 0, sizes, groups, out.data_ptr(), r, 0,
+      None, 0), dev, 'grouped product')
   return out
 
 
@@ -300,11 +345,16 @@ def bf16_contract_rows(lhs, g, group_sizes, out_dtype):
   dev = lhs.device
   out = _empty_out((group_sizes.shape[0], t, r), out_dtype, dev)
   lhs, g = rows_for_tma(lhs), rows_for_tma(g)
+  sizes, groups, int64 = _sizes(group_sizes)
   d = _lib.GroupedGemmDesc(
       1, _lib.BF16, _lib.BF16, engine._TORCH_CODE[out_dtype], r, t, rows, rows,  # pylint: disable=protected-access
-      g.data_ptr(), _ld(g, 0), 0, lhs.data_ptr(), _ld(lhs, 0), 1, 1, 0, 0,
-      None, 0, 0, 0, None, 0, None, 0, out.data_ptr(), r, t * r, None, 0)
-  _sizes(d, group_sizes)
+      g.data_ptr(), _ld(g, 0), 0, lhs.data_ptr(), _ld(lhs, 0), 1, 1, 0, int64,
+      None, 0, 0, 0, None, 0, sizes, groups, out.data_ptr(), r, t * r, None, 0)
+  # room for the groups' last, partial slabs
+  nbytes = _lib.load().aqtb200_grouped_gemm_workspace_bytes(C.byref(d))
+  if nbytes:
+    ws = engine._empty((nbytes,), torch.uint8, dev)  # pylint: disable=protected-access
+    d.workspace, d.workspace_bytes = ws.data_ptr(), nbytes
   _gemm(d, dev, 'grouped product')
   return out
 
@@ -316,18 +366,13 @@ class Residuals:
 
   __slots__ = ('stream', 'tensors')
 
-  def __init__(self, tensors, like):
-    self.tensors = [t for t in tensors if t is not None]
-    self.stream = torch.cuda.current_stream(like.device) if like.is_cuda else None
+  def __init__(self, *sides):
+    self.tensors = [s.keep for s in sides if s is not None]
+    self.stream = engine._stream()  # pylint: disable=protected-access
 
   def about_to_use(self):
-    if self.stream is None:
-      return
-    now = torch.cuda.current_stream(self.stream.device)
-    if now != self.stream:
+    """Called with the operands' device current."""
+    if engine._stream() != self.stream:  # pylint: disable=protected-access
       for t in self.tensors:
-        t.record_stream(now)
-
-
-def float_name(dtype):
-  return utils.as_dtype(dtype).name
+        if t.is_cuda:
+          t.record_stream(torch.cuda.current_stream())

@@ -55,7 +55,7 @@ def ragged_dot_vjp(lhs, rhs, group_sizes, cfg=None, preferred_element_type=None)
   out_dtype = _check(lhs, rhs, group_sizes, cfg, preferred_element_type)
   out, step = _forward(lhs.detach(), rhs.detach(), group_sizes, cfg, out_dtype,
                        (True, True))
-  return out, lambda g: _backward(step, g, (True, True))
+  return out, lambda g: _backward(step, g.detach(), (True, True))
 
 
 def _check(lhs, rhs, group_sizes, cfg, preferred):
@@ -89,14 +89,13 @@ class _Step:
 
 def _forward(lhs, rhs, sizes, cfg, out_dtype, grads):
   need_l, need_r = grads
+  step = None
   with be.on_device_of(lhs):
-    step = None
     if need_l or need_r:
       step = _Step()
       step.cfg, step.sizes = cfg, sizes
       step.lhs_dtype, step.rhs_dtype = lhs.dtype, rhs.dtype
       step.shape = (*lhs.shape, rhs.shape[2])
-      step.keep = None
     if cfg is None:
       out = be.bf16_rows(lhs, rhs, 1, sizes, out_dtype)
       if step is not None:
@@ -104,29 +103,23 @@ def _forward(lhs, rhs, sizes, cfg, out_dtype, grads):
         step.rhs = rhs if need_l else None
       return out, step
     if isinstance(rhs, aqt_tensor.QTensor):
-      a, a_scale, a_dtype = block_scaled._frozen_operand(rhs, -2)  # pylint: disable=protected-access
+      w, w_n = block_scaled._frozen_operand(rhs, -2), None  # pylint: disable=protected-access
     else:
-      w = be.quantize(rhs, cfg.fwd_dtype, row=need_l, col=True, square=True,
-                      po2=cfg.po2_scale)
-      a, a_scale, a_dtype = block_scaled._kept_major(w, -2)  # pylint: disable=protected-access
-    l = be.quantize(lhs, cfg.fwd_dtype, row=True, col=need_r, po2=cfg.po2_scale,
-                    group_sizes=sizes if need_r else None)
-    out = be.fp8_rows(l.row, l.row_scale, lhs.shape[0], a, a_dtype, a_scale,
-                      a.shape[-2], lhs.shape[1], cfg.fwd_dtype, out_dtype, sizes)
+      w_n, w = be.quantize(rhs, cfg.fwd_dtype, need_l, True, True, cfg.po2_scale)
+    l, l_t = be.quantize(lhs, cfg.fwd_dtype, True, need_r, False, cfg.po2_scale,
+                         sizes if need_r else None)
+    out = be.fp8_rows(l, w, lhs.shape[1], out_dtype, lhs.device, sizes)
     if step is not None:
-      if need_r:
-        l.row = l.row_scale = None
-      step.lhs = l if need_r else None
-      step.rhs = w if need_l else None
-      step.keep = be.Residuals(
-          (l.tensors() if need_r else []) + (w.tensors() if need_l else []), lhs)
-    return out, step
+      step.lhs, step.rhs = l_t, w_n if need_l else None
+      step.keep = be.Residuals(step.lhs, step.rhs)
+  return out, step
 
 
 def _backward(step, g, grads):
   need_l, need_r = grads
   cfg, sizes = step.cfg, step.sizes
   m, k, n = step.shape
+  be.check_operand(g, 'the cotangent')
   if tuple(g.shape) != (m, n):
     raise ValueError(f'the cotangent has shape {tuple(g.shape)}, the result '
                      f'{(m, n)}')
@@ -140,20 +133,16 @@ def _backward(step, g, grads):
       if need_r:
         drhs = be.bf16_contract_rows(step.lhs, g, sizes, step.rhs_dtype)
     return dlhs, drhs
-  be.check_operand(g, 'the cotangent')
-  step.keep.about_to_use()
   with be.on_device_of(g):
-    q = be.quantize(g, cfg.bwd_dtype, row=need_l, col=need_r, po2=cfg.po2_scale,
-                    group_sizes=sizes if need_r else None)
+    step.keep.about_to_use()
+    q, q_t = be.quantize(g, cfg.bwd_dtype, need_l, need_r, False, cfg.po2_scale,
+                         sizes if need_r else None)
     if need_l:
-      a, a_scale, a_dtype = block_scaled._kept_major(step.rhs, -1)  # pylint: disable=protected-access
-      dlhs = be.fp8_rows(q.row, q.row_scale, m, a, a_dtype, a_scale, k, n,
-                         cfg.bwd_dtype, step.lhs_dtype, sizes)
+      dlhs = be.fp8_rows(q, step.rhs, n, step.lhs_dtype, g.device, sizes)
     if need_r:
-      l = step.lhs
-      drhs = be.fp8_contract_rows(
-          l.col, l.col_scale, k, q.col, q.col_scale, n, l.col.shape[1], m,
-          cfg.bwd_dtype, cfg.fwd_dtype, step.rhs_dtype, sizes)
+      # positions along the groups' padded rows, as both operands were laid out
+      drhs = be.fp8_contract_rows(step.lhs, q_t, step.lhs.ld, m, step.rhs_dtype,
+                                  g.device, sizes)
   return dlhs, drhs
 
 

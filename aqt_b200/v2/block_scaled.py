@@ -48,6 +48,9 @@ class BlockTiling:
   square: bool
 
 
+_TILINGS = {(a, s): BlockTiling(a, s) for a in (-1, -2) for s in (False, True)}
+
+
 def _axis(contract_axis, ndim):
   if contract_axis in (-1, ndim - 1):
     return -1
@@ -76,17 +79,10 @@ def block_quantize(x, contract_axis: int = -1, square: bool = False,
   axis = _axis(contract_axis, x.ndim)
   dtype = be.fp8_dtype(bits)
   with be.on_device_of(x):
-    b = be.quantize(x, dtype, row=axis == -1, col=axis == -2, square=square,
-                    po2=po2_scale)
-  if axis == -1:
-    q = b.row[..., :x.shape[-1]].view(dtype)
-    s = b.row_scale if square else b.row_scale.transpose(-1, -2)
-  else:
-    q = b.col[..., :x.shape[-2]].view(dtype).transpose(-1, -2)
-    s = b.col_scale
+    q, s = be.quantize_tensors(x, dtype, axis, square, po2_scale)
   return aqt_tensor.QTensor(
       qvalue=q, scale=[s], scale_t=None, dequant_dtype=utils.as_dtype(x.dtype),
-      tiling_state=BlockTiling(axis, square))
+      tiling_state=_TILINGS[axis, bool(square)])
 
 
 def frozen(qvalue, scale, contract_axis: int = -2) -> aqt_tensor.QTensor:
@@ -134,8 +130,7 @@ def _contract_contiguous(q, axis):
 
 
 def _frozen_operand(qt, contract_axis):
-  """(values [.., R][ld] bytes, scale [.., R/128, K/128] view, dtype) of frozen
-  weights for a product that contracts `contract_axis`."""
+  """Frozen weights as the Side of a product that contracts `contract_axis`."""
   ts = qt.tiling_state
   if not isinstance(ts, BlockTiling) or not ts.square:
     raise NotImplementedError(
@@ -151,15 +146,30 @@ def _frozen_operand(qt, contract_axis):
   if not _contract_contiguous(q, contract_axis):
     raise ValueError('frozen values must keep the layout block_quantize or '
                      'frozen gave them (contraction contiguous, 16-byte rows)')
-  if contract_axis == -2:
-    q, s = q.transpose(-1, -2), s.transpose(-1, -2)
-  return q, s, q.dtype
+  want = (*q.shape[:-2], -(-q.shape[-2] // BLOCK), -(-q.shape[-1] // BLOCK))
+  if tuple(s.shape) != want or s.dtype != torch.float32 or s.device != q.device:
+    raise ValueError(
+        f'frozen values {tuple(q.shape)} need float32 scales {want} on their '
+        f'device (got {s.dtype} {tuple(s.shape)} on {s.device})')
+  kept_axis = -3 - contract_axis
+  # an axis of one entry may have any stride; the kernel wants a valid one
+  ld = (q.stride(kept_axis) if q.shape[kept_axis] > 1 else
+        (q.shape[contract_axis] + 15) & -16)
+  batched = q.ndim == 3
+  return be.Side(q.data_ptr(), ld, q.stride(0) if batched else 0,
+                 _CODES[q.dtype], s.data_ptr(), s.stride(0) if batched else 0,
+                 s.stride(contract_axis), s.stride(kept_axis),
+                 q.shape[kept_axis], (q, s))
+
+
+_CODES = {torch.float8_e4m3fn: _lib.E4M3, torch.float8_e5m2: _lib.E5M2}
 
 
 class _Step:
   """One forward product's operands, as its backward pass needs them."""
 
-  __slots__ = ('lhs', 'rhs', 'keep', 'out_dtype', 'lhs_shape', 'rhs_axis')
+  __slots__ = ('lhs', 'rhs', 'keep', 'rows', 'k', 'n', 'lhs_shape', 'lhs_axis',
+               'rhs_axis', 'lhs_dtype', 'rhs_dtype')
 
 
 @dataclasses.dataclass(frozen=True)
@@ -178,14 +188,14 @@ class BlockScaledDotGeneral:
                preferred_element_type=None):
     assert precision is None, (
         f'Precision {precision} requested together with quantization.')
-    out_dtype = _out_dtype(preferred_element_type, lhs)
     dims = _dims(lhs, rhs, dimension_numbers)
+    out_dtype = _out_dtype(preferred_element_type, lhs)
     if isinstance(rhs, aqt_tensor.QTensor):
-      if torch.is_grad_enabled() and lhs.requires_grad:
+      if lhs.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError(
             'a product with frozen weights has no gradient; pass float weights')
       return self._forward(lhs, rhs, dims, out_dtype, None)[0]
-    if torch.is_grad_enabled() and (lhs.requires_grad or rhs.requires_grad):
+    if (lhs.requires_grad or rhs.requires_grad) and torch.is_grad_enabled():
       return _BlockDot.apply(lhs, rhs, self, dims, out_dtype)
     return self._forward(lhs, rhs, dims, out_dtype, (False, False))[0]
 
@@ -194,87 +204,69 @@ class BlockScaledDotGeneral:
     if isinstance(rhs, aqt_tensor.QTensor):
       raise NotImplementedError(
           'a product with frozen weights has no gradient; pass float weights')
-    out_dtype = _out_dtype(preferred_element_type, lhs)
     dims = _dims(lhs, rhs, dimension_numbers)
+    out_dtype = _out_dtype(preferred_element_type, lhs)
     out, step = self._forward(lhs.detach(), rhs.detach(), dims, out_dtype,
                               (True, True))
-    return out, lambda g: self._backward(step, g, (True, True))
+    return out, lambda g: self._backward(step, g.detach(), (True, True))
 
   def _forward(self, lhs, rhs, dims, out_dtype, grads):
     lhs_axis, rhs_axis = dims
     x = _as_matrix(lhs, lhs_axis)
-    m, k = x.shape
+    device = lhs.device
     with be.on_device_of(lhs):
       if grads is None:
-        a, a_scale, a_dtype = _frozen_operand(rhs, rhs_axis)
         need_l = need_r = False
+        w, w_t = _frozen_operand(rhs, rhs_axis), None
       else:
         need_l, need_r = grads
-        w = be.quantize(rhs, self.fwd_dtype, row=rhs_axis == -1 or need_l,
-                        col=rhs_axis == -2 or need_l, square=True,
-                        po2=self.po2_scale)
-        a, a_scale, a_dtype = _kept_major(w, rhs_axis)
-      n = a.shape[-2]
-      l = be.quantize(x, self.fwd_dtype, row=True, col=need_r,
-                      po2=self.po2_scale)
-      out = be.fp8_rows(l.row, l.row_scale, m, a, a_dtype, a_scale, n, k,
-                        self.fwd_dtype, out_dtype)
-    step = None
-    if need_l or need_r:
-      step = _Step()
-      step.lhs = l if need_r else None
-      step.rhs = w if need_l else None
-      step.keep = be.Residuals(
-          ([l.col, l.col_scale] if need_r else []) +
-          (w.tensors() if need_l else []), lhs)
-      step.lhs_shape, step.rhs_axis = (lhs.shape, lhs_axis, lhs.dtype), rhs_axis
-      step.out_dtype = rhs.dtype
-      if need_r:
-        l.row = l.row_scale = None
-    shape = lhs.shape[:-1] if lhs_axis == -1 else lhs.shape[-1:]
-    return out.view(*shape, n), step
+        contracts_last = rhs_axis == -1
+        sides = be.quantize(rhs, self.fwd_dtype, contracts_last or need_l,
+                            not contracts_last or need_l, True, self.po2_scale)
+        w, w_t = sides if contracts_last else (sides[1], sides[0])
+      l, l_t = be.quantize(x, self.fwd_dtype, True, need_r, False,
+                           self.po2_scale)
+      m, k = x.shape
+      out = be.fp8_rows(l, w, k, out_dtype, device)
+      step = None
+      if need_l or need_r:
+        step = _Step()
+        step.lhs, step.rhs = l_t, w_t if need_l else None
+        step.keep = be.Residuals(step.lhs, step.rhs)
+        step.rows, step.k, step.n = m, k, w.kept
+        step.lhs_shape, step.lhs_axis, step.rhs_axis = lhs.shape, lhs_axis, rhs_axis
+        step.lhs_dtype, step.rhs_dtype = lhs.dtype, rhs.dtype
+    if lhs.ndim != 2:
+      out = out.view(*lhs.shape[:-1], w.kept)
+    return out, step
 
   def _backward(self, step, g, grads):
     need_l, need_r = grads
-    n = g.shape[-1]
-    lhs_shape, lhs_axis, lhs_dtype = step.lhs_shape
+    m, k, n = step.rows, step.k, step.n
     be.check_operand(g, 'the cotangent')
+    want = ((*step.lhs_shape[:-1], n) if step.lhs_axis == -1 else (m, n))
+    if tuple(g.shape) != want:
+      raise ValueError(f'the cotangent has shape {tuple(g.shape)}, the result '
+                       f'{want}')
+    device = g.device
     gm = _as_matrix(g, -1)
-    m = gm.shape[0]
-    step.keep.about_to_use()
+    dlhs = drhs = None
     with be.on_device_of(g):
-      q = be.quantize(gm, self.bwd_dtype, row=need_l, col=need_r,
-                      po2=self.po2_scale)
-      dlhs = drhs = None
+      step.keep.about_to_use()
+      q, q_t = be.quantize(gm, self.bwd_dtype, need_l, need_r, False,
+                           self.po2_scale)
       if need_l:
-        # contracts the axis the forward pass kept
-        keep_axis = -3 - step.rhs_axis
-        a, a_scale, a_dtype = _kept_major(step.rhs, keep_axis)
-        k = a.shape[-2]
-        dlhs = be.fp8_rows(q.row, q.row_scale, m, a, a_dtype, a_scale, k, n,
-                           self.bwd_dtype, lhs_dtype)
-        dlhs = (dlhs.view(lhs_shape) if lhs_axis == -1 else
-                dlhs.transpose(0, 1))
+        dlhs = be.fp8_rows(q, step.rhs, n, step.lhs_dtype, device)
       if need_r:
-        l = step.lhs
-        k = l.cols
-        if step.rhs_axis == -2:  # drhs [K, N]
-          drhs = be.fp8_contract_rows(
-              l.col, l.col_scale, k, q.col, q.col_scale, n, m, m,
-              self.bwd_dtype, self.fwd_dtype, step.out_dtype)
-        else:                    # drhs [N, K]
-          drhs = be.fp8_contract_rows(
-              q.col, q.col_scale, n, l.col, l.col_scale, k, m, m,
-              self.fwd_dtype, self.bwd_dtype, step.out_dtype)
+        # [K, N] as rhs lies: its last axis is the output's contiguous one
+        b, a = (step.lhs, q_t) if step.rhs_axis == -2 else (q_t, step.lhs)
+        drhs = be.fp8_contract_rows(b, a, m, m, step.rhs_dtype, device)
+    if need_l:
+      if step.lhs_axis == -2:
+        dlhs = dlhs.transpose(0, 1)
+      elif len(step.lhs_shape) != 2:
+        dlhs = dlhs.view(step.lhs_shape)
     return dlhs, drhs
-
-
-def _kept_major(blocks, contract_axis):
-  """Values [.., kept][contraction], square scale as [.., kept, contraction]."""
-  if contract_axis == -1:
-    return blocks.row[..., :blocks.cols], blocks.row_scale, blocks.dtype
-  return (blocks.col[..., :blocks.rows], blocks.col_scale.transpose(-1, -2),
-          blocks.dtype)
 
 
 class _BlockDot(torch.autograd.Function):
@@ -316,22 +308,28 @@ def _out_dtype(preferred, lhs):
 def _dims(lhs, rhs, dimension_numbers):
   """Checks the operands; returns the contracted axes as negative numbers."""
   (lca, rca), (lba, rba) = dimension_numbers
-  if tuple(lba) or tuple(rba) or len(tuple(lca)) != 1 or len(tuple(rca)) != 1:
+  if len(lba) or len(rba) or len(lca) != 1 or len(rca) != 1:
     raise NotImplementedError(
         'block-scaled products contract one axis of each operand and have no '
         f'batch axes (got {dimension_numbers})')
   be.check_operand(lhs, 'lhs')
-  q = isinstance(rhs, aqt_tensor.QTensor)
-  w = rhs.qvalue if q else rhs
-  be.check_operand(w, 'rhs', be._FP8 if q else be._FLOATS)  # pylint: disable=protected-access
+  if isinstance(rhs, aqt_tensor.QTensor):
+    w = rhs.qvalue
+    be.check_operand(w, 'rhs', be._FP8)  # pylint: disable=protected-access
+  else:
+    w = rhs
+    be.check_operand(w, 'rhs')
+    if lhs.dtype != w.dtype:
+      raise TypeError(f'Unmatched lhs and rhs dtype: {lhs.dtype} vs {w.dtype}')
   be.check_same_device(lhs, w)
-  if not q and lhs.dtype != rhs.dtype:
-    raise TypeError(f'Unmatched lhs and rhs dtype: {lhs.dtype} vs {rhs.dtype}')
   if w.ndim != 2:
     raise NotImplementedError(f'rhs is a matrix (got {tuple(w.shape)})')
-  la = int(tuple(lca)[0]) % max(lhs.ndim, 1) - lhs.ndim
-  ra = int(tuple(rca)[0]) % 2 - 2
-  if lhs.ndim < 1 or (la != -1 and lhs.ndim != 2):
+  la, ra = int(lca[0]), int(rca[0])
+  nd = lhs.ndim
+  if not -nd <= la < nd or not -2 <= ra < 2:
+    raise ValueError(f'contracted axes out of range: {dimension_numbers}')
+  la, ra = la % nd - nd, ra % 2 - 2
+  if la != -1 and nd != 2:
     raise NotImplementedError(
         'lhs is contracted over its last axis (or is a matrix)')
   if lhs.shape[la] != w.shape[ra]:
@@ -341,25 +339,19 @@ def _dims(lhs, rhs, dimension_numbers):
 
 
 def _as_matrix(x, axis):
-  """x as [rows, contraction] without a copy where its strides allow it."""
+  """x as [rows, contraction], without a copy where its strides allow it."""
   if axis == -2:
     return x.transpose(0, 1)
   if x.ndim == 2:
     return x
   if x.ndim == 1:
     return x.view(1, -1)
-  y = x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.new_empty(
-      (x.numel() if x.ndim == 0 else _prod(x.shape[:-1]), 0))
-  from aqt_b200 import engine
-  if y.numel() and y.data_ptr() != x.data_ptr() and engine._tape is not None:  # pylint: disable=protected-access
+  rows = 1
+  for n in x.shape[:-1]:
+    rows *= n
+  y = x.reshape(rows, x.shape[-1])
+  if y.numel() and y.data_ptr() != x.data_ptr() and be.tracing():
     raise _lib.AqtB200Error(
         'a traced step cannot copy an operand into another layout; make it '
         'contiguous first')
   return y
-
-
-def _prod(shape):
-  n = 1
-  for s in shape:
-    n *= s
-  return n
