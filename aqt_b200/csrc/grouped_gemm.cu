@@ -141,12 +141,20 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag) ? 1 : 0) != 0;
 }
 
-__device__ __forceinline__ void tma_load_3d_pair(void* dst, const CUtensorMap* tm, uint32_t leader_bar,
-                                                 int c0, int c1, int c2) {
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t elected, uint32_t dst, const CUtensorMap* tm,
+                                                 uint32_t leader_bar, int c0, int c1, int c2) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
-      "l"(tm), "r"(leader_bar), "r"(c0), "r"(c1), "r"(c2)
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];\n\t}" ::"r"(dst),
+      "l"(tm), "r"(leader_bar), "r"(c0), "r"(c1), "r"(c2), "r"(elected)
+      : "memory");
+}
+__device__ __forceinline__ void expect_tx_if(uint32_t elected, uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+      "@q mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar),
+      "r"(bytes), "r"(elected)
       : "memory");
 }
 // Two f32 multiply-adds in one instruction: (a0, a1) += (x0, x1) * (y0, y1).
@@ -369,51 +377,60 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     else if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   if (warp == 0) {
-    // ---------------- TMA producer (both CTAs) ----------------
-    if (lane == 0) {
+    // ---------------- TMA producer (both CTAs, whole warp) ----------------
+    {
       int stage = 0, cur = 0;
       uint32_t phase = 0;
-      const int b_boxes = P.b_mn ? (P.nt / 2 + 63) / 64 : 1;
-      const uint32_t lbar0 = map_to_cta(smem_u32(&full_bar[0]), lead);
+      const uint32_t elected = elect_one();
+      const uint32_t expecting = leader ? elected : 0u;
+      const bool a_mn = !FP8 && P.a_mn, b_mn = !FP8 && P.b_mn;
+      const int b_boxes = b_mn ? (P.nt / 2 + 63) / 64 : 1;
+      const uint32_t full0 = smem_u32(&full_bar[0]), lbar0 = map_to_cta(full0, lead);
+      const uint32_t ring = smem_u32(smem);
       for (int tile = cluster_id; tile < total && !fail; tile += num_clusters) {
         const TileAt T = gg_tile<FP8>(P, S, nseg, tile, cur);
-        const int kb0 = share_of(T.nkb, part, P.split), kb1 = share_of(T.nkb, part + 1, P.split);
-        const int ra = T.r0 + (int)rank * 128, tb = T.t0 + (int)rank * (T.n / 2);
-        const int ga = P.mode == 0 ? T.seg : 0;
+        const int nkb = __shfl_sync(0xffffffffu, T.nkb, 0);
+        const int kb0 = share_of(nkb, part, P.split), kb1 = share_of(nkb, part + 1, P.split);
+        const int ra = __shfl_sync(0xffffffffu, T.r0, 0) + (int)rank * 128;
+        const int tb = __shfl_sync(0xffffffffu, T.t0 + (int)rank * (T.n / 2), 0);
+        const int seg = __shfl_sync(0xffffffffu, T.seg, 0);
+        const int k0 = __shfl_sync(0xffffffffu, T.k0, 0);
+        const int ga = P.mode == 0 ? seg : 0;
+        // the slab a group of the contraction ends in, if it ends inside one
+        int tail = -1;
+        if (!FP8 && P.mode == 1 && P.groups > 0) {
+          const int klen = __shfl_sync(0xffffffffu, T.klen, 0);
+          if (klen % GG_TAIL) tail = klen / GG_TAIL;
+        }
         for (int ks = kb0; ks < kb1; ks += GG_KS) {
-          if (!mbar_wait(&empty_bar[stage], phase ^ 1, abortp)) { fail = 1; break; }
+          if (!warp_wait(&empty_bar[stage], phase ^ 1, abortp)) { fail = 1; break; }
           const uint32_t lbar = lbar0 + stage * 8;
           const int ke = min(ks + GG_KS, kb1);
-          if (leader) mbar_expect_tx(&full_bar[stage], 2 * (ke - ks) * slab_bytes);
-          uint8_t* sa = smem + stage * stage_bytes;
+          expect_tx_if(expecting, full0 + stage * 8, 2 * (ke - ks) * slab_bytes);
+          uint32_t sa = ring + stage * stage_bytes;
           for (int kb = ks; kb < ke; ++kb, sa += slab_bytes) {
-            uint8_t* sb = sa + GG_A_STAGE;
-            if (!FP8 && P.mode == 1 && T.klen - kb * GG_TAIL < GG_TAIL && P.groups > 0) {
-              // the group ends inside this slab: its copy, filled up with zeros
-              for (int j = 0; j < 2; ++j)
-                tma_load_3d_pair(sa + j * 8192, &tmAt, lbar, ra + j * 64, 0, T.seg);
-              for (int j = 0; j < b_boxes; ++j)
-                tma_load_3d_pair(sb + j * 8192, &tmBt, lbar, tb + j * 64, 0, T.seg);
-              continue;
-            }
-            const int kk = T.k0 + kb * P.bk;
-            if (!FP8 && P.a_mn) {
-              for (int j = 0; j < 2; ++j)
-                tma_load_3d_pair(sa + j * 8192, &tmA, lbar, ra + j * 64, kk, ga);
+            const uint32_t sb = sa + GG_A_STAGE;
+            const bool last = kb == tail;  // read the copy filled up with zeros
+            const CUtensorMap* ma = last ? &tmAt : &tmA;
+            const CUtensorMap* mb = last ? &tmBt : &tmB;
+            const int kk = last ? 0 : k0 + kb * P.bk, za = last ? seg : ga, zb = last ? seg : 0;
+            if (a_mn) {
+              tma_load_3d_pair(elected, sa, ma, lbar, ra, kk, za);
+              tma_load_3d_pair(elected, sa + 8192, ma, lbar, ra + 64, kk, za);
             } else {
-              tma_load_3d_pair(sa, &tmA, lbar, kk, ra, ga);
+              tma_load_3d_pair(elected, sa, ma, lbar, kk, ra, za);
             }
-            if (!FP8 && P.b_mn) {
-              for (int j = 0; j < b_boxes; ++j)
-                tma_load_3d_pair(sb + j * 8192, &tmB, lbar, tb + j * 64, kk, 0);
+            if (b_mn) {
+              tma_load_3d_pair(elected, sb, mb, lbar, tb, kk, zb);
+              if (b_boxes > 1) tma_load_3d_pair(elected, sb + 8192, mb, lbar, tb + 64, kk, zb);
             } else {
-              tma_load_3d_pair(sb, &tmB, lbar, kk, tb, 0);
+              tma_load_3d_pair(elected, sb, mb, lbar, kk, tb, zb);
             }
           }
           if (++stage == P.stages) { stage = 0; phase ^= 1; }
         }
       }
-      if (fail) {
+      if (fail && lane == 0) {
         *abortp = 1;
         st_cluster_u32(peer_abort, 1u);
         if (P.status) atomicCAS(P.status, 0, 1);
