@@ -45,10 +45,14 @@ int sm_count();
 //   3 slices: 512 threads start with 128: 128 *  56 + 384 * 152 = 65536
 //   4 slices: 640 threads start with  96: 128 *  32 + 512 * 112 = 61440 (fp8)
 //                                         128 *  64 + 512 * 104 = 61440 (bf16)
+// k-slabs a stage of the ring holds: two where that leaves four slabs and more in
+// flight, since each stage costs its producer and the MMA warp a wait
+constexpr int gg_slabs(bool pair, int tile) { return pair || tile <= 128 ? 2 : 1; }
 constexpr int gg_threads(int slices) { return 128 * (1 + slices); }
 constexpr int GG_A_STAGE = 128 * 128;        // this CTA's 128 rows of A, 128 bytes of k
-constexpr int GG_KS = 2;                     // k-slabs a stage of the ring holds
 constexpr int GG_MAX_STAGES = 5;
+// Whether fp8 tiles are a CTA pair's (cta_group::2) or one CTA's.
+constexpr bool GG_PAIR_NARROW = false, GG_PAIR_WIDE = true;
 constexpr int GG_RING = 192 * 1024;          // bytes of the operand ring
 // Scales travel in batches of GG_BATCH slabs: one barrier round for four of them.
 constexpr int GG_BATCH = 4;
@@ -102,32 +106,42 @@ __device__ __forceinline__ uint64_t smem_desc_mn(uint32_t saddr, uint32_t lbo) {
 // runs this, so that descriptors stay in uniform registers: issued from a
 // one-lane branch each MMA took about 70 clocks of moves, and the issuing thread
 // was what bounded every fp8 product.
-#define GG_MMA4(KIND)                                                                       \
+#define GG_MMA4(KIND, GROUP)                                                                \
   asm volatile(                                                                             \
       "{\n\t.reg .pred q, p, t;\n\t.reg .b64 a, b;\n\t.reg .b32 x, y;\n\t"                     \
       "setp.ne.b32 q, %8, 0;\n\tsetp.ne.b32 p, %7, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"            \
       "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"                                    \
-      "@q tcgen05.mma.cta_group::2.kind::" KIND " [%0], a, b, %9, p;\n\t"                   \
+      "@q tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], a, b, %9, p;\n\t"                   \
       "add.u32 x, %1, %5;\n\tadd.u32 y, %3, %6;\n\t"                                        \
       "mov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"                                      \
-      "@q tcgen05.mma.cta_group::2.kind::" KIND " [%0], a, b, %9, t;\n\t"                   \
+      "@q tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], a, b, %9, t;\n\t"                   \
       "add.u32 x, x, %5;\n\tadd.u32 y, y, %6;\n\t"                                          \
       "mov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"                                      \
-      "@q tcgen05.mma.cta_group::2.kind::" KIND " [%0], a, b, %9, t;\n\t"                   \
+      "@q tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], a, b, %9, t;\n\t"                   \
       "add.u32 x, x, %5;\n\tadd.u32 y, y, %6;\n\t"                                          \
       "mov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"                                      \
-      "@q tcgen05.mma.cta_group::2.kind::" KIND " [%0], a, b, %9, t;\n\t}" ::"r"(d_tmem),   \
+      "@q tcgen05.mma.cta_group::" GROUP ".kind::" KIND " [%0], a, b, %9, t;\n\t}" ::"r"(d_tmem),   \
       "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(a_step), "r"(b_step), "r"(accumulate), \
       "r"(elected), "r"(idesc)                                                              \
       : "memory")
-template <bool FP8>
+template <bool FP8, bool PAIR>
 __device__ __forceinline__ void gg_mma4(uint32_t elected, uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi,
                                         uint32_t b_lo, uint32_t b_hi, uint32_t a_step, uint32_t b_step,
                                         uint32_t idesc, uint32_t accumulate) {
-  if constexpr (FP8) GG_MMA4("f8f6f4");
-  else GG_MMA4("f16");
+  if constexpr (FP8 && PAIR) GG_MMA4("f8f6f4", "2");
+  else if constexpr (FP8) GG_MMA4("f8f6f4", "1");
+  else if constexpr (PAIR) GG_MMA4("f16", "2");
+  else GG_MMA4("f16", "1");
 }
 #undef GG_MMA4
+
+// Hands an accumulator back: only this warp's reads of it have to be over, which
+// the fence before orders (see mbar_arrive_cluster).
+template <bool PAIR>
+__device__ __forceinline__ void gg_arrive(uint32_t bar) {
+  if constexpr (PAIR) mbar_arrive_cluster(bar);
+  else asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 
 __device__ __forceinline__ uint32_t elect_one() {
   uint32_t e;
@@ -141,14 +155,23 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag) ? 1 : 0) != 0;
 }
 
-__device__ __forceinline__ void tma_load_3d_pair(uint32_t elected, uint32_t dst, const CUtensorMap* tm,
-                                                 uint32_t leader_bar, int c0, int c1, int c2) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
-      "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5}], [%2];\n\t}" ::"r"(dst),
-      "l"(tm), "r"(leader_bar), "r"(c0), "r"(c1), "r"(c2), "r"(elected)
-      : "memory");
+template <bool PAIR>
+__device__ __forceinline__ void tma_load_3d(uint32_t elected, uint32_t dst, const CUtensorMap* tm,
+                                            uint32_t bar, int c0, int c1, int c2) {
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];\n\t}" ::"r"(dst),
+        "l"(tm), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(elected)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5}], [%2];\n\t}" ::"r"(dst),
+        "l"(tm), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(elected)
+        : "memory");
 }
 __device__ __forceinline__ void expect_tx_if(uint32_t elected, uint32_t bar, uint32_t bytes) {
   asm volatile(
@@ -165,27 +188,48 @@ __device__ __forceinline__ void fma2(float& a0, float& a1, float x0, float x1, f
       : "+f"(a0), "+f"(a1)
       : "f"(x0), "f"(x1), "f"(y0), "f"(y1));
 }
-// Arrives at both CTAs of the pair once every MMA issued so far has completed.
+// Arrives, at both CTAs of a pair, once every MMA issued so far has completed.
+template <bool PAIR>
 __device__ __forceinline__ void gg_commit(uint32_t elected, uint32_t bar, uint32_t lead) {
-  asm volatile(
-      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
-      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
-      " [%0], %1;\n\t}" ::"r"(bar),
-      "h"((uint16_t)(3u << lead)), "r"(elected)
-      : "memory");
+  if constexpr (PAIR)
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+        "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;\n\t}" ::"r"(bar),
+        "h"((uint16_t)(3u << lead)), "r"(elected)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar),
+        "r"(elected)
+        : "memory");
 }
 
-// 16 lanes by 32 columns of TMEM; of every 8 columns a thread gets lane / 4's
-// columns 2 (lane % 4) and the next, then the same of lane / 4 + 8.
-__device__ __forceinline__ void tc_ld_16x256(uint32_t taddr, uint32_t* r) {
+// 16 lanes by 32 columns of TMEM; of every 8 columns a thread gets columns
+// 2 (lane % 4) and the next of lane / 4, then of lane / 4 + 8.
+__device__ __forceinline__ void tc_ld_16x256(uint32_t taddr, uint32_t* v) {
   asm volatile(
       "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
       "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-        "=r"(r[14]), "=r"(r[15])
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+        "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+        "=r"(v[14]), "=r"(v[15])
       : "r"(taddr)
       : "memory");
+}
+// Waits for the loads; what they brought passes through, so that no use of it can
+// be moved ahead of the wait.
+__device__ __forceinline__ void tc_wait_for(uint32_t (*v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0][0]), "+r"(v[0][1]), "+r"(v[0][2]), "+r"(v[0][3]), "+r"(v[0][4]), "+r"(v[0][5]),
+                 "+r"(v[0][6]), "+r"(v[0][7]), "+r"(v[0][8]), "+r"(v[0][9]), "+r"(v[0][10]), "+r"(v[0][11]),
+                 "+r"(v[0][12]), "+r"(v[0][13]), "+r"(v[0][14]), "+r"(v[0][15]), "+r"(v[1][0]), "+r"(v[1][1]),
+                 "+r"(v[1][2]), "+r"(v[1][3]), "+r"(v[1][4]), "+r"(v[1][5]), "+r"(v[1][6]), "+r"(v[1][7]),
+                 "+r"(v[1][8]), "+r"(v[1][9]), "+r"(v[1][10]), "+r"(v[1][11]), "+r"(v[1][12]), "+r"(v[1][13]),
+                 "+r"(v[1][14]), "+r"(v[1][15])
+               :
+               : "memory");
 }
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
   float4 v;
@@ -213,7 +257,7 @@ struct TileAt {
   int nkb;     // slabs of k
 };
 
-template <bool FP8>
+template <bool FP8, bool PAIR>
 __device__ __forceinline__ TileAt gg_tile(const GGParams& P, const Segments& S, int nseg, int tile,
                                           int& cur) {
   TileAt T;
@@ -236,7 +280,7 @@ __device__ __forceinline__ TileAt gg_tile(const GGParams& P, const Segments& S, 
   const int gt = min(G, tt - band * G);
   const int ri = in / gt, ti = band * G + (in - ri * gt);
   T.seg = cur;
-  T.r0 = ri * 256;
+  T.r0 = ri * (PAIR ? 256 : 128);
   T.k0 = 0;
   T.klen = 0;
   if (P.mode == 0) {
@@ -259,11 +303,12 @@ __device__ __forceinline__ int share_of(int nkb, int part, int split) {
   return (int)((int64_t)nkb * part / split);
 }
 
-template <bool FP8, bool A_ROW, int SLICES, int COLS>
+template <bool FP8, bool A_ROW, bool PAIR, int SLICES, int COLS>
 __global__ void __launch_bounds__(gg_threads(SLICES), 1)
 grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmAt, const __grid_constant__ CUtensorMap tmBt,
                     GGParams P) {
+  constexpr int KS = gg_slabs(PAIR, SLICES * COLS);
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) uint64_t full_bar[GG_MAX_STAGES];   // used in the pair's even CTA
@@ -280,12 +325,13 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t crank = cluster_ctarank();
-  const uint32_t rank = crank & 1u;        // within the pair
-  const uint32_t lead = crank & ~1u;       // the pair's even CTA
-  const int part = (int)(crank >> 1);
+  constexpr int CTAS = PAIR ? 2 : 1;       // that share a tile
+  const uint32_t rank = PAIR ? crank & 1u : 0u;   // within the pair
+  const uint32_t lead = PAIR ? crank & ~1u : crank;  // the pair's even CTA
+  const int part = (int)(crank / CTAS);
   const bool leader = rank == 0;
-  const int cluster_id = blockIdx.x / (2 * P.split);
-  const int num_clusters = gridDim.x / (2 * P.split);
+  const int cluster_id = blockIdx.x / (CTAS * P.split);
+  const int num_clusters = gridDim.x / (CTAS * P.split);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < P.stages; ++s) {
@@ -294,7 +340,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&tfull_bar[s], 1);
-      mbar_init(&tempty_bar[s], 2 * 4 * SLICES);
+      mbar_init(&tempty_bar[s], CTAS * 4 * SLICES);
     }
     for (int s = 0; s < GG_SLOTS; ++s) {
       mbar_init(&sfull_bar[s], 32);
@@ -305,11 +351,17 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                     smem_u32(&tmem_slot)),
-                 "r"(512)
-                 : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    if constexpr (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                       smem_u32(&tmem_slot))
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                       smem_u32(&tmem_slot))
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
   }
   if (warp == 2) {
     // prefix sums of the groups
@@ -360,14 +412,15 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();  // both CTAs' barriers exist before anyone signals them
+  // the barriers of every CTA of the cluster exist before anyone signals them
+  if (PAIR || P.split > 1) cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem_base = tmem_slot;
   const int nseg = nseg_s;
   const int total = total_s;
   volatile int* abortp = &abort_flag;
-  const uint32_t peer_abort = map_to_cta(smem_u32(&abort_flag), crank ^ 1u);
-  const int slab_bytes = GG_A_STAGE + P.b_stage, stage_bytes = GG_KS * slab_bytes;
+  const uint32_t peer_abort = map_to_cta(smem_u32(&abort_flag), PAIR ? crank ^ 1u : crank);
+  const int slab_bytes = GG_A_STAGE + P.b_stage, stage_bytes = KS * slab_bytes;
   float* const slots = (float*)(smem + P.stages * stage_bytes);
   int fail = 0;
 
@@ -384,15 +437,15 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       const uint32_t elected = elect_one();
       const uint32_t expecting = leader ? elected : 0u;
       const bool a_mn = !FP8 && P.a_mn, b_mn = !FP8 && P.b_mn;
-      const int b_boxes = b_mn ? (P.nt / 2 + 63) / 64 : 1;
-      const uint32_t full0 = smem_u32(&full_bar[0]), lbar0 = map_to_cta(full0, lead);
+      const int b_boxes = b_mn ? (P.nt / CTAS + 63) / 64 : 1;
+      const uint32_t full0 = smem_u32(&full_bar[0]), lbar0 = PAIR ? map_to_cta(full0, lead) : full0;
       const uint32_t ring = smem_u32(smem);
       for (int tile = cluster_id; tile < total && !fail; tile += num_clusters) {
-        const TileAt T = gg_tile<FP8>(P, S, nseg, tile, cur);
+        const TileAt T = gg_tile<FP8, PAIR>(P, S, nseg, tile, cur);
         const int nkb = __shfl_sync(0xffffffffu, T.nkb, 0);
         const int kb0 = share_of(nkb, part, P.split), kb1 = share_of(nkb, part + 1, P.split);
         const int ra = __shfl_sync(0xffffffffu, T.r0, 0) + (int)rank * 128;
-        const int tb = __shfl_sync(0xffffffffu, T.t0 + (int)rank * (T.n / 2), 0);
+        const int tb = __shfl_sync(0xffffffffu, T.t0 + (int)rank * (T.n / CTAS), 0);
         const int seg = __shfl_sync(0xffffffffu, T.seg, 0);
         const int k0 = __shfl_sync(0xffffffffu, T.k0, 0);
         const int ga = P.mode == 0 ? seg : 0;
@@ -402,11 +455,11 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           const int klen = __shfl_sync(0xffffffffu, T.klen, 0);
           if (klen % GG_TAIL) tail = klen / GG_TAIL;
         }
-        for (int ks = kb0; ks < kb1; ks += GG_KS) {
+        for (int ks = kb0; ks < kb1; ks += KS) {
           if (!warp_wait(&empty_bar[stage], phase ^ 1, abortp)) { fail = 1; break; }
           const uint32_t lbar = lbar0 + stage * 8;
-          const int ke = min(ks + GG_KS, kb1);
-          expect_tx_if(expecting, full0 + stage * 8, 2 * (ke - ks) * slab_bytes);
+          const int ke = min(ks + KS, kb1);
+          expect_tx_if(expecting, full0 + stage * 8, CTAS * (ke - ks) * slab_bytes);
           uint32_t sa = ring + stage * stage_bytes;
           for (int kb = ks; kb < ke; ++kb, sa += slab_bytes) {
             const uint32_t sb = sa + GG_A_STAGE;
@@ -415,16 +468,17 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             const CUtensorMap* mb = last ? &tmBt : &tmB;
             const int kk = last ? 0 : k0 + kb * P.bk, za = last ? seg : ga, zb = last ? seg : 0;
             if (a_mn) {
-              tma_load_3d_pair(elected, sa, ma, lbar, ra, kk, za);
-              tma_load_3d_pair(elected, sa + 8192, ma, lbar, ra + 64, kk, za);
+              tma_load_3d<PAIR>(elected, sa, ma, lbar, ra, kk, za);
+              tma_load_3d<PAIR>(elected, sa + 8192, ma, lbar, ra + 64, kk, za);
             } else {
-              tma_load_3d_pair(elected, sa, ma, lbar, kk, ra, za);
+              tma_load_3d<PAIR>(elected, sa, ma, lbar, kk, ra, za);
             }
             if (b_mn) {
-              tma_load_3d_pair(elected, sb, mb, lbar, tb, kk, zb);
-              if (b_boxes > 1) tma_load_3d_pair(elected, sb + 8192, mb, lbar, tb + 64, kk, zb);
+              tma_load_3d<PAIR>(elected, sb, mb, lbar, tb, kk, zb);
+              for (int j = 1; j < b_boxes; ++j)
+                tma_load_3d<PAIR>(elected, sb + j * 8192, mb, lbar, tb + j * 64, kk, zb);
             } else {
-              tma_load_3d_pair(elected, sb, mb, lbar, kk, tb, zb);
+              tma_load_3d<PAIR>(elected, sb, mb, lbar, kk, tb, zb);
             }
           }
           if (++stage == P.stages) { stage = 0; phase ^= 1; }
@@ -456,33 +510,33 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       const uint32_t empty0 = smem_u32(&empty_bar[0]);
       const uint32_t tfull0 = smem_u32(&tfull_bar[0]);
       for (int tile = cluster_id; tile < total && !fail; tile += num_clusters) {
-        const TileAt T = gg_tile<FP8>(P, S, nseg, tile, cur);
+        const TileAt T = gg_tile<FP8, PAIR>(P, S, nseg, tile, cur);
         const int nkb = __shfl_sync(0xffffffffu, T.nkb, 0);
         const int kb0 = share_of(nkb, part, P.split), kb1 = share_of(nkb, part + 1, P.split);
         const uint32_t idesc = P.idesc | ((uint32_t)(__shfl_sync(0xffffffffu, T.n, 0) >> 3) << 17);
         int in_half = 0;  // accumulators of the current half already filled
-        for (int ks = kb0; ks < kb1; ks += GG_KS) {
+        for (int ks = kb0; ks < kb1; ks += KS) {
           if (!warp_wait(&full_bar[stage], phase, abortp)) { fail = 2; break; }
-          const int ke = min(ks + GG_KS, kb1);
+          const int ke = min(ks + KS, kb1);
           uint32_t slab = (uint32_t)(stage * stage_bytes) >> 4;
           for (int kb = ks; kb < ke; ++kb, slab += (uint32_t)slab_bytes >> 4) {
             if (FP8 ? in_half == 0 : kb == kb0) {
               if (!warp_wait(&tempty_bar[half], hphase ^ 1u, abortp)) { fail = 2; break; }
             }
             tc_fence_after();
-            gg_mma4<FP8>(elected, tmem_base + half * 256u + (FP8 ? in_half * P.buf_cols : 0),
+            gg_mma4<FP8, PAIR>(elected, tmem_base + half * 256u + (FP8 ? in_half * P.buf_cols : 0),
                          a_lo0 + slab, a_hi, b_lo0 + slab, b_hi, a_step, b_step, idesc,
                          (!FP8 && kb > kb0) ? 1u : 0u);
             const bool last = kb + 1 == kb1;
             if (FP8 ? (++in_half == P.half_kb || last) : last) {
-              gg_commit(elected, tfull0 + half * 8, lead);
+              gg_commit<PAIR>(elected, tfull0 + half * 8, lead);
               in_half = 0;
               half ^= 1u;
               if (half == 0) hphase ^= 1u;
             }
           }
           if (fail) break;
-          gg_commit(elected, empty0 + stage * 8, lead);
+          gg_commit<PAIR>(elected, empty0 + stage * 8, lead);
           if (++stage == P.stages) { stage = 0; phase ^= 1; }
         }
       }
@@ -502,7 +556,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       int slot = 0, cur = 0;
       uint32_t phase = 0;
       for (int tile = cluster_id; tile < total && !fail; tile += num_clusters) {
-        const TileAt T = gg_tile<FP8>(P, S, nseg, tile, cur);
+        const TileAt T = gg_tile<FP8, PAIR>(P, S, nseg, tile, cur);
         const int kb0 = share_of(T.nkb, part, P.split), kb1 = share_of(T.nkb, part + 1, P.split);
         const int64_t kabs = T.k0 / 128 + kb0;
         const int row = min(T.r0 + (int)rank * 128, P.r - 1);
@@ -556,7 +610,6 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     // reads, 512 bytes to a warp each, took longer than the MMAs.)
     constexpr int GROUPS = COLS / 8;
     constexpr int HALF_KB = SLICES > 2 ? 1 : 128 / COLS;  // = P.half_kb
-    constexpr int LOADS = 32;                              // columns read at once
     const int quarter = warp & 3;
     const int c0 = ((warp - 4) >> 2) * COLS;  // first column of this warp
     uint32_t half = 0, hphase = 0;
@@ -565,13 +618,13 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     bool have = false;
     float acc[GROUPS][2][4];
     const uint32_t tlane = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c0;
-    const uint32_t tempty0 = map_to_cta(smem_u32(&tempty_bar[0]), lead);
+    const uint32_t tempty0 = PAIR ? map_to_cta(smem_u32(&tempty_bar[0]), lead) : smem_u32(&tempty_bar[0]);
     uint8_t* const stage_out = (uint8_t*)(slots + GG_SCALE_BYTES / 4) + (warp - 4) * GG_STAGE_OUT;
     // The place in the output is worked out anew (`again` hides that from the
     // compiler): kept across the contraction it would cost registers there.
     auto store = [&](int again) {
       asm volatile("" : "+r"(again));
-      const TileAt T = gg_tile<FP8>(P, S, nseg, again, cur);
+      const TileAt T = gg_tile<FP8, PAIR>(P, S, nseg, again, cur);
       const int r0 = T.r0 + (int)rank * 128 + quarter * 32;
       const int m = T.tvalid - c0;
       const int64_t at = (P.mode == 1 ? (int64_t)T.seg * P.o_g : 0) + (int64_t)(T.t0 + c0) * P.o_ld + r0;
@@ -634,7 +687,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       }
     };
     for (int tile = cluster_id; tile < total; tile += num_clusters) {
-      const TileAt T = gg_tile<FP8>(P, S, nseg, tile, cur);
+      const TileAt T = gg_tile<FP8, PAIR>(P, S, nseg, tile, cur);
       have = true;
       const int kb0 = share_of(T.nkb, part, P.split), kb1 = share_of(T.nkb, part + 1, P.split);
       const int cols = T.n - c0;  // this warp's columns that the MMAs write
@@ -675,7 +728,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         auto hand_back = [&]() {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(tempty0 + half * 8);
+          if (lane == 0) gg_arrive<PAIR>(tempty0 + half * 8);
         };
         const int here = FP8 && HALF_KB > 1 ? min(HALF_KB, kb1 - kb) : 1;  // accumulators in this half
         if (cols > 0) {
@@ -683,29 +736,21 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           for (int b = 0; b < here; ++b, ta += P.buf_cols, sc += GG_SLOT) {
             if (FP8 && HALF_KB > 1) factors();
 #pragma unroll
-            for (int c = 0; c < COLS; c += LOADS) {
+            for (int c = 0; c < COLS; c += 32) {
               if (c >= cols) break;  // the same for the whole warp
-              uint32_t p[LOADS / 32][2][16];
+              uint32_t p[2][16];
+              tc_ld_16x256(ta + c, p[0]);
+              tc_ld_16x256(ta + c + (16u << 16), p[1]);
+              tc_wait_for(p);
 #pragma unroll
-              for (int q = 0; q < LOADS / 32; ++q) {
-                tc_ld_16x256(ta + c + 32 * q, p[q][0]);
-                tc_ld_16x256(ta + c + 32 * q + (16u << 16), p[q][1]);
-              }
-              tc_wait_ld();
-              if constexpr (LOADS == COLS) {
-                // everything is in registers: hand the accumulators back before
-                // the arithmetic
-                if (b + 1 == here) hand_back();
-              }
-#pragma unroll
-              for (int g = 0; g < LOADS / 8; ++g) {
+              for (int g = 0; g < 4; ++g) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
 #pragma unroll
                   for (int i = 0; i < 4; i += 2) {
                     float* a = &acc[c / 8 + g][h][i];
-                    float x = __uint_as_float(p[g / 4][h][g % 4 * 4 + i]);
-                    float y = __uint_as_float(p[g / 4][h][g % 4 * 4 + i + 1]);
+                    float x = __uint_as_float(p[h][g * 4 + i]);
+                    float y = __uint_as_float(p[h][g * 4 + i + 1]);
                     if constexpr (!FP8) {
                       a[0] = x;
                       a[1] = y;
@@ -722,7 +767,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             }
           }
         }
-        if (LOADS != COLS || cols <= 0) hand_back();
+        hand_back();
         half ^= 1u;
         if (half == 0) hphase ^= 1u;
         if constexpr (FP8) {
@@ -756,7 +801,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       cluster_sync_all();
       if (busy && part == 0) {
         for (int p = 1; p < P.split; ++p) {
-          const uint32_t from = map_to_cta(smem_u32(mine), 2 * p + rank);
+          const uint32_t from = map_to_cta(smem_u32(mine), CTAS * p + rank);
           float4 v[GROUPS * 2];
 #pragma unroll
           for (int g = 0; g < GROUPS * 2; ++g) v[g] = ld_cluster_f32x4(from + g * 512);
@@ -787,11 +832,13 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();
+  if (PAIR || P.split > 1) cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512)
-                 : "memory");
+    if constexpr (PAIR)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem_base) : "memory");
   }
 }
 
@@ -914,22 +961,22 @@ static int choose_nt(int64_t len, int64_t r_tiles, bool one_group, int pairs, in
   return best;
 }
 
-// How many clusters of `pairs_each` CTA pairs the device holds at once (clusters
-// do not cross its processor groups: of 148 SMs, not 18 clusters of eight but
-// fewer than 16). Looked up once for each device and size.
-static int clusters_at_once(int dev, int pairs_each) {
-  static std::atomic<int> known[64][5];
-  std::atomic<int>& slot = known[dev & 63][pairs_each];
+// How many clusters of `ctas` CTAs the device holds at once (clusters do not cross
+// its processor groups: of 148 SMs, not 18 clusters of eight but fewer than 16).
+// Looked up once for each device and size.
+static int clusters_at_once(int dev, int ctas) {
+  static std::atomic<int> known[64][9];
+  std::atomic<int>& slot = known[dev & 63][ctas];
   int n = slot.load(std::memory_order_relaxed);
   if (n == 0) {
-    auto* fn = grouped_gemm_kernel<true, false, 2, 64>;
+    auto* fn = grouped_gemm_kernel<true, false, GG_PAIR_NARROW, 2, 64>;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * pairs_each);
+    cfg.gridDim = dim3(ctas);
     cfg.blockDim = dim3(gg_threads(2));
     cfg.dynamicSmemBytes = GG_SMEM;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = 2 * pairs_each;
+    attr[0].val.clusterDim.x = ctas;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
@@ -981,9 +1028,7 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   P.r = (int)d->r; P.t = (int)d->t;
   P.rows = (int)(P.mode == 0 ? d->t : (grouped ? d->rows : k));
   P.sizes = d->group_sizes; P.sizes64 = d->sizes_int64; P.groups = grouped ? (int)d->groups : 0;
-  P.r_tiles = (int)((d->r + 255) / 256);
   P.num_kb = (int)((k + P.bk - 1) / P.bk);
-  const int pairs = std::max(1, sm_count() / 2);
   const int64_t len = P.mode == 0 ? (d->t + groups - 1) / groups : d->t;
   // Row scales on both sides double the epilogue's arithmetic: its threads need
   // more registers than a 256-column tile leaves them (8192 x 4096 x 14336 drhs,
@@ -992,14 +1037,17 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   const bool a_row = fp8 && !d->a_scale_square;
   // Uneven groups: room for one and a half times the average before a second
   // pass. fp8 hands over an accumulator per 128-block, bf16 one per tile.
-  P.nt = choose_nt(grouped && P.mode == 0 ? len + len / 2 : len, P.r_tiles, !grouped, pairs,
-                   a_row ? 192 : 256, fp8 ? 80 : 8);
+  const int64_t want = grouped && P.mode == 0 ? len + len / 2 : len;
+  const bool pair = !fp8 || (want <= 128 ? GG_PAIR_NARROW : GG_PAIR_WIDE);
+  const int ctas = pair ? 2 : 1, units = std::max(1, sm_count() / ctas);
+  P.r_tiles = (int)((d->r + 128 * ctas - 1) / (128 * ctas));
+  P.nt = choose_nt(want, P.r_tiles, !grouped, units, a_row ? 192 : 256, fp8 ? 80 : 8);
   P.t_tiles = (int)((d->t + P.nt - 1) / P.nt);
   const uint32_t fa = fp8 ? (d->a_dtype == AQTB200_E5M2) : 1, fb = fp8 ? (d->b_dtype == AQTB200_E5M2) : 1;
   P.idesc = (1u << 4) | (fa << 7) | (fb << 10) | ((uint32_t)P.a_mn << 15) | ((uint32_t)P.b_mn << 16) |
-            (16u << 24);
-  P.b_stage = P.b_mn ? (P.nt / 2 + 63) / 64 * 8192 : P.nt / 2 * 128;
-  P.stages = std::min(GG_MAX_STAGES, GG_RING / (GG_KS * (GG_A_STAGE + P.b_stage)));
+            ((pair ? 16u : 8u) << 24);
+  P.b_stage = P.b_mn ? (P.nt / ctas + 63) / 64 * 8192 : P.nt / ctas * 128;
+  P.stages = std::min(GG_MAX_STAGES, GG_RING / (gg_slabs(pair, P.nt) * (GG_A_STAGE + P.b_stage)));
   P.buf_cols = P.nt <= 64 ? 64 : P.nt <= 128 ? 128 : 256;
   P.half_kb = 256 / P.buf_cols;
   P.a_scale = d->a_scale; P.sa_g = d->a_scale_group_stride; P.sa_k = d->a_scale_k_stride;
@@ -1019,14 +1067,14 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   AQT_REQUIRE(tiles < lim - 65536, AQTB200_EUNSUPPORTED, "more than 2^31 output tiles");
   int dev = 0;
   AQT_CUDA_OK(cudaGetDevice(&dev));
-  // Few tiles: the contraction of each is shared by up to four CTA pairs of one
-  // cluster, which add their sums through distributed shared memory, in order --
-  // as many as keep every cluster on the device at once (1 x 4096 x 4096 fp8:
-  // one pair a tile 13.7 us, two 10.9 us, four, in two rounds, 18.3 us).
+  // Few tiles: the contraction of each is shared by up to four of a cluster, which
+  // add their sums through distributed shared memory, in order -- as many as keep
+  // every cluster on the device at once (1 x 4096 x 4096 fp8 on CTA pairs: one a
+  // tile 13.7 us, two 10.9 us, four, in two rounds, 18.3 us).
   P.split = 1;
   if (P.mode == 0 && P.nt <= 128)
-    for (int s = 2; s <= 4 && P.num_kb >= s * 4 && tiles * s <= pairs; ++s)
-      if (tiles <= clusters_at_once(dev, s)) P.split = s;
+    for (int s = 2; s <= 4 && P.num_kb >= s * 4 && tiles * s <= units; ++s)
+      if (tiles <= clusters_at_once(dev, ctas * s)) P.split = s;
 
   CUtensorMap tmA, tmB, tmAt, tmBt;
   memset(&tmA, 0, sizeof(tmA));
@@ -1038,7 +1086,7 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
                 : operand_map(&tmA, d->a, fp8, k, d->r, ga, d->a_ld, d->a_group_stride, 128);
     if (rc) return rc;
     rc = P.b_mn ? operand_map(&tmB, d->b, fp8, d->t, k, 1, d->b_ld, 0, 64)
-                : operand_map(&tmB, d->b, fp8, k, d->t, 1, d->b_ld, 0, P.nt / 2);
+                : operand_map(&tmB, d->b, fp8, k, d->t, 1, d->b_ld, 0, P.nt / ctas);
     if (rc) return rc;
   }
   if (P.mode == 1 && !fp8 && grouped && k > 0) {
@@ -1068,40 +1116,45 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   }
 
   const size_t smem = GG_SMEM;
-  // Whole tiles round robin: the fewest pairs that keep the number of rounds.
-  const int64_t rounds = (tiles + pairs - 1) / pairs;
-  const int64_t clusters = P.split > 1 ? tiles : grouped ? std::min<int64_t>(tiles, pairs) : (tiles + rounds - 1) / rounds;
+  // Whole tiles round robin: the fewest CTAs that keep the number of rounds.
+  const int64_t rounds = (tiles + units - 1) / units;
+  const int64_t clusters = P.split > 1 ? tiles
+                           : grouped   ? std::min<int64_t>(tiles, units)
+                                       : (tiles + rounds - 1) / rounds;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(clusters * 2 * P.split));
+  cfg.gridDim = dim3((unsigned)(clusters * ctas * P.split));
   cfg.blockDim = dim3(gg_threads(P.nt <= 128 ? 2 : a_row ? 3 : 4));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2 * P.split;
+  attr[0].val.clusterDim.x = ctas * P.split;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-#define AQT_GG(F, R, S, C)                                                                        \
-  do {                                                                                           \
-    static bool attr_done[64] = {false};                                                         \
-    if (!attr_done[dev & 63]) {                                                                  \
-      AQT_CUDA_OK(cudaFuncSetAttribute(grouped_gemm_kernel<F, R, S, C>,                             \
+#define AQT_GG(...)                                                                                \
+  do {                                                                                             \
+    static bool attr_done[64] = {false};                                                           \
+    if (!attr_done[dev & 63]) {                                                                    \
+      AQT_CUDA_OK(cudaFuncSetAttribute(grouped_gemm_kernel<__VA_ARGS__>,                           \
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, (int)GG_SMEM)); \
-      attr_done[dev & 63] = true;                                                                \
-    }                                                                                            \
-    AQT_CUDA_OK(cudaLaunchKernelEx(&cfg, grouped_gemm_kernel<F, R, S, C>, tmA, tmB, tmAt, tmBt, P)); \
+      attr_done[dev & 63] = true;                                                                  \
+    }                                                                                              \
+    AQT_CUDA_OK(cudaLaunchKernelEx(&cfg, grouped_gemm_kernel<__VA_ARGS__>, tmA, tmB, tmAt, tmBt, P)); \
   } while (0)
-#define AQT_GG_C(F, R, S)                   \
-  do {                                      \
-    if (P.nt <= 64) AQT_GG(F, R, 2, 32);    \
-    else if (P.nt <= 128) AQT_GG(F, R, 2, 64); \
-    else AQT_GG(F, R, S, 64);               \
-  } while (0)
-  if (!fp8) AQT_GG_C(false, false, 4);
-  else if (!a_row) AQT_GG_C(true, false, 4);
-  else AQT_GG_C(true, true, 3);
-#undef AQT_GG_C
+  if (!fp8) {
+    if (P.nt <= 64) AQT_GG(false, false, true, 2, 32);
+    else if (P.nt <= 128) AQT_GG(false, false, true, 2, 64);
+    else AQT_GG(false, false, true, 4, 64);
+  } else if (!a_row) {
+    if (P.nt <= 64) AQT_GG(true, false, GG_PAIR_NARROW, 2, 32);
+    else if (P.nt <= 128) AQT_GG(true, false, GG_PAIR_NARROW, 2, 64);
+    else AQT_GG(true, false, GG_PAIR_WIDE, 4, 64);
+  } else {
+    if (P.nt <= 64) AQT_GG(true, true, GG_PAIR_NARROW, 2, 32);
+    else if (P.nt <= 128) AQT_GG(true, true, GG_PAIR_NARROW, 2, 64);
+    else AQT_GG(true, true, GG_PAIR_WIDE, 3, 64);
+  }
 #undef AQT_GG
   AQT_CUDA_OK(cudaGetLastError()); count_launch();
   return 0;
