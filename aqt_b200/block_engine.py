@@ -232,8 +232,19 @@ def _check(rc, what):
 
 def _gemm(desc, device, what):
   _check(engine._call(  # pylint: disable=protected-access
-      _lib.load().aqtb200_grouped_gemm, C.byref(desc),
-      engine._status_buf(device).data_ptr(), engine._stream()), what)  # pylint: disable=protected-access
+      _lib.load().aqtb200_grouped_gemm, C.byref(desc), _status(device),
+      engine._stream()), what)  # pylint: disable=protected-access
+
+
+def _status(device):
+  """Address of the device's status words. A first call under graph capture goes
+  without: the words would be memory of that graph."""
+  buf = engine._status.get(str(device))  # pylint: disable=protected-access
+  if buf is None:
+    if device.type == 'cuda' and torch.cuda.is_current_stream_capturing():
+      return None
+    buf = engine._status_buf(device)  # pylint: disable=protected-access
+  return buf.data_ptr()
 
 
 def _sizes(group_sizes):

@@ -881,8 +881,18 @@ __global__ void __launch_bounds__(256) group_tails_kernel(TailParams P) {
          i += (int64_t)gridDim.y * blockDim.x) {
       const int64_t k = i / vecs, c = (i - k * vecs) * 8;
       uint4 v = make_uint4(0, 0, 0, 0);
-      // operands are padded to whole 8-element pieces (strides are multiples of 8)
-      if (k < count) v = __ldg((const uint4*)(P.x[s] + (first + k) * P.ld[s] + c));
+      if (k < count) {
+        const uint16_t* x = P.x[s] + (first + k) * P.ld[s] + c;
+        if (c + 8 <= P.width[s]) {
+          v = __ldg((const uint4*)x);
+        } else {  // the row ends inside this piece, and so may the tensor's memory
+          __align__(16) uint16_t e[8] = {0};
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (c + q < P.width[s]) e[q] = __ldg(x + q);
+          v = *(const uint4*)e;
+        }
+      }
       *(uint4*)(P.out[s] + ((int64_t)g * GG_TAIL + k) * P.ld_out[s] + c) = v;
     }
   }

@@ -53,7 +53,10 @@ class ProjectionStack:
   """Weights, gradient buffers and one training step of the stack."""
 
   def __init__(self, device, layers: int = LAYERS, group=None, seed: int = 0,
-               stochastic_rounding: bool = False):
+               stochastic_rounding: bool = False, cfg=None):
+    """cfg: what carries out the projections, anything with DotGeneral's vjp
+    (block_scaled.dot_general_make() for block-scaled fp8); None: int8 per
+    channel."""
     self.device, self.layers, self.group = device, layers, group
     gen = torch.Generator(device=device)
     gen.manual_seed(seed)  # the same weights on every rank
@@ -61,7 +64,7 @@ class ProjectionStack:
         torch.bfloat16) for n, i, o in PROJ} for _ in range(layers)]
     self.grad = [{n: torch.zeros(i, o, device=device, dtype=torch.bfloat16)
                   for n, i, o in PROJ} for _ in range(layers)]
-    self.cfg = config.fully_quantized(
+    self.cfg = cfg if cfg is not None else config.fully_quantized(
         fwd_bits=8, bwd_bits=8, use_stochastic_rounding=stochastic_rounding)
 
   def _dot(self, x, w):

@@ -22,6 +22,7 @@ zero, and the running sum is cut at M.
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from aqt_b200 import block_engine as be
 from aqt_b200.v2 import aqt_tensor
@@ -48,7 +49,11 @@ def ragged_dot(lhs, rhs, group_sizes, cfg=None, preferred_element_type=None):
 
 
 def ragged_dot_vjp(lhs, rhs, group_sizes, cfg=None, preferred_element_type=None):
-  """(out, backprop) of ragged_dot with backprop(g) -> (dlhs, drhs)."""
+  """(out, backprop) of ragged_dot with backprop(g) -> (dlhs, drhs).
+
+  backprop reads group_sizes (and, without cfg, the operands) again: they have to
+  hold what they held at the call.
+  """
   if isinstance(rhs, aqt_tensor.QTensor):
     raise NotImplementedError(
         'a product with frozen weights has no gradient; pass float weights')
@@ -164,6 +169,7 @@ class _RaggedDot(torch.autograd.Function):
     return out
 
   @staticmethod
+  @once_differentiable
   def backward(ctx, g):
     step = ctx.step
     step.sizes = ctx.saved_tensors[0]

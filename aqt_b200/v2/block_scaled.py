@@ -31,6 +31,7 @@ import dataclasses
 from typing import Any
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from aqt_b200 import _lib
 from aqt_b200 import block_engine as be
@@ -280,6 +281,7 @@ class _BlockDot(torch.autograd.Function):
     return out
 
   @staticmethod
+  @once_differentiable
   def backward(ctx, g):
     dlhs, drhs = ctx.cfg._backward(  # pylint: disable=protected-access
         ctx.step, g, ctx.needs_input_grad[:2])

@@ -1,0 +1,182 @@
+"""Host logic of the block-scaled and grouped products on the CPU: layouts,
+operand orders, gradients and groups against the definition in 64 bits, with the
+library replaced by tests/fake_block_lib.py."""
+
+import numpy as np
+import pytest
+import torch
+
+from aqt_b200.v2 import aqt_dot_general
+from aqt_b200.v2 import aqt_ragged_dot as rd
+from aqt_b200.v2 import block_scaled as bs
+from tests import block_ref as ref
+from tests import fake_block_lib
+from tests import util
+
+DIMS = (((1,), (0,)), ((), ()))
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+
+
+@pytest.fixture(autouse=True)
+def fake(monkeypatch):
+  return fake_block_lib.install(monkeypatch)
+
+
+def _data(shape, dtype, seed, scale=1.0):
+  rng = np.random.default_rng(seed)
+  return torch.from_numpy((rng.standard_normal(shape) * scale).astype(
+      np.float32)).to(dtype)
+
+
+def _np(t):
+  return t.detach().float().numpy()
+
+
+def _off(t):
+  wide = torch.zeros(*t.shape[:-1], t.shape[-1] + 5, dtype=t.dtype)
+  wide[..., 2:2 + t.shape[-1]] = t
+  return wide[..., 2:2 + t.shape[-1]]
+
+
+def _flip(t):
+  return t.transpose(-1, -2).contiguous().transpose(-1, -2)
+
+
+@pytest.mark.parametrize('shape', [(1, 1), (5, 130), (129, 16), (3, 40, 150)])
+@pytest.mark.parametrize('axis', [-1, -2])
+@pytest.mark.parametrize('square', [False, True])
+@pytest.mark.parametrize('layout', [lambda t: t, _off, _flip])
+def test_quantize(shape, axis, square, layout):
+  x = _data(shape, torch.bfloat16, 1)
+  qt = bs.block_quantize(layout(x), axis, square, 'e5m2', po2_scale=True)
+  br = 128 if square or axis == -2 else 1
+  bc = 128 if square or axis == -1 else 1
+  for g in range(shape[0] if len(shape) == 3 else 1):
+    pick = (lambda t: t[g]) if len(shape) == 3 else (lambda t: t)
+    q, s = ref.quantize(_np(pick(x)), br, bc, 'e5m2', True)
+    np.testing.assert_array_equal(pick(qt.scale[0]).numpy(), s)
+    np.testing.assert_array_equal(util.to_numpy(pick(qt.qvalue)).view(np.uint8),
+                                  q.view(np.uint8))
+
+
+def _dot_want(x, w, g):
+  f = ref.fake
+  wq = f(w, 128, 128, 'e4m3')
+  return (f(x, 1, 128, 'e4m3') @ wq, f(g, 1, 128, 'e5m2') @ wq.T,
+          f(x, 128, 1, 'e4m3').T @ f(g, 128, 1, 'e5m2'))
+
+
+def _same(got, want, half):
+  got = _np(got).astype(np.float64)
+  assert got.shape == want.shape
+  # computed in 64 bits and rounded through f32: half a step each
+  tol = (half + 2.0 ** -24) * np.abs(want) + 2.0 ** -120
+  assert (np.abs(got - want) <= tol).all()
+
+
+@pytest.mark.parametrize('m,k,n', [(1, 5, 3), (40, 200, 136), (130, 129, 257)])
+@pytest.mark.parametrize('rhs_axis', [0, 1])
+@pytest.mark.parametrize('lhs_t', [False, True])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_dot_step(m, k, n, rhs_axis, lhs_t, dtype):
+  x, w, g = (_data((m, k), dtype, 2), _data((k, n), dtype, 3, 0.3), _data(
+      (m, n), dtype, 4))
+  a = x.t().contiguous() if lhs_t else _off(x)
+  b = w.t().contiguous() if rhs_axis else w
+  dims = (((0 if lhs_t else 1,), (rhs_axis,)), ((), ()))
+  out, bp = bs.dot_general_make().vjp(a, b, dims)
+  dl, dr = bp(_off(g))
+  want = _dot_want(_np(x), _np(w), _np(g))
+  _same(out, want[0], HALF[dtype])
+  _same(dl, want[1].T if lhs_t else want[1], HALF[dtype])
+  _same(dr, want[2].T if rhs_axis else want[2], HALF[dtype])
+
+
+def test_dot_shapes_and_frozen():
+  x, w = _data((2, 3, 200), torch.bfloat16, 5), _data((200, 24), torch.bfloat16, 6)
+  cfg = bs.dot_general_make()
+  plain = cfg(x.reshape(6, 200), w, DIMS)
+  assert torch.equal(cfg(x, w, (((2,), (0,)), ((), ()))), plain.view(2, 3, 24))
+  assert torch.equal(cfg(x, w, (((-1,), (-2,)), ((), ()))), plain.view(2, 3, 24))
+  assert torch.equal(aqt_dot_general.einsum('abk,kn->abn', x, w, dg=cfg),
+                     plain.view(2, 3, 24))
+  assert torch.equal(cfg(x[1, 2], w, (((0,), (0,)), ((), ()))), plain[5])
+  qt = bs.block_quantize(w, 0, square=True)
+  assert torch.equal(cfg(x.reshape(6, 200), qt, DIMS), plain)
+  again = bs.frozen(qt.qvalue.contiguous(), qt.scale[0])
+  assert torch.equal(cfg(x.reshape(6, 200), again, DIMS), plain)
+  qt = bs.block_quantize(w.t().contiguous(), 1, square=True)
+  assert torch.equal(cfg(x.reshape(6, 200), qt, (((1,), (1,)), ((), ()))), plain)
+
+
+def test_dot_autograd():
+  x, w, g = (_data((9, 40), torch.float32, 7), _data((40, 24), torch.float32, 8),
+             _data((9, 24), torch.float32, 9))
+  cfg = bs.dot_general_make()
+  out, bp = cfg.vjp(x, w, DIMS)
+  dl, dr = bp(g)
+  for need_l, need_r in ((True, True), (True, False), (False, True)):
+    a, b = x.clone().requires_grad_(need_l), w.clone().requires_grad_(need_r)
+    y = cfg(a, b, DIMS)
+    y.backward(g)
+    assert torch.equal(y, out)
+    assert torch.equal(a.grad, dl) if need_l else a.grad is None
+    assert torch.equal(b.grad, dr) if need_r else b.grad is None
+  # no second derivative: refused, not silently zero
+  a, h = x.clone().requires_grad_(), g.clone().requires_grad_()
+  first, = torch.autograd.grad(cfg(a, w, DIMS), a, h, create_graph=True)
+  with pytest.raises(RuntimeError, match='once_differentiable'):
+    first.sum().backward()
+  with pytest.raises(ValueError, match='cotangent'):
+    bp(g[:4])
+
+
+RAGGED = [(1, 8, 8, [1]), (7, 200, 24, [3, 0, 2]), (300, 40, 72, [130, 0, 129]),
+          (20, 16, 8, [-3, 15, 9]), (6, 8, 16, [0, 0])]
+
+
+@pytest.mark.parametrize('m,k,n,sizes', RAGGED)
+@pytest.mark.parametrize('q', [False, True])
+@pytest.mark.parametrize('index', [torch.int32, torch.int64])
+@pytest.mark.parametrize('layout', [lambda t: t, _off, _flip])
+def test_ragged_step(m, k, n, sizes, q, index, layout):
+  x, w, g = (_data((m, k), torch.bfloat16, 10), _data(
+      (len(sizes), k, n), torch.bfloat16, 11, 0.2), _data((m, n), torch.bfloat16, 12))
+  out, bp = rd.ragged_dot_vjp(layout(x), layout(w), torch.tensor(sizes, dtype=index),
+                              cfg=bs.dot_general_make() if q else None)
+  dl, dr = bp(layout(g))
+  xs, ws, gs = _np(x), _np(w), _np(g)
+  want = [np.zeros((m, n)), np.zeros((m, k)), np.zeros((len(sizes), k, n))]
+  for e, (a, b) in enumerate(ref.spans(sizes, m)):
+    if b > a:
+      part = (_dot_want(xs[a:b], ws[e], gs[a:b]) if q else
+              tuple(v.astype(np.float64) for v in (
+                  xs[a:b].astype(np.float64) @ ws[e],
+                  gs[a:b].astype(np.float64) @ ws[e].T,
+                  xs[a:b].T.astype(np.float64) @ gs[a:b])))
+      want[0][a:b], want[1][a:b], want[2][e] = part
+  for got, value in zip((out, dl, dr), want):
+    _same(got, value, 2.0 ** -8)
+
+
+def test_ragged_frozen_and_autograd():
+  m, k, n, sizes = 12, 40, 24, [5, 0, 6]
+  x, w, g = (_data((m, k), torch.bfloat16, 13), _data(
+      (3, k, n), torch.bfloat16, 14), _data((m, n), torch.bfloat16, 15))
+  s = torch.tensor(sizes)
+  for cfg in (None, bs.dot_general_make()):
+    out, bp = rd.ragged_dot_vjp(x, w, s, cfg=cfg)
+    dl, dr = bp(g)
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y = rd.ragged_dot(a, b, s, cfg=cfg)
+    y.backward(g)
+    assert torch.equal(y, out) and torch.equal(a.grad, dl)
+    assert torch.equal(b.grad, dr)
+    # sizes written over before the backward pass are noticed
+    y = rd.ragged_dot(a, b, s, cfg=cfg)
+    s.add_(0)
+    with pytest.raises(RuntimeError, match='modified by an inplace'):
+      y.backward(g)
+    if cfg is not None:
+      qt = bs.block_quantize(w, 1, square=True)
+      assert torch.equal(rd.ragged_dot(x, qt, s, cfg=cfg), out)

@@ -363,3 +363,22 @@ def test_traced_step():
   want = cfg(x, qt, DIMS)
   _done()
   assert torch.equal(got, want)
+
+
+def test_projection_stack_runs_on_block_scaled_products():
+  """The decoder stack's projections, one layer, a training micro-step: runs, and
+  the weight gradients agree with the int8 stack's to what 8 bits leave."""
+  from aqt_b200 import layer_stack
+  x = _data((128, layer_stack.D_MODEL), torch.bfloat16, 29, 0.0)
+  grads = []
+  for cfg in (bs.dot_general_make('e4m3', 'e4m3'), None):
+    stack = layer_stack.ProjectionStack('cuda', layers=1, cfg=cfg)
+    loss = stack.micro_step(x)
+    _done()
+    assert torch.isfinite(loss)
+    grads.append(stack.grad[0])
+  for name in grads[0]:
+    a, b = grads[0][name].double(), grads[1][name].double()
+    # two operands a product, each off by at most 2^-4 (e4m3); the longest chain
+    # to a weight gradient is five products deep
+    assert float((a - b).norm() / b.norm()) < 2 * 2.0 ** -4 * 5, name
