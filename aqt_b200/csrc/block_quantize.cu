@@ -108,6 +108,21 @@ struct Elems<true> {
     const uint4 u = __ldg((const uint4*)((const unsigned short*)p + at));
     w[i][0] = u.x; w[i][1] = u.y; w[i][2] = u.z; w[i][3] = u.w;
   }
+  // The same eight elements from an address that is only element aligned: aligned
+  // words, shifted into place. Reads the word that holds the element before (at an
+  // odd address) and after; the caller makes sure that they exist.
+  __device__ __forceinline__ void load_words(int i, const void* p, int64_t at) {
+    const uintptr_t a = (uintptr_t)((const unsigned short*)p + at);
+    const uint32_t* q = (const uint32_t*)(a & ~(uintptr_t)3);
+    const uint32_t t0 = __ldg(q), t1 = __ldg(q + 1), t2 = __ldg(q + 2), t3 = __ldg(q + 3);
+    w[i][0] = t0; w[i][1] = t1; w[i][2] = t2; w[i][3] = t3;
+    if (a & 2) {
+      w[i][0] = __funnelshift_r(t0, t1, 16);
+      w[i][1] = __funnelshift_r(t1, t2, 16);
+      w[i][2] = __funnelshift_r(t2, t3, 16);
+      w[i][3] = __funnelshift_r(t3, __ldg(q + 4), 16);
+    }
+  }
   __device__ __forceinline__ void set(int i, int j, const void* p, int64_t at) {
     const uint32_t v = __ldg((const unsigned short*)p + at);
     w[i][j >> 1] = (j & 1) ? (w[i][j >> 1] & 0xffffu) | (v << 16) : (w[i][j >> 1] & 0xffff0000u) | v;
@@ -142,6 +157,10 @@ struct Elems<false> {
     const float4 a = __ldg(q), b = __ldg(q + 1);
     v[i][0] = a.x; v[i][1] = a.y; v[i][2] = a.z; v[i][3] = a.w;
     v[i][4] = b.x; v[i][5] = b.y; v[i][6] = b.z; v[i][7] = b.w;
+  }
+  __device__ __forceinline__ void load_words(int i, const void* p, int64_t at) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[i][j] = __ldg((const float*)p + at + j);
   }
   __device__ __forceinline__ void set(int i, int j, const void* p, int64_t at) {
     v[i][j] = __ldg((const float*)p + at);
@@ -209,6 +228,8 @@ __global__ void __launch_bounds__(BQ_THREADS, BF16 ? 4 : 2) block_quantize_kerne
         const int64_t at = base + (row + i) * P.rs + col * P.cs;
         if (VEC && col + 8 <= P.cols) {
           x.load(i, P.x, at);
+        } else if (!VEC && P.cs == 1 && col > 0 && col + 8 < P.cols) {
+          x.load_words(i, P.x, at);
         } else {
 #pragma unroll
           for (int j = 0; j < 8; ++j)

@@ -898,13 +898,44 @@ __global__ void __launch_bounds__(256) group_tails_kernel(TailParams P) {
   }
 }
 
+// One warp a row, four elements a lane. Contiguous columns are read as aligned
+// words and shifted into place, so that a row may start at any element; the words
+// that hold a row's first and last elements are not read whole, since they may lie
+// half outside the tensor.
 __global__ void __launch_bounds__(256) pack_bf16_kernel(const uint16_t* x, int64_t rows, int64_t cols,
                                                         int64_t b1, int64_t bs0, int64_t bs1, int64_t rs,
                                                         int64_t cs, uint16_t* out, int64_t ld, int64_t n) {
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t c = i % ld, rr = i / ld, row = rr % rows, b = rr / rows;
-    out[i] = c < cols ? __ldg(x + (b / b1) * bs0 + (b % b1) * bs1 + row * rs + c * cs) : 0;
+  const int lane = threadIdx.x & 31;
+  const int64_t step = (int64_t)gridDim.x * (blockDim.x >> 5);
+  for (int64_t r = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); r < n; r += step) {
+    const int64_t b = r / rows, row = r - b * rows;
+    const uint16_t* src = x + (b / b1) * bs0 + (b % b1) * bs1 + row * rs;
+    uint16_t* dst = out + r * ld;  // ld: a multiple of 4, 8-byte aligned rows
+    if (cs == 1) {
+#pragma unroll 2
+      for (int64_t c = lane * 4; c < ld; c += 128) {
+        uint32_t lo = 0, hi = 0;
+        const uint16_t* p = src + c;
+        const bool odd = (uintptr_t)p & 2;
+        if (c + 4 < cols && (c > 0 || !odd)) {
+          const uint32_t* w = (const uint32_t*)((uintptr_t)p & ~(uintptr_t)3);
+          lo = __ldg(w);
+          hi = __ldg(w + 1);
+          if (odd) {
+            lo = __funnelshift_r(lo, hi, 16);
+            hi = __funnelshift_r(hi, __ldg(w + 2), 16);
+          }
+        } else {
+          if (c < cols) lo = __ldg(p);
+          if (c + 1 < cols) lo |= (uint32_t)__ldg(p + 1) << 16;
+          if (c + 2 < cols) hi = __ldg(p + 2);
+          if (c + 3 < cols) hi |= (uint32_t)__ldg(p + 3) << 16;
+        }
+        *(uint2*)(dst + c) = make_uint2(lo, hi);
+      }
+    } else {
+      for (int64_t c = lane; c < ld; c += 32) dst[c] = c < cols ? __ldg(src + c * cs) : 0;
+    }
   }
 }
 
@@ -1188,10 +1219,12 @@ int aqtb200_pack_bf16(const aqtb200_view* x, void* out, int64_t ld, void* stream
   AQT_REQUIRE(x != nullptr && x->dtype == AQTB200_BF16, AQTB200_EINVAL, "pack: a bf16 view");
   AQT_REQUIRE(x->b0 >= 0 && x->b1 >= 0 && x->rows >= 0 && x->cols >= 0 && ld >= x->cols, AQTB200_EINVAL,
               "pack: bad extents");
-  const int64_t n = x->b0 * x->b1 * x->rows * ld;
-  if (n == 0) return 0;
+  const int64_t n = x->b0 * x->b1 * x->rows;
+  if (n == 0 || ld == 0) return 0;
+  AQT_REQUIRE(ld % 8 == 0 && ((uintptr_t)out & 15) == 0, AQTB200_EINVAL,
+              "pack: rows of whole 16-byte pieces, 16-byte aligned");
   AQT_REQUIRE(out != nullptr && (x->ptr != nullptr || x->cols == 0), AQTB200_EINVAL, "pack: null pointer");
-  const int64_t blocks = std::min<int64_t>((n + 255) / 256, (int64_t)sm_count() * 16);
+  const int64_t blocks = std::min<int64_t>((n + 7) / 8, (int64_t)sm_count() * 16);
   pack_bf16_kernel<<<(unsigned)blocks, 256, 0, (cudaStream_t)stream>>>(
       (const uint16_t*)x->ptr, x->rows, x->cols, x->b1, x->b0_stride, x->b1_stride, x->row_stride,
       x->col_stride, (uint16_t*)out, ld, n);

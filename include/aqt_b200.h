@@ -658,8 +658,9 @@ int aqtb200_grouped_gemm(const aqtb200_grouped_gemm_desc* desc, int32_t* status,
 
 /*
  * aqtb200_pack_bf16: out[b][rows][ld] = x[b][rows][cols] (bf16, any strides; b =
- * b0 * b1), columns from `cols` to `ld` zero: brings an operand whose strides a
- * tensor map cannot describe into a layout aqtb200_grouped_gemm takes.
+ * b0 * b1), columns from `cols` to `ld` (a multiple of 8) zero: brings an operand
+ * whose strides a tensor map cannot describe into a layout aqtb200_grouped_gemm
+ * takes.
  */
 int aqtb200_pack_bf16(const aqtb200_view* x, void* out, int64_t ld, void* stream);
 

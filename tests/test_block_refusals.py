@@ -213,4 +213,6 @@ def test_abi_pack(lib):
   v.dtype = _lib.BF16
   assert lib.aqtb200_pack_bf16(C.byref(v), 256, 4, None) == -1
   assert lib.aqtb200_pack_bf16(C.byref(v), None, 8, None) == -1
+  assert lib.aqtb200_pack_bf16(C.byref(v), 264, 8, None) == -1
+  assert lib.aqtb200_pack_bf16(C.byref(v), 256, 12, None) == -1
   assert lib.aqtb200_pack_bf16(None, 256, 8, None) == -1
