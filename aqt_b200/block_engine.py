@@ -108,6 +108,13 @@ def _align(n):
   return (n + 255) & -256
 
 
+def _scratch(nbytes, device):
+  t = torch.empty(nbytes, dtype=torch.uint8, device=device)
+  if engine._tape is not None:  # pylint: disable=protected-access
+    engine._tape.keep.append(t)  # pylint: disable=protected-access
+  return t
+
+
 def quantize(x, dtype, row=True, col=False, square=False, po2=False,
              group_sizes=None):
   """Quantizes a matrix [R, C] or matrices [G, R, C] in blocks of 128.
@@ -155,7 +162,7 @@ def quantize(x, dtype, row=True, col=False, square=False, po2=False,
     if not square:
       at_s_col = end
       end += _align(batch * row_blocks * c * 4)
-  ws = engine._empty((end,), torch.uint8, x.device)  # pylint: disable=protected-access
+  ws = _scratch(end, x.device)
   base = ws.data_ptr()
   desc = _lib.BlockQuantDesc(
       _lib.View(x.data_ptr(), code[x.dtype], 0, batch, 1, r, c, bs, 0, rs, cs),
@@ -239,12 +246,17 @@ def _gemm(desc, device, what):
 def _status(device):
   """Address of the device's status words. A first call under graph capture goes
   without: the words would be memory of that graph."""
-  buf = engine._status.get(str(device))  # pylint: disable=protected-access
-  if buf is None:
-    if device.type == 'cuda' and torch.cuda.is_current_stream_capturing():
+  at = _status_at.get(device)
+  if at is None:
+    if (device.type == 'cuda' and str(device) not in engine._status and  # pylint: disable=protected-access
+        torch.cuda.is_current_stream_capturing()):
       return None
-    buf = engine._status_buf(device)  # pylint: disable=protected-access
-  return buf.data_ptr()
+    # the engine keeps the words for good
+    at = _status_at[device] = engine._status_buf(device).data_ptr()  # pylint: disable=protected-access
+  return at
+
+
+_status_at = {}
 
 
 def _sizes(group_sizes):
@@ -364,7 +376,7 @@ def bf16_contract_rows(lhs, g, group_sizes, out_dtype):
   # room for the groups' last, partial slabs
   nbytes = _lib.load().aqtb200_grouped_gemm_workspace_bytes(C.byref(d))
   if nbytes:
-    ws = engine._empty((nbytes,), torch.uint8, dev)  # pylint: disable=protected-access
+    ws = _scratch(nbytes, dev)
     d.workspace, d.workspace_bytes = ws.data_ptr(), nbytes
   _gemm(d, dev, 'grouped product')
   return out

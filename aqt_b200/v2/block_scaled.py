@@ -310,7 +310,7 @@ def _out_dtype(preferred, lhs):
 def _dims(lhs, rhs, dimension_numbers):
   """Checks the operands; returns the contracted axes as negative numbers."""
   (lca, rca), (lba, rba) = dimension_numbers
-  if len(lba) or len(rba) or len(lca) != 1 or len(rca) != 1:
+  if lba or rba or len(lca) != 1 or len(rca) != 1:
     raise NotImplementedError(
         'block-scaled products contract one axis of each operand and have no '
         f'batch axes (got {dimension_numbers})')
@@ -326,7 +326,7 @@ def _dims(lhs, rhs, dimension_numbers):
   be.check_same_device(lhs, w)
   if w.ndim != 2:
     raise NotImplementedError(f'rhs is a matrix (got {tuple(w.shape)})')
-  la, ra = int(lca[0]), int(rca[0])
+  la, ra = lca[0], rca[0]
   nd = lhs.ndim
   if not -nd <= la < nd or not -2 <= ra < 2:
     raise ValueError(f'contracted axes out of range: {dimension_numbers}')
