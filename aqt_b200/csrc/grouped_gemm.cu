@@ -47,7 +47,7 @@ int sm_count();
 //                                         128 *  64 + 512 * 104 = 61440 (bf16)
 // k-slabs a stage of the ring holds: two where that leaves four slabs and more in
 // flight, since each stage costs its producer and the MMA warp a wait
-constexpr int gg_slabs(bool pair, int tile) { return pair || tile <= 128 ? 2 : 1; }
+constexpr int gg_slabs(bool fp8, int tile) { return fp8 && tile > 128 ? 1 : 2; }
 constexpr int gg_threads(int slices) { return 128 * (1 + slices); }
 constexpr int GG_A_STAGE = 128 * 128;        // this CTA's 128 rows of A, 128 bytes of k
 constexpr int GG_MAX_STAGES = 5;
@@ -59,8 +59,11 @@ constexpr int GG_BATCH = 4;
 constexpr int GG_SLOTS = 2;                  // batches on their way or in use
 constexpr int GG_SLOT = 256 + 128;           // floats a slab: 256 columns, this CTA's 128 rows
 constexpr int GG_SCALE_BYTES = GG_SLOTS * GG_BATCH * GG_SLOT * 4;
-constexpr int GG_STAGE_OUT = 512;            // a warp's staging: 8 columns by 32 rows of bf16
+constexpr int GG_STAGE_OUT = 512;            // a warp's staging: 8 columns by 32 rows of bf16,
+constexpr int GG_STAGE_WIDE = 4096;          // or all of its 64 columns
+constexpr int GG_RING_WIDE = 128 * 1024;
 constexpr size_t GG_SMEM = GG_RING + GG_SCALE_BYTES + 16 * GG_STAGE_OUT + 1024;
+static_assert(GG_RING_WIDE + GG_SCALE_BYTES + 16 * GG_STAGE_WIDE + 1024 <= GG_SMEM, "shared memory");
 constexpr int GG_MAX_SEG = AQTB200_MAX_GROUPS + 1;
 constexpr int GG_TAIL = 64;                  // k-slab of bf16 elements
 
@@ -85,6 +88,7 @@ struct GGParams {
   void* out;
   int out_f32;
   int out_staged;  // bf16 rows of whole 16-byte pieces
+  int tma_out;     // and a map of them
   int64_t o_ld, o_g;
   int32_t* status;
 };
@@ -308,7 +312,12 @@ __global__ void __launch_bounds__(gg_threads(SLICES), 1)
 grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmAt, const __grid_constant__ CUtensorMap tmBt,
                     GGParams P) {
-  constexpr int KS = gg_slabs(PAIR, SLICES * COLS);
+  constexpr int KS = gg_slabs(FP8, SLICES * COLS);
+  // Wide fp8 tiles keep every warp busy with the sums, so their results leave
+  // through the TMA unit: written to shared memory (4 KB a warp) and stored from
+  // there under the next tile. Stored by the warps themselves they cost 65 us of
+  // the 626 us of an 8192 x 4096 x 14336 forward product.
+  constexpr bool TMA_OUT = FP8 && SLICES * COLS > 128;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) uint64_t full_bar[GG_MAX_STAGES];   // used in the pair's even CTA
@@ -619,7 +628,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     float acc[GROUPS][2][4];
     const uint32_t tlane = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c0;
     const uint32_t tempty0 = PAIR ? map_to_cta(smem_u32(&tempty_bar[0]), lead) : smem_u32(&tempty_bar[0]);
-    uint8_t* const stage_out = (uint8_t*)(slots + GG_SCALE_BYTES / 4) + (warp - 4) * GG_STAGE_OUT;
+    uint8_t* const stage_out =
+        (uint8_t*)(slots + GG_SCALE_BYTES / 4) + (warp - 4) * (TMA_OUT ? GG_STAGE_WIDE : GG_STAGE_OUT);
     // The place in the output is worked out anew (`again` hides that from the
     // compiler): kept across the contraction it would cost registers there.
     auto store = [&](int again) {
@@ -638,6 +648,40 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         const int col = lane >> 2, piece = lane & 3;
         const uint8_t* get = stage_out + col * 64 + ((piece ^ ((col >> 1) & 3)) << 4);
         const int left = P.r - r0 - piece * 8;
+        if (TMA_OUT && P.tma_out && m >= COLS) {
+          // all of this warp's columns are the group's: one box of them
+          if (lane == 0) tma_store_wait_read();  // of the tile before
+          __syncwarp();
+#pragma unroll
+          for (int g = 0; g < GROUPS; ++g) {
+            uint32_t w[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const __nv_bfloat162 v =
+                  __floats2bfloat162_rn(acc[g][q >> 1][(q & 1) * 2], acc[g][q >> 1][(q & 1) * 2 + 1]);
+              w[q] = *(const uint32_t*)&v;
+            }
+            asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                             put + g * 512),
+                         "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                         : "memory");
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0 && r0 < P.r) {
+            asm volatile(
+                "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+                    &tmAt),
+                "r"(st), "r"(r0), "r"(T.t0 + c0), "r"(P.mode == 1 ? T.seg : 0)
+                : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+          return;
+        }
+        if (TMA_OUT) {
+          if (lane == 0) tma_store_wait_read();
+          __syncwarp();
+        }
         __nv_bfloat16* o = (__nv_bfloat16*)P.out + at + (int64_t)col * P.o_ld + piece * 8;
 #pragma unroll
         for (int g = 0; g < GROUPS; ++g) {
@@ -817,6 +861,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         store(cluster_id);
       }
     }
+    if (TMA_OUT && lane == 0) tma_store_wait_read();  // shared memory outlives its last store
     if (fail && lane == 0) {
       *abortp = 1;
       st_cluster_u32(peer_abort, 1u);
@@ -983,6 +1028,21 @@ static int operand_map(CUtensorMap* tm, const void* ptr, bool fp8, int64_t inner
   return 0;
 }
 
+// Map of bf16 results [group][t][r]: boxes of 64 t by 32 r in the 64-byte swizzle.
+static bool output_map(CUtensorMap* tm, void* ptr, int64_t r, int64_t t, int64_t groups, int64_t ld,
+                       int64_t s_group) {
+  EncodeTiledFn enc = encode_fn();
+  if (groups <= 1) s_group = ld * t;
+  if (enc == nullptr || ld < r || ld % 8 || s_group % 8 || s_group <= 0) return false;
+  cuuint64_t dims[3] = {(cuuint64_t)r, (cuuint64_t)t, (cuuint64_t)groups};
+  cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)s_group * 2};
+  cuuint32_t box[3] = {32, 64, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, ptr, dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 static bool is_fp8_dtype(int dt) { return dt == AQTB200_E4M3 || dt == AQTB200_E5M2; }
 
 // Columns of a tile, at most `most`. A group of `len` rows costs ceil(len / nt)
@@ -1088,7 +1148,7 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   P.idesc = (1u << 4) | (fa << 7) | (fb << 10) | ((uint32_t)P.a_mn << 15) | ((uint32_t)P.b_mn << 16) |
             ((pair ? 16u : 8u) << 24);
   P.b_stage = P.b_mn ? (P.nt / ctas + 63) / 64 * 8192 : P.nt / ctas * 128;
-  P.stages = std::min(GG_MAX_STAGES, GG_RING / (gg_slabs(pair, P.nt) * (GG_A_STAGE + P.b_stage)));
+  P.stages = std::min(GG_MAX_STAGES, (fp8 && P.nt > 128 ? GG_RING_WIDE : GG_RING) / (gg_slabs(fp8, P.nt) * (GG_A_STAGE + P.b_stage)));
   P.buf_cols = P.nt <= 64 ? 64 : P.nt <= 128 ? 128 : 256;
   P.half_kb = 256 / P.buf_cols;
   P.a_scale = d->a_scale; P.sa_g = d->a_scale_group_stride; P.sa_k = d->a_scale_k_stride;
@@ -1154,6 +1214,12 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
     rc = operand_map(&tmBt, Q.out[1], false, d->t, GG_TAIL, d->groups, Q.ld_out[1],
                      Q.ld_out[1] * GG_TAIL, 64);
     if (rc) return rc;
+  }
+
+  if (fp8 && P.nt > 128 && P.out_staged) {
+    // the results' map travels in the place of the tails', which fp8 has no use for
+    P.tma_out = output_map(&tmAt, d->out, d->r, d->t, P.mode == 1 ? groups : 1, d->out_ld,
+                           d->out_group_stride);
   }
 
   const size_t smem = GG_SMEM;
