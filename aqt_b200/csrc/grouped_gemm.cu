@@ -1113,6 +1113,11 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   AQT_REQUIRE(!grouped || (d->groups >= 1 && d->groups <= AQTB200_MAX_GROUPS), AQTB200_EUNSUPPORTED,
               "between 1 and %d groups (got %lld)", AQTB200_MAX_GROUPS, (long long)d->groups);
   const int64_t groups = grouped ? d->groups : 1;
+  if (grouped && d->contract_groups == 1)
+    // the groups' positions are worked out from the sizes and `rows` alone
+    AQT_REQUIRE(fp8 ? d->k / 128 >= d->rows / 128 + std::min(groups, d->rows) : d->k >= d->rows,
+                AQTB200_EINVAL, "k = %lld positions do not hold %lld grouped rows", (long long)d->k,
+                (long long)d->rows);
   if (d->r == 0 || d->t == 0) return 0;
   AQT_REQUIRE(d->out != nullptr, AQTB200_EINVAL, "null output");
   const int64_t lim = (int64_t)1 << 31;

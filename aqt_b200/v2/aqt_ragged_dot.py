@@ -125,6 +125,7 @@ def _backward(step, g, grads):
   cfg, sizes = step.cfg, step.sizes
   m, k, n = step.shape
   be.check_operand(g, 'the cotangent')
+  be.check_same_device(sizes, g)
   if tuple(g.shape) != (m, n):
     raise ValueError(f'the cotangent has shape {tuple(g.shape)}, the result '
                      f'{(m, n)}')

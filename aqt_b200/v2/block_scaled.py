@@ -245,6 +245,7 @@ class BlockScaledDotGeneral:
     need_l, need_r = grads
     m, k, n = step.rows, step.k, step.n
     be.check_operand(g, 'the cotangent')
+    be.check_same_device(step.keep.tensors[0], g)
     want = ((*step.lhs_shape[:-1], n) if step.lhs_axis == -1 else (m, n))
     if tuple(g.shape) != want:
       raise ValueError(f'the cotangent has shape {tuple(g.shape)}, the result '

@@ -616,7 +616,8 @@ int aqtb200_block_quantize(const aqtb200_block_quant_desc* desc, void* stream);
  *
  * r         : extent of the output's contiguous index; t: of its row index.
  * k         : extent of the contraction; contract_groups 1 with groups: number of
- *             grouped rows (bf16), or of padded positions in a and b (fp8; see
+ *             grouped rows (bf16), or of padded positions in a and b (fp8: at
+ *             least 128 * (rows/128 + min(groups, rows)); see
  *             aqtb200_block_quantize).
  * a, b      : element (r, k) of group g at g*a_group_stride + r*a_ld + k, or
  *             with a_mn_major at g*a_group_stride + k*a_ld + r (bf16 only; b

@@ -216,3 +216,33 @@ def test_abi_pack(lib):
   assert lib.aqtb200_pack_bf16(C.byref(v), 264, 8, None) == -1
   assert lib.aqtb200_pack_bf16(C.byref(v), 256, 12, None) == -1
   assert lib.aqtb200_pack_bf16(None, 256, 8, None) == -1
+
+
+def test_abi_gemm_grouped_positions(lib):
+  """The contraction over grouped rows has to hold all of them."""
+  call = lambda d: lib.aqtb200_grouped_gemm(C.byref(d), None, None)
+  common = dict(contract_groups=1, group_sizes=256, groups=3)
+  assert call(_gemm_desc(a_mn_major=1, b_mn_major=1, k=64, rows=65,
+                         **common)) == -1
+  # fp8: 300 rows in three groups take up to 2 + 3 blocks
+  fp8 = dict(a_dtype=_lib.E4M3, b_dtype=_lib.E5M2, a_scale=256, b_scale=256,
+             rows=300, **common)
+  assert call(_gemm_desc(k=4 * 128, **fp8)) == -1
+  assert call(_gemm_desc(k=5 * 128, r=0, **fp8)) == 0
+  assert call(_gemm_desc(k=0, rows=0, r=0, **common)) == 0
+
+
+@pytest.mark.parametrize('q', [False, True])
+def test_cotangent_on_another_device(monkeypatch, q):
+  """Refused before any address of one device meets a kernel of another."""
+  from tests import fake_block_lib
+  fake_block_lib.install(monkeypatch)
+  cfg = bs.dot_general_make()
+  x, w = torch.zeros(4, 128, dtype=BF), torch.zeros(2, 128, 8, dtype=BF)
+  s = torch.tensor([2, 2], dtype=torch.int32)
+  backs = [rd.ragged_dot_vjp(x, w, s, cfg=cfg if q else None)[1]]
+  if q:
+    backs.append(cfg.vjp(x, w[0], DIMS)[1])
+  for back in backs:
+    with pytest.raises(ValueError, match='different devices'):
+      back(torch.zeros(4, 8, dtype=BF, device='meta'))
