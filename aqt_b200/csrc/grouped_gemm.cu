@@ -11,16 +11,18 @@
 // decode batch streams its weights at memory speed. Each tile issues MMAs only
 // as wide as the rows it has (a multiple of 32).
 //
-// Persistent kernel, one CTA pair (cta_group::2) per two SMs, 12 or 20 warps a CTA:
+// Persistent kernel, a CTA pair (cta_group::2) per two SMs, or, for fp8 tiles of
+// at most 128 columns, single CTAs with 128 rows each; 12 or 20 warps a CTA:
 //   warp 0      TMA producer, 128-byte k-slabs, 128-byte swizzle, no multicast
-//   warp 1      MMA issuer (even CTA)
-//   warp 2      scales (fp8)
+//   warp 1      MMA issuer (of a pair: in its even CTA)
+//   warp 2      first the scan of the groups, then scales (fp8)
 //   warps 4-    epilogue: two or four per TMEM lane quarter, up to 64 columns each
-// bf16 accumulates the whole contraction in TMEM (two 256-column accumulators:
-// the epilogue of one tile runs under the next tile's MMAs). fp8 accumulates
-// one 128-block there; the epilogue warps read it, multiply by the two scales
-// and add it to f32 registers (64 a thread) while the tensor core fills the
-// other accumulator.
+// Warps 0 and 1 run whole, with one elected lane issuing. bf16 accumulates the
+// whole contraction in TMEM (two 256-column accumulators: the epilogue of one tile
+// runs under the next tile's MMAs). fp8 accumulates one 128-block there; the
+// epilogue warps read it, multiply by the two scales and add it to f32 registers
+// (up to 64 a thread) while the tensor core fills the other half of TMEM, which
+// holds two or four blocks of a narrow tile.
 //
 // Group sizes stay on the device: every CTA scans them once (prefix sums in
 // shared memory) and finds its tiles from that, so no call waits for the host.
@@ -42,7 +44,6 @@ int sm_count();
 // up to SLICES * COLS columns wide. Four more warps carry the other roles.
 // Registers (setmaxnreg): the first warpgroup gives up what the epilogue takes.
 //   2 slices: 384 threads start with 168: 128 *  88 + 256 * 208 = 64512
-//   3 slices: 512 threads start with 128: 128 *  56 + 384 * 152 = 65536
 //   4 slices: 640 threads start with  96: 128 *  32 + 512 * 112 = 61440 (fp8)
 //                                         128 *  64 + 512 * 104 = 61440 (bf16)
 // k-slabs a stage of the ring holds: two where that leaves four slabs and more in
@@ -74,7 +75,7 @@ struct GGParams {
   // TMEM: two halves of 256 columns, handed over one at a time; each holds
   // `half_kb` accumulators `buf_cols` columns apart (fp8: of consecutive slabs)
   int half_kb, buf_cols;
-  int split;           // CTA pairs of a cluster that share one tile's contraction
+  int split;           // CTAs or pairs of a cluster that share one tile's contraction
   int a_mn, b_mn, bk;  // bk: elements of k per slab
   uint32_t idesc;      // without the column count
   int r, t, rows;
@@ -302,7 +303,7 @@ __device__ __forceinline__ TileAt gg_tile(const GGParams& P, const Segments& S, 
   return T;
 }
 
-// Slabs [kb0, kb1) of the pair's share of a tile's contraction.
+// First slab of share `part` of a tile's contraction.
 __device__ __forceinline__ int share_of(int nkb, int part, int split) {
   return (int)((int64_t)nkb * part / split);
 }
@@ -324,7 +325,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   __shared__ __align__(8) uint64_t empty_bar[GG_MAX_STAGES];  // one per CTA
   __shared__ __align__(8) uint64_t tfull_bar[2];              // one per CTA
   __shared__ __align__(8) uint64_t tempty_bar[2];             // used in the pair's even CTA
-  __shared__ __align__(8) uint64_t sfull_bar[GG_SLOTS];       // scales of a slab; one per CTA
+  __shared__ __align__(8) uint64_t sfull_bar[GG_SLOTS];       // a batch of scales; one per CTA
   __shared__ __align__(8) uint64_t sempty_bar[GG_SLOTS];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -435,7 +436,6 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 
   if (warp < 4) {
     if constexpr (SLICES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    else if constexpr (SLICES == 3) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     else if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   if (warp == 0) {
@@ -502,7 +502,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     __syncwarp();
     if (P.split > 1) cluster_sync_all();
   } else if (warp == 1) {
-    // ---------------- MMA issuer (even CTA, whole warp) ----------------
+    // ---------------- MMA issuer (of a pair: the even CTA; whole warp) ----------------
     if (leader) {
       int stage = 0, cur = 0;
       uint32_t phase = 0;
@@ -606,9 +606,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     if (P.split > 1) cluster_sync_all();
   }
   } else {
-    // ---------------- epilogue (both CTAs, own 128 rows) ----------------
+    // ---------------- epilogue (every CTA, its own 128 rows) ----------------
     if constexpr (SLICES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    else if constexpr (SLICES == 3) asm volatile("setmaxnreg.inc.sync.aligned.u32 152;");
     else if constexpr (FP8) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     // A warp reads its 32 rows by COLS columns with 16x256b loads: a thread then
@@ -1136,10 +1135,6 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   P.sizes = d->group_sizes; P.sizes64 = d->sizes_int64; P.groups = grouped ? (int)d->groups : 0;
   P.num_kb = (int)((k + P.bk - 1) / P.bk);
   const int64_t len = P.mode == 0 ? (d->t + groups - 1) / groups : d->t;
-  // Row scales on both sides double the epilogue's arithmetic: its threads need
-  // more registers than a 256-column tile leaves them (8192 x 4096 x 14336 drhs,
-  // 192 columns 0.82 ms, 256 columns 0.98 ms; forward the other way round, 0.64
-  // against 0.60 ms).
   const bool a_row = fp8 && !d->a_scale_square;
   // Uneven groups: room for one and a half times the average before a second
   // pass. fp8 hands over an accumulator per 128-block, bf16 one per tile.
@@ -1147,7 +1142,7 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   const bool pair = !fp8 || (want <= 128 ? GG_PAIR_NARROW : GG_PAIR_WIDE);
   const int ctas = pair ? 2 : 1, units = std::max(1, sm_count() / ctas);
   P.r_tiles = (int)((d->r + 128 * ctas - 1) / (128 * ctas));
-  P.nt = choose_nt(want, P.r_tiles, !grouped, units, a_row ? 192 : 256, fp8 ? 80 : 8);
+  P.nt = choose_nt(want, P.r_tiles, !grouped, units, 256, fp8 ? 80 : 8);
   P.t_tiles = (int)((d->t + P.nt - 1) / P.nt);
   const uint32_t fa = fp8 ? (d->a_dtype == AQTB200_E5M2) : 1, fb = fp8 ? (d->b_dtype == AQTB200_E5M2) : 1;
   P.idesc = (1u << 4) | (fa << 7) | (fb << 10) | ((uint32_t)P.a_mn << 15) | ((uint32_t)P.b_mn << 16) |
@@ -1235,7 +1230,7 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
                                        : (tiles + rounds - 1) / rounds;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(clusters * ctas * P.split));
-  cfg.blockDim = dim3(gg_threads(P.nt <= 128 ? 2 : a_row ? 3 : 4));
+  cfg.blockDim = dim3(gg_threads(P.nt <= 128 ? 2 : 4));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -1265,7 +1260,7 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   } else {
     if (P.nt <= 64) AQT_GG(true, true, GG_PAIR_NARROW, 2, 32);
     else if (P.nt <= 128) AQT_GG(true, true, GG_PAIR_NARROW, 2, 64);
-    else AQT_GG(true, true, GG_PAIR_WIDE, 3, 64);
+    else AQT_GG(true, true, GG_PAIR_WIDE, 4, 64);
   }
 #undef AQT_GG
   AQT_CUDA_OK(cudaGetLastError()); count_launch();
