@@ -15,14 +15,18 @@
 // at most 128 columns, single CTAs with 128 rows each; 12 or 20 warps a CTA:
 //   warp 0      TMA producer, 128-byte k-slabs, 128-byte swizzle, no multicast
 //   warp 1      MMA issuer (of a pair: in its even CTA)
-//   warp 2      first the scan of the groups, then scales (fp8)
+//   warp 2      first the scan of the groups, then scales (fp8; MX: warp 3 too)
 //   warps 4-    epilogue: two or four per TMEM lane quarter, up to 64 columns each
 // Warps 0 and 1 run whole, with one elected lane issuing. bf16 accumulates the
 // whole contraction in TMEM (two 256-column accumulators: the epilogue of one tile
 // runs under the next tile's MMAs). fp8 accumulates one 128-block there; the
 // epilogue warps read it, multiply by the two scales and add it to f32 registers
 // (up to 64 a thread) while the tensor core fills the other half of TMEM, which
-// holds two or four blocks of a narrow tile.
+// holds two or four blocks of a narrow tile. Wide fp8 tiles whose scales are powers
+// of two (MX) are scaled by the tensor core (kind::mxf8f6f4, one 8-bit exponent for
+// 32 elements, the same for the four MMAs of a block), so that they too accumulate
+// the whole contraction in TMEM: warps 2 and 3 turn the f32 scales into exponents,
+// warp 1 copies them to TMEM four blocks at a time.
 //
 // Group sizes stay on the device: every CTA scans them once (prefix sums in
 // shared memory) and finds its tiles from that, so no call waits for the host.
@@ -60,10 +64,21 @@ constexpr int GG_BATCH = 4;
 constexpr int GG_SLOTS = 2;                  // batches on their way or in use
 constexpr int GG_SLOT = 256 + 128;           // floats a slab: 256 columns, this CTA's 128 rows
 constexpr int GG_SCALE_BYTES = GG_SLOTS * GG_BATCH * GG_SLOT * 4;
+// Scales on the tensor core (MX): two batches of words in TMEM, behind the columns
+// of the first accumulator. Of each, eight columns for 256 columns of the tile and
+// four for 128 rows.
+constexpr int GG_MX_COLS = 224;
+constexpr int GG_MX_AHEAD = 4;               // batches of f32 scales on their way
+// of a slab: 256 columns and 128 rows, each with up to 3 floats more at both ends
+// (whole 16-byte pieces), and how far the first one lies in its piece
+constexpr int GG_MX_ROWS = 264, GG_MX_SHIFTS = GG_MX_ROWS + 136, GG_MX_SLOT = GG_MX_SHIFTS + 4;
 constexpr int GG_STAGE_OUT = 512;            // a warp's staging: 8 columns by 32 rows of bf16,
 constexpr int GG_STAGE_WIDE = 4096;          // or all of its 64 columns
 constexpr int GG_RING_WIDE = 128 * 1024;
 constexpr size_t GG_SMEM = GG_RING + GG_SCALE_BYTES + 16 * GG_STAGE_OUT + 1024;
+constexpr int GG_MX_BYTES = GG_SLOTS * 3 * 512 + GG_MX_AHEAD * GG_BATCH * GG_MX_SLOT * 4;
+static_assert(GG_MAX_STAGES * (GG_A_STAGE + GG_A_STAGE) + GG_MX_BYTES + 16 * GG_STAGE_OUT + 1024 <= GG_SMEM,
+              "shared memory");
 static_assert(GG_RING_WIDE + GG_SCALE_BYTES + 16 * GG_STAGE_WIDE + 1024 <= GG_SMEM, "shared memory");
 constexpr int GG_MAX_SEG = AQTB200_MAX_GROUPS + 1;
 constexpr int GG_TAIL = 64;                  // k-slab of bf16 elements
@@ -75,6 +90,7 @@ struct GGParams {
   // TMEM: two halves of 256 columns, handed over one at a time; each holds
   // `half_kb` accumulators `buf_cols` columns apart (fp8: of consecutive slabs)
   int half_kb, buf_cols;
+  int one_half;        // MX: one accumulator, the scales in the other half
   int split;           // CTAs or pairs of a cluster that share one tile's contraction
   int a_mn, b_mn, bk;  // bk: elements of k per slab
   uint32_t idesc;      // without the column count
@@ -139,6 +155,43 @@ __device__ __forceinline__ void gg_mma4(uint32_t elected, uint32_t d_tmem, uint3
   else GG_MMA4("f16", "1");
 }
 #undef GG_MMA4
+
+
+// The same with the tensor core's own block scales, one 8-bit exponent for 32
+// elements: of the bytes of a column's word in TMEM, the one `idesc` names.
+__device__ __forceinline__ void gg_mma4_scaled(uint32_t elected, uint32_t d_tmem, uint32_t a_lo,
+                                               uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                               uint32_t idesc, uint32_t sa, uint32_t sb,
+                                               uint32_t accumulate) {
+#define GG_MMA_SCALED(ACC)                                                                      \
+  "@q tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], a, b, %7, [%8], [%9], " ACC \
+  ";\n\t"
+#define GG_MMA_STEP                                                                             \
+  "add.u32 x, x, 2;\n\tadd.u32 y, y, 2;\n\tmov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"
+  asm volatile(
+      "{\n\t.reg .pred q, p, t;\n\t.reg .b64 a, b;\n\t.reg .b32 x, y;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\tsetp.ne.b32 p, %5, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+      "mov.b32 x, %1;\n\tmov.b32 y, %3;\n\tmov.b64 a, {x, %2};\n\tmov.b64 b, {y, %4};\n\t"
+      GG_MMA_SCALED("p") GG_MMA_STEP GG_MMA_SCALED("t") GG_MMA_STEP GG_MMA_SCALED("t")
+      GG_MMA_STEP GG_MMA_SCALED("t") "}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(accumulate), "r"(elected), "r"(idesc), "r"(sa),
+      "r"(sb)
+      : "memory");
+#undef GG_MMA_STEP
+#undef GG_MMA_SCALED
+}
+// Copies 32 pieces of 16 bytes, one after the other in shared memory, to four
+// columns of TMEM, the same in every lane quarter, in both CTAs of the pair.
+__device__ __forceinline__ void tc_copy_scales(uint32_t elected, uint32_t tmem, uint32_t at) {
+  // no swizzle, groups of eight pieces 128 bytes apart
+  const uint64_t desc = (uint64_t)((at & 0x3FFFFu) >> 4) | (uint64_t)1 << 16 |
+                        (uint64_t)(128 >> 4) << 32 | (uint64_t)1 << 46;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+      "@q tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(tmem),
+      "l"(desc), "r"(elected)
+      : "memory");
+}
 
 // Hands an accumulator back: only this warp's reads of it have to be over, which
 // the fence before orders (see mbar_arrive_cluster).
@@ -308,17 +361,19 @@ __device__ __forceinline__ int share_of(int nkb, int part, int split) {
   return (int)((int64_t)nkb * part / split);
 }
 
-template <bool FP8, bool A_ROW, bool PAIR, int SLICES, int COLS>
+template <bool FP8, bool A_ROW, bool PAIR, int SLICES, int COLS, bool MX = false>
 __global__ void __launch_bounds__(gg_threads(SLICES), 1)
 grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmAt, const __grid_constant__ CUtensorMap tmBt,
                     GGParams P) {
+  static_assert(!MX || (FP8 && PAIR && SLICES * COLS > 128), "scales on the tensor core: wide fp8 tiles");
+  constexpr bool SUMS = FP8 && !MX;  // the epilogue scales and adds every 128-block
   constexpr int KS = gg_slabs(FP8, SLICES * COLS);
   // Wide fp8 tiles keep every warp busy with the sums, so their results leave
   // through the TMA unit: written to shared memory (4 KB a warp) and stored from
   // there under the next tile. Stored by the warps themselves they cost 65 us of
   // the 626 us of an 8192 x 4096 x 14336 forward product.
-  constexpr bool TMA_OUT = FP8 && SLICES * COLS > 128;
+  constexpr bool TMA_OUT = SUMS && SLICES * COLS > 128;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   __shared__ __align__(8) uint64_t full_bar[GG_MAX_STAGES];   // used in the pair's even CTA
@@ -327,6 +382,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   __shared__ __align__(8) uint64_t tempty_bar[2];             // used in the pair's even CTA
   __shared__ __align__(8) uint64_t sfull_bar[GG_SLOTS];       // a batch of scales; one per CTA
   __shared__ __align__(8) uint64_t sempty_bar[GG_SLOTS];
+  __shared__ __align__(8) uint64_t raw_bar[MX ? 2 * GG_MX_AHEAD : 1];  // MX: f32 scales, by warp
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   __shared__ int nseg_s;
@@ -353,9 +409,11 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       mbar_init(&tempty_bar[s], CTAS * 4 * SLICES);
     }
     for (int s = 0; s < GG_SLOTS; ++s) {
-      mbar_init(&sfull_bar[s], 32);
-      mbar_init(&sempty_bar[s], 4 * SLICES);
+      mbar_init(&sfull_bar[s], MX ? 2 * CTAS : 32);
+      mbar_init(&sempty_bar[s], MX ? 1 : 4 * SLICES);
     }
+    if constexpr (MX)
+      for (int s = 0; s < 2 * GG_MX_AHEAD; ++s) mbar_init(&raw_bar[s], 1);
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -436,7 +494,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 
   if (warp < 4) {
     if constexpr (SLICES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    else if constexpr (FP8) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+    else if constexpr (SUMS) asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     else asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
   if (warp == 0) {
     // ---------------- TMA producer (both CTAs, whole warp) ----------------
@@ -518,6 +576,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       const uint32_t a_lo0 = (uint32_t)a_desc + ring, b_lo0 = (uint32_t)b_desc + ring + (GG_A_STAGE >> 4);
       const uint32_t empty0 = smem_u32(&empty_bar[0]);
       const uint32_t tfull0 = smem_u32(&tfull_bar[0]);
+      const uint32_t sempty0 = smem_u32(&sempty_bar[0]), slots0 = smem_u32(slots);
+      int slot = 0;  // batch of scales (MX)
+      uint32_t sphase = 0;
       for (int tile = cluster_id; tile < total && !fail; tile += num_clusters) {
         const TileAt T = gg_tile<FP8, PAIR>(P, S, nseg, tile, cur);
         const int nkb = __shfl_sync(0xffffffffu, T.nkb, 0);
@@ -529,18 +590,37 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           const int ke = min(ks + KS, kb1);
           uint32_t slab = (uint32_t)(stage * stage_bytes) >> 4;
           for (int kb = ks; kb < ke; ++kb, slab += (uint32_t)slab_bytes >> 4) {
-            if (FP8 ? in_half == 0 : kb == kb0) {
+            if (SUMS ? in_half == 0 : kb == kb0) {
               if (!warp_wait(&tempty_bar[half], hphase ^ 1u, abortp)) { fail = 2; break; }
             }
-            tc_fence_after();
-            gg_mma4<FP8, PAIR>(elected, tmem_base + half * 256u + (FP8 ? in_half * P.buf_cols : 0),
-                         a_lo0 + slab, a_hi, b_lo0 + slab, b_hi, a_step, b_step, idesc,
-                         (!FP8 && kb > kb0) ? 1u : 0u);
             const bool last = kb + 1 == kb1;
-            if (FP8 ? (++in_half == P.half_kb || last) : last) {
+            if constexpr (MX) {
+              const int j = (kb - kb0) & (GG_BATCH - 1);
+              const uint32_t ts = tmem_base + (P.one_half ? 256u : GG_MX_COLS) + slot * 16u;
+              if (j == 0) {
+                if (!warp_wait(&sfull_bar[slot], sphase, abortp)) { fail = 2; break; }
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 3; ++c)
+                  tc_copy_scales(elected, ts + c * 4, slots0 + (slot * 3 + c) * 512);
+              }
+              tc_fence_after();
+              gg_mma4_scaled(elected, tmem_base + half * 256u, a_lo0 + slab, a_hi, b_lo0 + slab, b_hi,
+                             idesc | (uint32_t)j << 29 | (uint32_t)j << 4, ts + 8, ts, kb > kb0 ? 1u : 0u);
+              if (j == GG_BATCH - 1 || last) {
+                gg_commit<PAIR>(elected, sempty0 + slot * 8, lead);
+                if (++slot == GG_SLOTS) { slot = 0; sphase ^= 1u; }
+              }
+            } else {
+              tc_fence_after();
+              gg_mma4<FP8, PAIR>(elected, tmem_base + half * 256u + (FP8 ? in_half * P.buf_cols : 0),
+                                 a_lo0 + slab, a_hi, b_lo0 + slab, b_hi, a_step, b_step, idesc,
+                                 (!FP8 && kb > kb0) ? 1u : 0u);
+            }
+            if (SUMS ? (++in_half == P.half_kb || last) : last) {
               gg_commit<PAIR>(elected, tfull0 + half * 8, lead);
               in_half = 0;
-              half ^= 1u;
+              half = MX && P.one_half ? 0u : half ^ 1u;
               if (half == 0) hphase ^= 1u;
             }
           }
@@ -561,7 +641,78 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     // ---------------- scales, ahead of the epilogue (one warp) ----------------
     // A load issued by the epilogue warps a slab ahead put a memory round trip on
     // every 128-block (0.7 us a slab on the 8192 x 28672 decode, 90 us in all).
-    if (FP8 && warp == 2) {
+    if constexpr (MX) {
+      // Warp 2: of the columns; warp 3: of this CTA's rows. GG_MX_AHEAD batches are
+      // on their way at once, across tiles, as bulk copies: loaded and waited for
+      // one by one a batch took up to 8000 clocks, in 4-byte asynchronous copies
+      // 2100, and its MMAs take 1800.
+      const bool rows = warp == 3, square = rows && !A_ROW;
+      int slot = 0, cur = 0, issued = 0, done = 0;
+      uint32_t phase = 0;
+      const uint32_t sfull0 = map_to_cta(smem_u32(&sfull_bar[0]), lead);
+      uint64_t* const bars = raw_bar + (rows ? GG_MX_AHEAD : 0);
+      float* const raw = slots + GG_SLOTS * 384 + (rows ? GG_MX_ROWS : 0);
+      int* const shifts = (int*)(slots + GG_SLOTS * 384 + GG_MX_SHIFTS + (rows ? 1 : 0));
+      auto convert = [&]() {
+        const int at = (done % GG_MX_AHEAD) * GG_BATCH * GG_MX_SLOT;
+        if (!warp_wait(&bars[done % GG_MX_AHEAD], (done / GG_MX_AHEAD) & 1, abortp)) return false;
+        uint32_t w[8] = {0};
+#pragma unroll
+        for (int b = 0; b < GG_BATCH; ++b) {
+          const float* x = raw + at + b * GG_MX_SLOT + (shifts[at + b * GG_MX_SLOT] & 3);
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < (A_ROW ? 4 : 1) || !rows)
+              w[e] |= (__float_as_uint(x[square ? 0 : e * 32 + lane]) >> 23 & 255u) << (8 * b);
+        }
+        if (square) w[1] = w[2] = w[3] = w[0];
+        ++done;
+        if (!warp_wait(&sempty_bar[slot], phase ^ 1u, abortp)) return false;
+        uint4* out = (uint4*)slots + slot * 96 + lane + (rows ? 64 : 0);
+        out[0] = make_uint4(w[0], w[1], w[2], w[3]);
+        if (!rows) out[32] = make_uint4(w[4], w[5], w[6], w[7]);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0)
+          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(sfull0 + slot * 8)
+                       : "memory");
+        if (++slot == GG_SLOTS) { slot = 0; phase ^= 1u; }
+        return true;
+      };
+      for (int tile = cluster_id; tile < total && !fail; tile += num_clusters) {
+        const TileAt T = gg_tile<FP8, PAIR>(P, S, nseg, tile, cur);
+        const int row = min(T.r0 + (int)rank * 128, P.r - 1);
+        const int have = !rows ? T.tvalid : A_ROW ? min(128, P.r - row) : 1;
+        const int64_t step_k = rows ? P.sa_k : P.sb_k;
+        const float* p = !rows ? P.b_scale + T.t0
+                               : P.a_scale + (P.mode == 0 ? (int64_t)T.seg * P.sa_g : 0) +
+                                     (int64_t)(A_ROW ? row : row >> 7) * P.sa_r;
+        p += (T.k0 / 128 + lane) * step_k;  // a lane each for the slabs of a batch
+        for (int kb = 0; kb < T.nkb; kb += GG_BATCH, p += GG_BATCH * step_k) {
+          uint64_t* const bar = &bars[issued % GG_MX_AHEAD];
+          const int at = ((issued % GG_MX_AHEAD) * GG_BATCH + lane) * GG_MX_SLOT;
+          // whole 16-byte pieces around the scales
+          const uintptr_t first = (uintptr_t)p & ~(uintptr_t)15;
+          const bool mine = lane < min(GG_BATCH, T.nkb - kb);
+          const uint32_t bytes = mine ? (uint32_t)((((uintptr_t)(p + have) + 15) & ~(uintptr_t)15) - first) : 0u;
+          const uint32_t all = __reduce_add_sync(0xffffffffu, bytes);
+          if (lane == 0) mbar_expect_tx(bar, all);
+          if (mine) shifts[at] = (int)((uintptr_t)p - first) >> 2;
+          __syncwarp();
+          if (mine) bulk_load(raw + at, (const void*)first, bytes, bar);
+          if (++issued - done == GG_MX_AHEAD && !convert()) { fail = 4; break; }
+          __syncwarp();
+        }
+      }
+      while (done < issued && !fail)
+        if (!convert()) fail = 4;
+      if (fail && lane == 0) {
+        *abortp = 1;
+        st_cluster_u32(peer_abort, 1u);
+        if (P.status) atomicCAS(P.status, 0, 4);
+      }
+    }
+    if (SUMS && warp == 2) {
       int slot = 0, cur = 0;
       uint32_t phase = 0;
       for (int tile = cluster_id; tile < total && !fail; tile += num_clusters) {
@@ -608,7 +759,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   } else {
     // ---------------- epilogue (every CTA, its own 128 rows) ----------------
     if constexpr (SLICES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-    else if constexpr (FP8) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
+    else if constexpr (SUMS) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
     // A warp reads its 32 rows by COLS columns with 16x256b loads: a thread then
     // holds, of every 8 columns, two neighbouring ones in four rows,
@@ -628,7 +779,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const uint32_t tlane = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)c0;
     const uint32_t tempty0 = PAIR ? map_to_cta(smem_u32(&tempty_bar[0]), lead) : smem_u32(&tempty_bar[0]);
     uint8_t* const stage_out =
-        (uint8_t*)(slots + GG_SCALE_BYTES / 4) + (warp - 4) * (TMA_OUT ? GG_STAGE_WIDE : GG_STAGE_OUT);
+        (uint8_t*)slots + (MX ? GG_MX_BYTES : GG_SCALE_BYTES) + (warp - 4) * (TMA_OUT ? GG_STAGE_WIDE : GG_STAGE_OUT);
     // The place in the output is worked out anew (`again` hides that from the
     // compiler): kept across the contraction it would cost registers there.
     auto store = [&](int again) {
@@ -740,7 +891,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         for (int i = 0; i < 8; ++i) acc[g][i >> 2][i & 3] = 0.f;
       int in_batch = 0;  // slabs of the current batch of scales already used
       for (int kb = kb0; kb < kb1;) {
-        if (FP8 && in_batch == 0) {
+        if (SUMS && in_batch == 0) {
           const int got = mbar_wait(&sfull_bar[slot], sphase, abortp) ? 1 : 0;
           if (!__all_sync(0xffffffffu, got)) { fail = 3; break; }
         }
@@ -763,7 +914,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             }
           }
         };
-        if (FP8 && HALF_KB == 1) factors();  // while the MMAs still run
+        if (SUMS && HALF_KB == 1) factors();  // while the MMAs still run
         int ok = mbar_wait(&tfull_bar[half], hphase, abortp) ? 1 : 0;
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) { fail = 3; break; }
@@ -773,11 +924,11 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           __syncwarp();
           if (lane == 0) gg_arrive<PAIR>(tempty0 + half * 8);
         };
-        const int here = FP8 && HALF_KB > 1 ? min(HALF_KB, kb1 - kb) : 1;  // accumulators in this half
+        const int here = SUMS && HALF_KB > 1 ? min(HALF_KB, kb1 - kb) : 1;  // accumulators in this half
         if (cols > 0) {
           uint32_t ta = tlane + half * 256u;
           for (int b = 0; b < here; ++b, ta += P.buf_cols, sc += GG_SLOT) {
-            if (FP8 && HALF_KB > 1) factors();
+            if (SUMS && HALF_KB > 1) factors();
 #pragma unroll
             for (int c = 0; c < COLS; c += 32) {
               if (c >= cols) break;  // the same for the whole warp
@@ -794,7 +945,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     float* a = &acc[c / 8 + g][h][i];
                     float x = __uint_as_float(p[h][g * 4 + i]);
                     float y = __uint_as_float(p[h][g * 4 + i + 1]);
-                    if constexpr (!FP8) {
+                    if constexpr (!SUMS) {
                       a[0] = x;
                       a[1] = y;
                     } else {
@@ -811,9 +962,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           }
         }
         hand_back();
-        half ^= 1u;
+        half = MX && P.one_half ? 0u : half ^ 1u;
         if (half == 0) hphase ^= 1u;
-        if constexpr (FP8) {
+        if constexpr (SUMS) {
           kb += here;
           in_batch += here;
           if (in_batch == GG_BATCH || kb == kb1) {
@@ -1139,16 +1290,38 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   // Uneven groups: room for one and a half times the average before a second
   // pass. fp8 hands over an accumulator per 128-block, bf16 one per tile.
   const int64_t want = grouped && P.mode == 0 ? len + len / 2 : len;
+  // Scales that are powers of two can be left to the tensor core, which then sums
+  // the whole contraction (8192 x 4096 x 14336: 459 / 446 / 550 us against 588 / 537
+  // / 711; 300 x 4096 x 4096: 22 / 22 / 27 against 29 / 29 / 26). Its sums drop what does not fit 24 bits, each step of 32 products
+  // less than 2^-23 of the running sum (measured, all products positive: 2^-26 a
+  // step, 8e-6 over 14336): nothing beside a bf16 result's rounding of 2^-9 as long
+  // as the steps' total stays below 2^-10. f32 results keep the f32 registers.
+  const bool mx = fp8 && d->scales_po2 && want > 128 && d->out_dtype == AQTB200_BF16 &&
+                  P.num_kb * 4 <= 1 << 13 && (d->a_scale_square || d->a_scale_r_stride == 1);
   const bool pair = !fp8 || (want <= 128 ? GG_PAIR_NARROW : GG_PAIR_WIDE);
   const int ctas = pair ? 2 : 1, units = std::max(1, sm_count() / ctas);
   P.r_tiles = (int)((d->r + 128 * ctas - 1) / (128 * ctas));
-  P.nt = choose_nt(want, P.r_tiles, !grouped, units, 256, fp8 ? 80 : 8);
+  // Tiles, or the most there can be: groups that end inside a tile add one each.
+  const auto tiles_of = [&](int nt) {
+    const int64_t per = (d->t + nt - 1) / nt;
+    return P.r_tiles * (P.mode == 1 ? groups * per
+                        : grouped   ? d->t / nt + std::min<int64_t>(d->groups + 1, d->t)
+                                    : per);
+  };
+  // Scales in TMEM leave two accumulators of 224 columns, or one of 256: enough
+  // where no CTA pair has a second tile to overlap (1024 x 4096 x 4096, 64 tiles on
+  // 74 pairs and not 80: 25 / 25 / 37 us against 37 / 37 / 36).
+  P.one_half = mx && tiles_of(256) <= units;
+  P.nt = choose_nt(want, P.r_tiles, !grouped, units, mx && !P.one_half ? GG_MX_COLS : 256,
+                   fp8 && !mx ? 80 : 8);
   P.t_tiles = (int)((d->t + P.nt - 1) / P.nt);
   const uint32_t fa = fp8 ? (d->a_dtype == AQTB200_E5M2) : 1, fb = fp8 ? (d->b_dtype == AQTB200_E5M2) : 1;
   P.idesc = (1u << 4) | (fa << 7) | (fb << 10) | ((uint32_t)P.a_mn << 15) | ((uint32_t)P.b_mn << 16) |
             ((pair ? 16u : 8u) << 24);
+  // with scales: no accumulator type, 8-bit exponents
+  if (mx) P.idesc = (P.idesc & ~(1u << 4)) | (1u << 23);
   P.b_stage = P.b_mn ? (P.nt / ctas + 63) / 64 * 8192 : P.nt / ctas * 128;
-  P.stages = std::min(GG_MAX_STAGES, (fp8 && P.nt > 128 ? GG_RING_WIDE : GG_RING) / (gg_slabs(fp8, P.nt) * (GG_A_STAGE + P.b_stage)));
+  P.stages = std::min(GG_MAX_STAGES, (fp8 && !mx && P.nt > 128 ? GG_RING_WIDE : GG_RING) / (gg_slabs(fp8, P.nt) * (GG_A_STAGE + P.b_stage)));
   P.buf_cols = P.nt <= 64 ? 64 : P.nt <= 128 ? 128 : 256;
   P.half_kb = 256 / P.buf_cols;
   P.a_scale = d->a_scale; P.sa_g = d->a_scale_group_stride; P.sa_k = d->a_scale_k_stride;
@@ -1160,11 +1333,7 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
                  (P.mode == 0 || !grouped || d->out_group_stride % 8 == 0);
   P.status = status;
 
-  // Tiles, or the most there can be: groups that end inside a tile add one each.
-  const int64_t t_most = P.mode == 1 ? groups * P.t_tiles
-                         : grouped   ? d->t / P.nt + std::min<int64_t>(d->groups + 1, d->t)
-                                     : P.t_tiles;
-  const int64_t tiles = t_most * P.r_tiles;
+  const int64_t tiles = tiles_of(P.nt);
   AQT_REQUIRE(tiles < lim - 65536, AQTB200_EUNSUPPORTED, "more than 2^31 output tiles");
   int dev = 0;
   AQT_CUDA_OK(cudaGetDevice(&dev));
@@ -1216,7 +1385,7 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
     if (rc) return rc;
   }
 
-  if (fp8 && P.nt > 128 && P.out_staged) {
+  if (fp8 && !mx && P.nt > 128 && P.out_staged) {
     // the results' map travels in the place of the tails', which fp8 has no use for
     P.tma_out = output_map(&tmAt, d->out, d->r, d->t, P.mode == 1 ? groups : 1, d->out_ld,
                            d->out_group_stride);
@@ -1253,6 +1422,9 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
     if (P.nt <= 64) AQT_GG(false, false, true, 2, 32);
     else if (P.nt <= 128) AQT_GG(false, false, true, 2, 64);
     else AQT_GG(false, false, true, 4, 64);
+  } else if (mx) {
+    if (a_row) AQT_GG(true, true, true, 4, 64, true);
+    else AQT_GG(true, false, true, 4, 64, true);
   } else if (!a_row) {
     if (P.nt <= 64) AQT_GG(true, false, GG_PAIR_NARROW, 2, 32);
     else if (P.nt <= 128) AQT_GG(true, false, GG_PAIR_NARROW, 2, 64);

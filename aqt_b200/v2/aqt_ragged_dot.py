@@ -113,7 +113,8 @@ def _forward(lhs, rhs, sizes, cfg, out_dtype, grads):
       w_n, w = be.quantize(rhs, cfg.fwd_dtype, need_l, True, True, cfg.po2_scale)
     l, l_t = be.quantize(lhs, cfg.fwd_dtype, True, need_r, False, cfg.po2_scale,
                          sizes if need_r else None)
-    out = be.fp8_rows(l, w, lhs.shape[1], out_dtype, lhs.device, sizes)
+    out = be.fp8_rows(l, w, lhs.shape[1], out_dtype, lhs.device, sizes,
+                      cfg.po2_scale and not isinstance(rhs, aqt_tensor.QTensor))
     if step is not None:
       step.lhs, step.rhs = l_t, w_n if need_l else None
       step.keep = be.Residuals(step.lhs, step.rhs)
@@ -144,11 +145,12 @@ def _backward(step, g, grads):
     q, q_t = be.quantize(g, cfg.bwd_dtype, need_l, need_r, False, cfg.po2_scale,
                          sizes if need_r else None)
     if need_l:
-      dlhs = be.fp8_rows(q, step.rhs, n, step.lhs_dtype, g.device, sizes)
+      dlhs = be.fp8_rows(q, step.rhs, n, step.lhs_dtype, g.device, sizes,
+                         cfg.po2_scale)
     if need_r:
       # positions along the groups' padded rows, as both operands were laid out
       drhs = be.fp8_contract_rows(step.lhs, q_t, step.lhs.ld, m, step.rhs_dtype,
-                                  g.device, sizes)
+                                  g.device, sizes, cfg.po2_scale)
   return dlhs, drhs
 
 

@@ -20,7 +20,10 @@ weights serves the forward product and dlhs:
 
 A block: a = max|x|, s = max((a or 1) / bound, 2^-126) in f32 [, up to a power of
 two], q = fp8(x * (1 / s)); products of 128 are summed on the tensor core, scaled
-and added in f32, and the result is rounded once to the output's dtype. A NaN or
+and added in f32, and the result is rounded once to the output's dtype. With
+po2_scale, more than 128 rows and a bfloat16 result the tensor core scales and sums
+by itself, 1.3 times as fast; its sums drop what does not fit 24 bits (up to 2^-23
+of the running sum for each 32 products). A NaN or
 an infinity in a block makes that block's scale, and what is computed from it,
 NaN or infinite, as absmax calibration does (calibration.py:117-157).
 """
@@ -228,7 +231,8 @@ class BlockScaledDotGeneral:
       l, l_t = be.quantize(x, self.fwd_dtype, True, need_r, False,
                            self.po2_scale)
       m, k = x.shape
-      out = be.fp8_rows(l, w, k, out_dtype, device)
+      out = be.fp8_rows(l, w, k, out_dtype, device,
+                        po2=self.po2_scale and grads is not None)
       step = None
       if need_l or need_r:
         step = _Step()
@@ -258,11 +262,13 @@ class BlockScaledDotGeneral:
       q, q_t = be.quantize(gm, self.bwd_dtype, need_l, need_r, False,
                            self.po2_scale)
       if need_l:
-        dlhs = be.fp8_rows(q, step.rhs, n, step.lhs_dtype, device)
+        dlhs = be.fp8_rows(q, step.rhs, n, step.lhs_dtype, device,
+                           po2=self.po2_scale)
       if need_r:
         # [K, N] as rhs lies: its last axis is the output's contiguous one
         b, a = (step.lhs, q_t) if step.rhs_axis == -2 else (q_t, step.lhs)
-        drhs = be.fp8_contract_rows(b, a, m, m, step.rhs_dtype, device)
+        drhs = be.fp8_contract_rows(b, a, m, m, step.rhs_dtype, device,
+                                    po2=self.po2_scale)
     if need_l:
       if step.lhs_axis == -2:
         dlhs = dlhs.transpose(0, 1)

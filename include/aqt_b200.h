@@ -625,6 +625,12 @@ int aqtb200_block_quantize(const aqtb200_block_quant_desc* desc, void* stream);
  * a_scale   : fp8 only. f32 of (r, block kb) at g*a_scale_group_stride +
  *             kb*a_scale_k_stride + (a_scale_square ? r/128 : r)*a_scale_r_stride.
  * b_scale   : f32 of (t, kb) at kb*b_scale_k_stride + t.
+ * scales_po2: fp8: every scale is a power of two (po2_scale of
+ *             aqtb200_block_quantize). Products of more than 128 rows t (grouped:
+ *             of more than 85 a group on average) with a bf16 result and k up to
+ *             2^18 are then scaled and summed on the tensor core, which takes a
+ *             scale's exponent and nothing else of it, and reads the scales in
+ *             whole aligned 16-byte pieces.
  * group_sizes, groups, sizes_int64: as for aqtb200_block_quantize; at most
  *             AQTB200_MAX_GROUPS groups.
  * rows      : number of grouped rows (contract_groups 1; t otherwise).
@@ -641,7 +647,7 @@ typedef struct aqtb200_grouped_gemm_desc {
   int64_t a_ld, a_group_stride;
   const void* b;
   int64_t b_ld;
-  int32_t a_mn_major, b_mn_major, a_scale_square, sizes_int64;
+  int32_t a_mn_major, b_mn_major, a_scale_square, sizes_int64, scales_po2;
   const float* a_scale;
   int64_t a_scale_group_stride, a_scale_k_stride, a_scale_r_stride;
   const float* b_scale;

@@ -180,3 +180,41 @@ def test_ragged_frozen_and_autograd():
     if cfg is not None:
       qt = bs.block_quantize(w, 1, square=True)
       assert torch.equal(rd.ragged_dot(x, qt, s, cfg=cfg), out)
+
+
+def test_scales_named_powers_of_two_are(monkeypatch):
+  """The product is told so exactly where every scale it gets is one."""
+  import ctypes as C
+  from aqt_b200 import _lib
+  lib = _lib.load()
+  told = []
+  gemm = lib.aqtb200_grouped_gemm
+
+  def spy(desc, *args):
+    d = desc._obj
+    told.append(d.scales_po2)
+    if d.scales_po2:
+      nb = -(-d.k // 128)
+      b = np.frombuffer((C.c_char * (4 * nb * d.t)).from_address(d.b_scale),
+                        np.float32)
+      if not d.group_sizes or d.contract_groups == 0:
+        assert (np.frexp(b)[0] == 0.5).all()
+    return gemm(desc, *args)
+
+  monkeypatch.setattr(lib, 'aqtb200_grouped_gemm', spy, raising=False)
+  x, w, g = (_data((140, 200), torch.bfloat16, 60), _data(
+      (200, 30), torch.bfloat16, 61), _data((140, 30), torch.bfloat16, 62))
+  s = torch.tensor([100, 40], dtype=torch.int32)
+  wg = _data((2, 200, 30), torch.bfloat16, 63)
+  for po2 in (False, True):
+    cfg = bs.dot_general_make(po2_scale=po2)
+    for run in (lambda: cfg.vjp(x, w, DIMS),
+                lambda: rd.ragged_dot_vjp(x, wg, s, cfg=cfg)):
+      told.clear()
+      run()[1](g)
+      assert told == [int(po2)] * 3
+    told.clear()
+    cfg(x, bs.block_quantize(w, 0, square=True), DIMS)
+    rd.ragged_dot(x, bs.block_quantize(wg, 1, square=True), s, cfg=cfg)
+    rd.ragged_dot(x, wg, s)
+    assert told == [0, 0, 0]
