@@ -1337,6 +1337,9 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   AQT_REQUIRE(tiles < lim - 65536, AQTB200_EUNSUPPORTED, "more than 2^31 output tiles");
   int dev = 0;
   AQT_CUDA_OK(cudaGetDevice(&dev));
+  // A thread whose first CUDA call this is (a backward pass runs on one of its own)
+  // has no context yet, and the driver call that encodes a map needs one.
+  AQT_CUDA_OK(cudaSetDevice(dev));
   // Few tiles: the contraction of each is shared by up to four of a cluster, which
   // add their sums through distributed shared memory, in order -- as many as keep
   // every cluster on the device at once (1 x 4096 x 4096 fp8 on CTA pairs: one a

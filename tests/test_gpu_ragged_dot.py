@@ -374,3 +374,30 @@ def test_expert_layer():
     _done()
     for a, b in zip(got, want):
       assert float((a - b).norm() / b.norm()) < tol
+
+
+@pytest.mark.parametrize('what', ['bf16', 'frozen', 'backward'])
+def test_first_call_of_a_thread(what):
+  """A thread that has made no CUDA call yet."""
+  import threading
+  x, w, g = (_data((40, 64), torch.bfloat16, 60), _data(
+      (2, 64, 72), torch.bfloat16, 61), _data((40, 72), torch.bfloat16, 62))
+  sizes = _sizes([25, 10])
+  cfg = bs.dot_general_make()
+  if what == 'bf16':
+    run = lambda: (rd.ragged_dot(x, w, sizes),)
+  elif what == 'frozen':
+    qt = bs.block_quantize(w, 1, square=True)
+    run = lambda: (rd.ragged_dot(x, qt, sizes, cfg=cfg),)
+  else:
+    back = rd.ragged_dot_vjp(x, w, sizes)[1]
+    run = lambda: back(g)
+  want = run()
+  _done()
+  got = []
+  t = threading.Thread(target=lambda: got.extend(run()))
+  t.start()
+  t.join()
+  _done()
+  assert len(got) == len(want)
+  assert all(torch.equal(a, b) for a, b in zip(got, want))
