@@ -179,6 +179,8 @@ SYMBOLS = {
         C.POINTER(GroupedGemmDesc), C.c_void_p, C.c_void_p]),
     'aqtb200_pack_bf16': (C.c_int, [
         C.POINTER(View), C.c_void_p, C.c_int64, C.c_void_p]),
+    'aqtb200_pack_bf16_groups': (C.c_int, [
+        C.POINTER(View), C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]),
     'aqtb200_dequantize': (C.c_int, [
         C.POINTER(View), C.POINTER(View), C.c_int32, C.c_void_p, C.c_void_p]),
     'aqtb200_set_device': (C.c_int, [C.c_int]),

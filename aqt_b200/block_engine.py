@@ -316,16 +316,18 @@ def _fits(x, contiguous_axis, other_axis):
   return all(s > 0 and s % 8 == 0 for s in strides)
 
 
-def pack(x):
-  """A copy of bf16 [.., R, C] with C contiguous and rows padded to 16 bytes."""
+def pack(x, group_sizes=None):
+  """A copy of bf16 [.., R, C] with C contiguous and rows padded to 16 bytes;
+  given the sizes of x's groups, of those matrices only whose group has rows."""
   ld = (max(x.shape[-1], 1) + 7) & -8
   batch = x.shape[0] if x.ndim == 3 else 1
   buf = _empty_out((*x.shape[:-1], ld), torch.bfloat16, x.device)
   v = _lib.View(x.data_ptr(), _lib.BF16, 0, batch, 1, x.shape[-2], x.shape[-1],
                 x.stride(0) if x.ndim == 3 else 0, 0, x.stride(-2), x.stride(-1))
-  _lib.check(engine._call(  # pylint: disable=protected-access
-      _lib.load().aqtb200_pack_bf16, C.byref(v), buf.data_ptr(), ld,
-      engine._stream()), 'pack_bf16')  # pylint: disable=protected-access
+  sizes, _, int64 = _sizes(group_sizes)
+  _check(engine._call(  # pylint: disable=protected-access
+      _lib.load().aqtb200_pack_bf16_groups, C.byref(v), sizes, int64,
+      buf.data_ptr(), ld, engine._stream()), 'pack_bf16')  # pylint: disable=protected-access
   return buf[..., :x.shape[-1]]
 
 
@@ -334,26 +336,29 @@ def rows_for_tma(x):
   return x if _fits(x, -1, -2) else pack(x)
 
 
+def matrices_for_tma(x, group_sizes):
+  """x [G, R, C] bf16 itself, if a tensor map can describe it with either of the
+  last axes contiguous, or a packed copy."""
+  return x if _fits(x, -1, -2) or _fits(x, -2, -1) else pack(x, group_sizes)
+
+
 def _ld(x, axis):
   """Stride of `axis`, made a valid one where the axis has a single entry."""
   return x.stride(axis) if x.shape[axis] > 1 else (max(x.shape[-1], x.shape[-2]) + 7) & -8
 
 
 def bf16_rows(tokens, a, contract_axis, group_sizes, out_dtype):
-  """out[t] = tokens[t] . a[g(t)], contracting a's `contract_axis` (1 or 2)."""
+  """out[t] = tokens[t] . a[g(t)], contracting a's `contract_axis` (1 or 2);
+  tokens from rows_for_tma, a from matrices_for_tma."""
   t, k = tokens.shape
   keep = 3 - contract_axis
   r = a.shape[keep]
   dev = tokens.device
   out = _empty_out((t, r), out_dtype, dev)
-  tokens = rows_for_tma(tokens)
   if _fits(a, contract_axis, keep):
     mn, ld = 0, _ld(a, keep)
-  elif _fits(a, keep, contract_axis):
-    mn, ld = 1, _ld(a, contract_axis)
   else:
-    a = pack(a)  # its last axis is contiguous
-    mn, ld = int(contract_axis == 1), a.stride(1)
+    mn, ld = 1, _ld(a, contract_axis)
   sizes, groups, int64 = _sizes(group_sizes)
   _gemm(_lib.GroupedGemmDesc(
       0, _lib.BF16, _lib.BF16, engine._TORCH_CODE[out_dtype], r, t, k, t,  # pylint: disable=protected-access
@@ -364,12 +369,12 @@ def bf16_rows(tokens, a, contract_axis, group_sizes, out_dtype):
 
 
 def bf16_contract_rows(lhs, g, group_sizes, out_dtype):
-  """out[e] = lhs_e^T . g_e for the rows of every group e."""
+  """out[e] = lhs_e^T . g_e for the rows of every group e; both from
+  rows_for_tma."""
   rows, t = lhs.shape
   r = g.shape[1]
   dev = lhs.device
   out = _empty_out((group_sizes.shape[0], t, r), out_dtype, dev)
-  lhs, g = rows_for_tma(lhs), rows_for_tma(g)
   sizes, groups, int64 = _sizes(group_sizes)
   d = _lib.GroupedGemmDesc(
       1, _lib.BF16, _lib.BF16, engine._TORCH_CODE[out_dtype], r, t, rows, rows,  # pylint: disable=protected-access
@@ -385,14 +390,15 @@ def bf16_contract_rows(lhs, g, group_sizes, out_dtype):
 
 
 class Residuals:
-  """Buffers a backward pass reads. They are torch allocations of the forward
+  """Buffers a backward pass reads (tensors, or the memory of Sides). They are torch allocations of the forward
   pass's stream; used on another one, the allocator is told before they can be
   handed out again."""
 
   __slots__ = ('stream', 'tensors')
 
-  def __init__(self, *sides):
-    self.tensors = [s.keep for s in sides if s is not None]
+  def __init__(self, *of):
+    self.tensors = [s.keep if isinstance(s, Side) else s for s in of
+                    if s is not None]
     self.stream = engine._stream()  # pylint: disable=protected-access
 
   def about_to_use(self):

@@ -51,7 +51,7 @@ def ragged_dot(lhs, rhs, group_sizes, cfg=None, preferred_element_type=None):
 def ragged_dot_vjp(lhs, rhs, group_sizes, cfg=None, preferred_element_type=None):
   """(out, backprop) of ragged_dot with backprop(g) -> (dlhs, drhs).
 
-  backprop reads group_sizes (and, without cfg, the operands) again: they have to
+  backprop may read group_sizes and, without cfg, the operands again: they have to
   hold what they held at the call.
   """
   if isinstance(rhs, aqt_tensor.QTensor):
@@ -88,8 +88,8 @@ def _check(lhs, rhs, group_sizes, cfg, preferred):
 
 
 class _Step:
-  __slots__ = ('cfg', 'lhs', 'rhs', 'sizes', 'keep', 'lhs_dtype', 'rhs_dtype',
-               'shape')
+  __slots__ = ('cfg', 'lhs', 'rhs', 'copied', 'sizes', 'keep', 'lhs_dtype',
+               'rhs_dtype', 'shape')
 
 
 def _forward(lhs, rhs, sizes, cfg, out_dtype, grads):
@@ -102,10 +102,15 @@ def _forward(lhs, rhs, sizes, cfg, out_dtype, grads):
       step.lhs_dtype, step.rhs_dtype = lhs.dtype, rhs.dtype
       step.shape = (*lhs.shape, rhs.shape[2])
     if cfg is None:
-      out = be.bf16_rows(lhs, rhs, 1, sizes, out_dtype)
+      l, w = be.rows_for_tma(lhs), be.matrices_for_tma(rhs, sizes)
+      out = be.bf16_rows(l, w, 1, sizes, out_dtype)
       if step is not None:
-        step.lhs = lhs if need_r else None
-        step.rhs = rhs if need_l else None
+        # a copy, where one had to be made, serves the backward pass too
+        step.lhs = l if need_r else None
+        step.rhs = w if need_l else None
+        step.copied = l is not lhs, w is not rhs
+        step.keep = be.Residuals(*(t for t, c in zip(
+            (step.lhs, step.rhs), step.copied) if c))
       return out, step
     if isinstance(rhs, aqt_tensor.QTensor):
       w, w_n = block_scaled._frozen_operand(rhs, -2), None  # pylint: disable=protected-access
@@ -135,6 +140,8 @@ def _backward(step, g, grads):
     if g.dtype != torch.bfloat16:
       g = g.to(torch.bfloat16)
     with be.on_device_of(g):
+      step.keep.about_to_use()
+      g = be.rows_for_tma(g)
       if need_l:
         dlhs = be.bf16_rows(g, step.rhs, 2, sizes, step.lhs_dtype)
       if need_r:
@@ -162,9 +169,12 @@ class _RaggedDot(torch.autograd.Function):
                          ctx.needs_input_grad[:2])
     if cfg is None:
       # operands themselves: saved the way torch watches for writes into them
-      ctx.save_for_backward(sizes, step.lhs if step.lhs is None else lhs,
-                            step.rhs if step.rhs is None else rhs)
-      step.lhs = step.rhs = None
+      own = [t is not None and not c
+             for t, c in zip((step.lhs, step.rhs), step.copied)]
+      ctx.save_for_backward(sizes, lhs if own[0] else None,
+                            rhs if own[1] else None)
+      step.lhs = None if own[0] else step.lhs
+      step.rhs = None if own[1] else step.rhs
     else:
       ctx.save_for_backward(sizes)
     step.sizes = None
@@ -176,11 +186,11 @@ class _RaggedDot(torch.autograd.Function):
   def backward(ctx, g):
     step = ctx.step
     step.sizes = ctx.saved_tensors[0]
+    copies = step.lhs, step.rhs
     if step.cfg is None:
       _, lhs, rhs = ctx.saved_tensors
-      step.lhs = None if lhs is None else lhs.detach()
-      step.rhs = None if rhs is None else rhs.detach()
+      step.lhs = step.lhs if lhs is None else lhs.detach()
+      step.rhs = step.rhs if rhs is None else rhs.detach()
     dlhs, drhs = _backward(step, g, ctx.needs_input_grad[:2])
-    if step.cfg is None:
-      step.lhs = step.rhs = None
+    step.lhs, step.rhs = copies
     return dlhs, drhs, None, None, None

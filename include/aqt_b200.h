@@ -671,6 +671,14 @@ int aqtb200_grouped_gemm(const aqtb200_grouped_gemm_desc* desc, int32_t* status,
  */
 int aqtb200_pack_bf16(const aqtb200_view* x, void* out, int64_t ld, void* stream);
 
+/*
+ * aqtb200_pack_bf16_groups: the same for the matrices of b0 * b1 groups whose
+ * sizes (device pointer, int32, or int64 when sizes_int64) are given; the places
+ * of groups without rows are left as they were. NULL sizes: every matrix.
+ */
+int aqtb200_pack_bf16_groups(const aqtb200_view* x, const void* group_sizes, int32_t sizes_int64, void* out,
+                             int64_t ld, void* stream);
+
 #ifdef __cplusplus
 } /* extern "C" */
 #endif

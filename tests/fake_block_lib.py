@@ -146,15 +146,24 @@ class FakeBlockLib(fake_lib.FakeLib):
     return 0
 
   def aqtb200_pack_bf16(self, view, out, ld, stream):
+    return self.aqtb200_pack_bf16_groups(view, None, 0, out, ld, stream)
+
+  def aqtb200_pack_bf16_groups(self, view, sizes, int64, out, ld, stream):
     del stream
     v = view._obj
     n = v.b0 * v.b1 * v.rows
     if not n:
       return 0
     to = _strided(out, _lib.BF16, [n, ld], [ld, 1], True)
-    to[...] = 0
-    if v.cols:
-      to[:, :v.cols] = fake_lib._view_array(v).reshape(n, v.cols)  # pylint: disable=protected-access
+    x = fake_lib._view_array(v).reshape(n, v.cols)  # pylint: disable=protected-access
+    for b in range(v.b0 * v.b1):
+      rows = slice(b * v.rows, (b + 1) * v.rows)
+      span = _sizes(sizes, v.b0 * v.b1, int64, 1 << 40)
+      if span is not None and span[b][0] == span[b][1]:
+        continue
+      to[rows] = 0
+      if v.cols:
+        to[rows, :v.cols] = x[rows]
     return 0
 
 

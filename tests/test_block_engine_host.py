@@ -218,3 +218,45 @@ def test_scales_named_powers_of_two_are(monkeypatch):
     rd.ragged_dot(x, bs.block_quantize(wg, 1, square=True), s, cfg=cfg)
     rd.ragged_dot(x, wg, s)
     assert told == [0, 0, 0]
+
+
+@pytest.mark.parametrize('lhs_copy,rhs_copy', [(True, False), (False, True),
+                                               (True, True)])
+def test_ragged_copies_are_made_once(monkeypatch, lhs_copy, rhs_copy):
+  """Operands no tensor map describes are copied once a step; the backward pass
+  reads the copies."""
+  from aqt_b200 import _lib
+  m, k, n, sizes = 20, 24 + 5 * lhs_copy, 16, [8, 0, 9]
+  x = _data((m, k), torch.bfloat16, 70)
+  w = _data((3, k, n), torch.bfloat16, 71)
+  if rhs_copy:
+    w = _off(w)
+  g, s = _data((m, n), torch.bfloat16, 72), torch.tensor(sizes)
+  lib = _lib.load()
+  calls = []
+  pack = lib.aqtb200_pack_bf16_groups
+  monkeypatch.setattr(
+      lib, 'aqtb200_pack_bf16_groups',
+      lambda *a: calls.append(a[1]) or pack(*a), raising=False)
+  a = x.clone().requires_grad_()
+  b = (_off(w) if rhs_copy else w.clone()).requires_grad_()
+  y = rd.ragged_dot(a, b, s)
+  y.backward(g)
+  # lhs, rhs (with the sizes: empty groups are skipped); g needs none
+  assert sorted(bool(c) for c in calls) == [False] * lhs_copy + [True] * rhs_copy
+  x64, w64, g64 = (_np(t).astype(np.float64) for t in (x, w, g))
+  _same(y, ref.ragged(x64, w64, sizes)[0], 2.0 ** -8)
+  _same(a.grad, ref.ragged(g64, w64.transpose(0, 2, 1), sizes)[0], 2.0 ** -8)
+  _same(b.grad, ref.ragged_drhs(x64, g64, sizes, 3)[0], 2.0 ** -8)
+  # twice through the same graph
+  a.grad = b.grad = None
+  y = rd.ragged_dot(a, b, s)
+  y.backward(g, retain_graph=True)
+  once = a.grad.clone(), b.grad.clone()
+  a.grad = b.grad = None
+  y.backward(g)
+  assert torch.equal(a.grad, once[0]) and torch.equal(b.grad, once[1])
+  out, bp = rd.ragged_dot_vjp(x, w, s)
+  p, q = bp(g)
+  p2, q2 = bp(g)
+  assert torch.equal(p, p2) and torch.equal(q, q2)

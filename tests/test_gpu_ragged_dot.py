@@ -401,3 +401,22 @@ def test_first_call_of_a_thread(what):
   _done()
   assert len(got) == len(want)
   assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_copies_of_experts_without_rows_are_left_out():
+  """Rows no tensor map describes: only the matrices in use are copied, the
+  places of the others hold whatever they held."""
+  g, k, n = 40, 133, 77
+  sizes = [0] * g
+  sizes[3], sizes[17], sizes[39] = 5, 1, 2
+  x, w, ct = (_data((9, k), torch.bfloat16, 50), _data(
+      (g, k, n), torch.bfloat16, 51, 0.1), _data((9, n), torch.bfloat16, 52))
+  # memory the allocator hands out next: NaN
+  torch.full((4 * g * k * 80,), float('nan'), dtype=torch.bfloat16, device='cuda')
+  for index in (torch.int32, torch.int64):
+    out, bp = rd.ragged_dot_vjp(x, w, _sizes(sizes, index))
+    dl, dr = bp(ct)
+    _done()
+    for got, wt in zip((out, dl, dr), _want(_f32(x), _f32(w), _f32(ct), sizes,
+                                            False)):
+      _check(got, wt, 2.0 ** -8, '')
