@@ -1199,23 +1199,6 @@ static bool output_map(CUtensorMap* tm, void* ptr, int64_t r, int64_t t, int64_t
 
 static bool is_fp8_dtype(int dt) { return dt == AQTB200_E4M3 || dt == AQTB200_E5M2; }
 
-// Columns of a tile, at most `most`. A group of `len` rows costs ceil(len / nt)
-// passes over its weights, an MMA's time goes with its columns, and each tile has
-// a cost of its own that goes with neither (`extra`, in columns).
-static int choose_nt(int64_t len, int64_t r_tiles, bool one_group, int pairs, int most, int extra) {
-  if (len <= most) return (int)std::max<int64_t>(32, (len + 31) / 32 * 32);
-  if (!one_group) return most;
-  // one group, all sizes known: the width whose rounds cost least in total
-  int best = most;
-  int64_t least = INT64_MAX;
-  for (int nt = most; nt >= 160; nt -= 32) {
-    const int64_t tiles = r_tiles * ((len + nt - 1) / nt);
-    const int64_t cost = (tiles + pairs - 1) / pairs * (nt + extra);
-    if (cost < least) { least = cost; best = nt; }
-  }
-  return best;
-}
-
 // How many clusters of `ctas` CTAs the device holds at once (clusters do not cross
 // its processor groups: of 148 SMs, not 18 clusters of eight but fewer than 16).
 // Looked up once for each device and size.
@@ -1296,32 +1279,54 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   const int64_t want = grouped && P.mode == 0 ? len + len / 2 : len;
   // Scales that are powers of two can be left to the tensor core, which then sums
   // the whole contraction (8192 x 4096 x 14336: 459 / 446 / 550 us against 588 / 537
-  // / 711; 300 x 4096 x 4096: 22 / 22 / 27 against 29 / 29 / 26). Its sums drop what does not fit 24 bits, each step of 32 products
-  // less than 2^-23 of the running sum (measured, all products positive: 2^-26 a
-  // step, 8e-6 over 14336): nothing beside a bf16 result's rounding of 2^-9 as long
-  // as the steps' total stays below 2^-10. f32 results keep the f32 registers.
-  const bool mx = fp8 && d->scales_po2 && want > 128 && d->out_dtype == AQTB200_BF16 &&
-                  P.num_kb * 4 <= 1 << 13 && (d->a_scale_square || d->a_scale_r_stride == 1);
-  const bool pair = !fp8 || (want <= 128 ? GG_PAIR_NARROW : GG_PAIR_WIDE);
-  const int ctas = pair ? 2 : 1, units = std::max(1, sm_count() / ctas);
-  P.r_tiles = (int)((d->r + 128 * ctas - 1) / (128 * ctas));
+  // / 711; 300 x 4096 x 4096: 22 / 22 / 27 against 29 / 29 / 26). Its sums drop what
+  // does not fit 24 bits, each step of 32 products less than 2^-23 of the running
+  // sum (measured, all products positive: 2^-26 a step, 8e-6 over 14336): nothing
+  // beside a bf16 result's rounding of 2^-9 as long as the steps' total stays below
+  // 2^-10. f32 results keep the f32 registers.
+  const bool po2 = fp8 && d->scales_po2 && d->out_dtype == AQTB200_BF16 && P.num_kb * 4 <= 1 << 13 &&
+                   (d->a_scale_square || d->a_scale_r_stride == 1);
+  const auto ctas_of = [&](int nt) { return !fp8 || (nt <= 128 ? GG_PAIR_NARROW : GG_PAIR_WIDE) ? 2 : 1; };
+  const auto units_of = [&](int nt) { return std::max(1, sm_count() / ctas_of(nt)); };
   // Tiles, or the most there can be: groups that end inside a tile add one each.
   const auto tiles_of = [&](int nt) {
-    const int64_t per = (d->t + nt - 1) / nt;
-    return P.r_tiles * (P.mode == 1 ? groups * per
-                        : grouped   ? d->t / nt + std::min<int64_t>(d->groups + 1, d->t)
-                                    : per);
+    const int64_t per = (d->t + nt - 1) / nt, rows = 128 * ctas_of(nt);
+    return (d->r + rows - 1) / rows *
+           (P.mode == 1 ? groups * per : grouped ? d->t / nt + std::min<int64_t>(d->groups + 1, d->t) : per);
   };
   // Scales in TMEM leave two accumulators of 224 columns, or one of 256: enough
   // where no CTA pair has a second tile to overlap (1024 x 4096 x 4096, 64 tiles on
   // 74 pairs and not 80: 25 / 25 / 37 us against 37 / 37 / 36).
-  P.one_half = mx && tiles_of(256) <= units;
-  P.nt = choose_nt(want, P.r_tiles, !grouped, units, mx && !P.one_half ? GG_MX_COLS : 256,
-                   fp8 && !mx ? 80 : 8);
+  P.one_half = po2 && tiles_of(256) <= units_of(256);
+  const int most = po2 && !P.one_half ? GG_MX_COLS : 256;
+  // Columns of a tile. A group of `want` rows costs ceil(want / nt) passes over its
+  // weights, and an MMA's time goes with its columns.
+  P.nt = want <= most ? (int)std::max<int64_t>(32, (want + 31) / 32 * 32) : most;
+  if (want > most && !grouped) {
+    // all sizes known: the width whose rounds cost least in total; each tile has a
+    // cost of its own besides, larger where the epilogue adds every 128-block
+    const int extra = po2 || !fp8 ? 8 : 80;
+    int64_t least = INT64_MAX;
+    for (int nt = most; nt >= 160; nt -= 32) {
+      const int64_t cost = (tiles_of(nt) + units_of(nt) - 1) / units_of(nt) * (nt + extra);
+      if (cost < least) { least = cost; P.nt = nt; }
+    }
+  }
+  // Where narrow tiles too fit the device at once, they share the work out further
+  // (449 x 173 x 5426, forward and gradients: 64 us wide, 33 us so; 775 x 3418 x 386
+  // in two groups, bf16: 59, 47 us). 32 columns gain nothing on 64 and lost up to
+  // 10 %. Short products over the rows divide the contraction instead (`split`).
+  if (want > (P.mode == 1 ? 64 : 128))
+    for (int nt = 64; nt <= 128 && nt < P.nt; nt += 32)
+      if (tiles_of(nt) <= units_of(nt)) { P.nt = nt; break; }
+  const bool mx = po2 && P.nt > 128;
+  P.one_half = P.one_half && mx;
+  const int ctas = ctas_of(P.nt), units = units_of(P.nt);
+  P.r_tiles = (int)((d->r + 128 * ctas - 1) / (128 * ctas));
   P.t_tiles = (int)((d->t + P.nt - 1) / P.nt);
   const uint32_t fa = fp8 ? (d->a_dtype == AQTB200_E5M2) : 1, fb = fp8 ? (d->b_dtype == AQTB200_E5M2) : 1;
   P.idesc = (1u << 4) | (fa << 7) | (fb << 10) | ((uint32_t)P.a_mn << 15) | ((uint32_t)P.b_mn << 16) |
-            ((pair ? 16u : 8u) << 24);
+            ((ctas == 2 ? 16u : 8u) << 24);
   // with scales: no accumulator type, 8-bit exponents
   if (mx) P.idesc = (P.idesc & ~(1u << 4)) | (1u << 23);
   P.b_stage = P.b_mn ? (P.nt / ctas + 63) / 64 * 8192 : P.nt / ctas * 128;

@@ -626,11 +626,11 @@ int aqtb200_block_quantize(const aqtb200_block_quant_desc* desc, void* stream);
  *             kb*a_scale_k_stride + (a_scale_square ? r/128 : r)*a_scale_r_stride.
  * b_scale   : f32 of (t, kb) at kb*b_scale_k_stride + t.
  * scales_po2: fp8: every scale is a power of two (po2_scale of
- *             aqtb200_block_quantize). Products of more than 128 rows t (grouped:
- *             of more than 85 a group on average) with a bf16 result and k up to
- *             2^18 are then scaled and summed on the tensor core, which takes a
- *             scale's exponent and nothing else of it, and reads the scales in
- *             whole aligned 16-byte pieces.
+ *             aqtb200_block_quantize). Products with a bf16 result, k up to 2^18 and
+ *             enough rows t to fill the device with tiles of more than 128 are then
+ *             scaled and summed on the tensor core, which takes a scale's exponent
+ *             and nothing else of it, and reads the scales in whole aligned 16-byte
+ *             pieces.
  * group_sizes, groups, sizes_int64: as for aqtb200_block_quantize; at most
  *             AQTB200_MAX_GROUPS groups.
  * rows      : number of grouped rows (contract_groups 1; t otherwise).

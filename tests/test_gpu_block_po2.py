@@ -1,7 +1,7 @@
-"""Block-scaled products whose scales are powers of two: more than 128 rows and a
-bfloat16 result let the tensor core scale and sum. Against the definition in 64
-bits, with blocks of very different sizes, so that a scale in the wrong place
-shows."""
+"""Block-scaled products whose scales are powers of two: wide tiles (results of some
+1500 x 1500 and more) with a bfloat16 result let the tensor core scale and sum.
+Against the definition in 64 bits, with blocks of very different sizes, so that a
+scale in the wrong place shows."""
 
 import numpy as np
 import pytest
@@ -56,7 +56,9 @@ def _check_step(x, w, g, got, fwd='e4m3', bwd='e5m2'):
 
 @pytest.mark.parametrize('m,k,n', [
     (129, 129, 129), (160, 64, 300), (224, 512, 225), (256, 1, 257),
-    (300, 640, 520), (449, 1300, 16), (700, 384, 1000), (2047, 257, 130), (512, 1100, 512)])
+    (300, 640, 520), (449, 1300, 16), (700, 384, 1000), (2047, 257, 130), (512, 1100, 512),
+    # forward, or all three products, in wide tiles: one accumulator, two
+    (2048, 300, 2000), (1700, 1650, 1750), (3000, 200, 2000), (1999, 129, 2561)])
 @pytest.mark.parametrize('fwd,bwd', [('e4m3', 'e5m2'), ('e5m2', 'e4m3')])
 def test_step(m, k, n, fwd, bwd):
   x, w, g = _data((m, k), 1), _data((k, n), 2), _data((m, n), 3)
@@ -81,7 +83,8 @@ def test_step_over_either_axis_of_rhs():
     (900, 384, 264, [1, 0, 127, 300, 65, 400]),     # seven rows left over
     (600, 129, 450, [128, 129, 300, 43]),
     (513, 130, 256, [-5, 300, -1, 600]),            # cut at the end
-    (400, 64, 200, [0, 0, 0])])
+    (400, 64, 200, [0, 0, 0]),
+    (3000, 1400, 1300, [0, 700, 1, 1500, 130, 600])])
 @pytest.mark.parametrize('index', [torch.int32, torch.int64])
 def test_ragged_step(m, k, n, sizes, index):
   x, w, g = _data((m, k), 7), _data((len(sizes), k, n), 8), _data((m, n), 9)
@@ -123,7 +126,7 @@ def test_one_accumulator_and_a_second_tile():
   """Few tiles expected, so that one wide accumulator is chosen, and more come."""
   sizes = [193] * 31 + [1] * 19
   m = sum(sizes)
-  x, w = _data((m, 136), 30), _data((50, 136, 100), 31)
+  x, w = _data((m, 136), 30), _data((50, 136, 256), 31)
   out = rd.ragged_dot(x, w, torch.tensor(sizes, dtype=torch.int32, device='cuda'),
                       cfg=bs.dot_general_make(po2_scale=True))
   _done()
@@ -134,7 +137,7 @@ def test_one_accumulator_and_a_second_tile():
 
 def test_zero_blocks_and_extreme_scales():
   """Blocks of zeros, and scales at both ends of what a product can hold."""
-  x, w = _data((300, 512), 13), _data((512, 200), 14)
+  x, w = _data((2048, 512), 13), _data((512, 1400), 14)
   x[:, 128:256] = 0
   x[5] = 0
   w[256:384, :128] = 0
@@ -150,7 +153,8 @@ def test_zero_blocks_and_extreme_scales():
 
 @pytest.mark.parametrize('bad', [float('nan'), float('inf')])
 def test_nan_and_inf_stay_in_their_rows(bad):
-  x, w, g = _data((300, 256), 15), _data((256, 300), 16), _data((300, 300), 17)
+  x, w, g = (_data((1700, 1650), 15), _data((1650, 1750), 16),
+             _data((1700, 1750), 17))
   cfg = bs.dot_general_make(po2_scale=True)
 
   def step():
@@ -159,7 +163,7 @@ def test_nan_and_inf_stay_in_their_rows(bad):
 
   clean = step()
   x[7, 3] = bad
-  g[200, 299] = bad
+  g[200, 1749] = bad
   out, dl, dr = step()
   _done()
   rows = lambda t, *skip: t[[i for i in range(t.shape[0]) if i not in skip]]
@@ -167,14 +171,14 @@ def test_nan_and_inf_stay_in_their_rows(bad):
   assert torch.isnan(out[7]).all()
   assert torch.equal(rows(dl, 200), rows(clean[1], 200))
   assert torch.isnan(dl[200]).all()
-  # x[7, 3] reaches row 3 of drhs, g[200, 299] its last column
-  assert torch.isnan(dr[3]).all() and torch.isnan(dr[:, 299]).all()
-  assert torch.equal(rows(dr, 3)[:, :299], rows(clean[2], 3)[:, :299])
+  # x[7, 3] reaches row 3 of drhs, g[200, 1749] its last column
+  assert torch.isnan(dr[3]).all() and torch.isnan(dr[:, 1749]).all()
+  assert torch.equal(rows(dr, 3)[:, :1749], rows(clean[2], 3)[:, :1749])
 
 
 def test_groups_do_not_mix():
-  sizes = [200, 0, 170, 129]
-  m, k, n = 520, 136, 260
+  sizes = [1000, 0, 850, 645]
+  m, k, n = 2600, 1400, 1700
   x, w, g = _data((m, k), 18), _data((4, k, n), 19), _data((m, n), 20)
   s = torch.tensor(sizes, dtype=torch.int32, device='cuda')
   cfg = bs.dot_general_make(po2_scale=True)
@@ -184,17 +188,17 @@ def test_groups_do_not_mix():
     return (out, *bp(g))
 
   out, dl, dr = step()
-  x[499:] = float('nan')
-  g[499:] = float('nan')
-  x[200, 5] = float('nan')   # first row of the third group
-  g[369, 7] = float('inf')   # its last row
+  x[2495:] = float('nan')
+  g[2495:] = float('nan')
+  x[1000, 5] = float('nan')   # first row of the third group
+  g[1849, 7] = float('inf')   # its last row
   out2, dl2, dr2 = step()
   _done()
-  keep = [i for i in range(520) if not 200 <= i < 370]
+  keep = [i for i in range(m) if not 1000 <= i < 1850]
   assert torch.equal(out[keep], out2[keep]) and torch.equal(dl[keep], dl2[keep])
   for e in (0, 1, 3):
     assert torch.equal(dr[e], dr2[e]), e
-  assert torch.isnan(out2[200]).all() and torch.isnan(dr2[2, 5]).all()
+  assert torch.isnan(out2[1000]).all() and torch.isnan(dr2[2, 5]).all()
 
 
 @pytest.mark.parametrize('k', [14336, 262144, 262400])
@@ -203,8 +207,8 @@ def test_long_positive_sums(k):
   2^-23 of the result for each 32 products as long as it is left to sum (262144
   products), and stays below a bfloat16 step. Equal values make the result exact:
   every block is its maximum, one code, and the sum k times one product."""
-  x = torch.full((160, k), 1.25, dtype=BF, device='cuda')
-  w = torch.full((k, 8), 0.75, dtype=BF, device='cuda')
+  x = torch.full((), 1.25, dtype=BF, device='cuda').expand(2048, k)
+  w = torch.full((), 0.75, dtype=BF, device='cuda').expand(k, 1300)
   out = bs.dot_general_make(po2_scale=True)(x, w, DIMS)
   _done()
   # 1.25 and 0.75 are codes of e4m3 under any power of two
@@ -235,7 +239,7 @@ def test_frozen_scales_need_not_be_powers_of_two():
 
 
 def test_captured_and_replayed():
-  x, w, g = _data((300, 260), 25), _data((260, 200), 26), _data((300, 200), 27)
+  x, w, g = _data((1700, 260), 25), _data((260, 1750), 26), _data((1700, 1750), 27)
   cfg = bs.dot_general_make(po2_scale=True)
 
   def step():
@@ -249,7 +253,7 @@ def test_captured_and_replayed():
   with torch.cuda.graph(graph, stream=side):
     got = step()
   for seed in (28, 29):
-    x.copy_(_data((300, 260), seed))
+    x.copy_(_data((1700, 260), seed))
     graph.replay()
     _done()
     _check_step(x, w, g, got)

@@ -382,3 +382,18 @@ def test_projection_stack_runs_on_block_scaled_products():
     # two operands a product, each off by at most 2^-4 (e4m3); the longest chain
     # to a weight gradient is five products deep
     assert float((a - b).norm() / b.norm()) < 2 * 2.0 ** -4 * 5, name
+
+
+@pytest.mark.parametrize('m,k,n', [(1700, 1650, 1750), (3000, 200, 2001),
+                                   (2048, 129, 2560)])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_step_in_wide_tiles(m, k, n, dtype):
+  """Results that take more tiles of 128 columns than the device holds at once."""
+  x, w, g = (_data((m, k), dtype, 40, 1.0), _data((k, n), dtype, 41, 0.3),
+             _data((m, n), dtype, 42, 1.0))
+  out, bp = bs.dot_general_make().vjp(x, w, DIMS)
+  got = (out, *bp(g))
+  _done()
+  for name, a, (want, mag, kk) in zip(('out', 'dlhs', 'drhs'), got,
+                                      _want(_f32(x), _f32(w), _f32(g))):
+    ref.assert_close(_f32(a).astype(np.float64), want, mag, kk, HALF[dtype], name)

@@ -420,3 +420,26 @@ def test_copies_of_experts_without_rows_are_left_out():
     for got, wt in zip((out, dl, dr), _want(_f32(x), _f32(w), _f32(ct), sizes,
                                             False)):
       _check(got, wt, 2.0 ** -8, '')
+
+
+@pytest.mark.parametrize('m,k,n,sizes', [
+    (3000, 1400, 1304, [0, 700, 1, 1500, 130, 600]),
+    (2500, 1401, 1303, [1250, 1249]),
+    (5000, 72, 1800, [300, 0, 900, 64, 2000, 1, 257, 1400])])
+@pytest.mark.parametrize('q', [False, True])
+@pytest.mark.parametrize('out', [torch.bfloat16, torch.float32])
+def test_step_in_wide_tiles(m, k, n, sizes, q, out):
+  """More tiles of 128 columns than the device holds at once."""
+  x, w, g = (_data((m, k), torch.bfloat16, 53), _data(
+      (len(sizes), k, n), torch.bfloat16, 54, 0.1), _data((m, n), out, 55))
+  y, bp = rd.ragged_dot_vjp(x, w, _sizes(sizes), preferred_element_type=out,
+                            cfg=bs.dot_general_make() if q else None)
+  dl, dr = bp(g)
+  _done()
+  assert y.dtype == out
+  gf = g if q else g.bfloat16()  # without cfg cotangents are bfloat16
+  for name, got, wt in zip(('out', 'dlhs', 'drhs'), (y, dl, dr),
+                           _want(_f32(x), _f32(w), _f32(gf), sizes, q)):
+    _check(got, wt, HALF[got.dtype], name)
+  left = sum(sizes)
+  assert not y[left:].any() and not dl[left:].any()
