@@ -106,7 +106,7 @@ class GroupedGemmDesc(C.Structure):
       ('b', C.c_void_p), ('b_ld', C.c_int64),
       ('a_mn_major', C.c_int32), ('b_mn_major', C.c_int32),
       ('a_scale_square', C.c_int32), ('sizes_int64', C.c_int32),
-      ('scales_po2', C.c_int32),
+      ('scales_po2', C.c_int32), ('follows_quantize', C.c_int32),
       ('a_scale', C.c_void_p), ('a_scale_group_stride', C.c_int64),
       ('a_scale_k_stride', C.c_int64), ('a_scale_r_stride', C.c_int64),
       ('b_scale', C.c_void_p), ('b_scale_k_stride', C.c_int64),

@@ -272,14 +272,15 @@ def _empty_out(shape, dtype, device):
 
 
 def fp8_rows(tokens, a, k, out_dtype, device, group_sizes=None, po2=False):
-  """out[t][r] = sum_k tokens[t][k] a[g(t)][r][k]; a has 128 x 128 blocks. po2:
-  all scales are powers of two."""
+  """out[t][r] = sum_k tokens[t][k] a[g(t)][r][k]; a has 128 x 128 blocks. The
+  call before this one has to be the one that quantized the tokens. po2: all
+  scales are powers of two."""
   t, r = tokens.kept, a.kept
   out = _empty_out((t, r), out_dtype, device)
   sizes, groups, int64 = _sizes(group_sizes)
   _gemm(_lib.GroupedGemmDesc(
       0, a.code, tokens.code, engine._TORCH_CODE[out_dtype], r, t, k, t,  # pylint: disable=protected-access
-      a.ptr, a.ld, a.group, tokens.ptr, tokens.ld, 0, 0, 1, int64, po2,
+      a.ptr, a.ld, a.group, tokens.ptr, tokens.ld, 0, 0, 1, int64, po2, 1,
       a.scale, a.scale_group, a.scale_k, a.scale_r,
       tokens.scale, tokens.scale_k, sizes, groups,
       out.data_ptr(), r, 0, None, 0), device, 'block-scaled product')
@@ -296,7 +297,7 @@ def fp8_contract_rows(b, a, k, rows, out_dtype, device, group_sizes=None,
   sizes, groups, int64 = _sizes(group_sizes)
   _gemm(_lib.GroupedGemmDesc(
       1, a.code, b.code, engine._TORCH_CODE[out_dtype], r, t, k, rows,  # pylint: disable=protected-access
-      a.ptr, a.ld, 0, b.ptr, b.ld, 0, 0, 0, int64, po2,
+      a.ptr, a.ld, 0, b.ptr, b.ld, 0, 0, 0, int64, po2, 0,
       a.scale, 0, a.scale_k, 1, b.scale, b.scale_k, sizes, groups,
       out.data_ptr(), r, t * r, None, 0), device, 'block-scaled product')
   return out
@@ -363,7 +364,7 @@ def bf16_rows(tokens, a, contract_axis, group_sizes, out_dtype):
   _gemm(_lib.GroupedGemmDesc(
       0, _lib.BF16, _lib.BF16, engine._TORCH_CODE[out_dtype], r, t, k, t,  # pylint: disable=protected-access
       a.data_ptr(), ld, a.stride(0), tokens.data_ptr(), _ld(tokens, 0), mn, 0,
-      0, int64, 0, None, 0, 0, 0, None, 0, sizes, groups, out.data_ptr(), r, 0,
+      0, int64, 0, 0, None, 0, 0, 0, None, 0, sizes, groups, out.data_ptr(), r, 0,
       None, 0), dev, 'grouped product')
   return out
 
@@ -378,7 +379,7 @@ def bf16_contract_rows(lhs, g, group_sizes, out_dtype):
   sizes, groups, int64 = _sizes(group_sizes)
   d = _lib.GroupedGemmDesc(
       1, _lib.BF16, _lib.BF16, engine._TORCH_CODE[out_dtype], r, t, rows, rows,  # pylint: disable=protected-access
-      g.data_ptr(), _ld(g, 0), 0, lhs.data_ptr(), _ld(lhs, 0), 1, 1, 0, int64, 0,
+      g.data_ptr(), _ld(g, 0), 0, lhs.data_ptr(), _ld(lhs, 0), 1, 1, 0, int64, 0, 0,
       None, 0, 0, 0, None, 0, sizes, groups, out.data_ptr(), r, t * r, None, 0)
   # room for the groups' last, partial slabs
   nbytes = _lib.load().aqtb200_grouped_gemm_workspace_bytes(C.byref(d))

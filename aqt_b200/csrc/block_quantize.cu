@@ -180,6 +180,9 @@ __global__ void __launch_bounds__(BQ_THREADS, BF16 ? 4 : 2) block_quantize_kerne
   const int64_t rt = blockIdx.x / P.col_tiles % P.row_tiles;  // with groups, of the padded order
   const int64_t b = blockIdx.x / P.col_tiles / P.row_tiles;
 
+  // a product launched to follow may take the SMs that come free and fetch its
+  // weights; it waits for this grid's end before it reads what is written here
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   int64_t row0 = rt * QB, row_end = P.rows;
   if (P.sizes != nullptr) {
     if (warp == 0) {

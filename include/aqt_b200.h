@@ -631,6 +631,10 @@ int aqtb200_block_quantize(const aqtb200_block_quant_desc* desc, void* stream);
  *             scaled and summed on the tensor core, which takes a scale's exponent
  *             and nothing else of it, and reads the scales in whole aligned 16-byte
  *             pieces.
+ * follows_quantize: fp8, contract_groups 0: the last work put on the stream is the
+ *             aqtb200_block_quantize call that makes b and b_scale, and a, a_scale
+ *             and group_sizes do not come from it. The product is then launched while
+ *             that call still runs and fetches the first of a meanwhile.
  * group_sizes, groups, sizes_int64: as for aqtb200_block_quantize; at most
  *             AQTB200_MAX_GROUPS groups.
  * rows      : number of grouped rows (contract_groups 1; t otherwise).
@@ -647,7 +651,7 @@ typedef struct aqtb200_grouped_gemm_desc {
   int64_t a_ld, a_group_stride;
   const void* b;
   int64_t b_ld;
-  int32_t a_mn_major, b_mn_major, a_scale_square, sizes_int64, scales_po2;
+  int32_t a_mn_major, b_mn_major, a_scale_square, sizes_int64, scales_po2, follows_quantize;
   const float* a_scale;
   int64_t a_scale_group_stride, a_scale_k_stride, a_scale_r_stride;
   const float* b_scale;

@@ -260,3 +260,46 @@ def test_ragged_copies_are_made_once(monkeypatch, lhs_copy, rhs_copy):
   p, q = bp(g)
   p2, q2 = bp(g)
   assert torch.equal(p, p2) and torch.equal(q, q2)
+
+
+def test_products_that_follow_their_quantizer(monkeypatch):
+  """A product is launched early exactly where the call before it is the one that
+  wrote its tokens and their scales, and nothing else of it."""
+  from aqt_b200 import _lib
+  lib = _lib.load()
+  seen = []
+  quantize, gemm = lib.aqtb200_block_quantize, lib.aqtb200_grouped_gemm
+
+  def q(desc, *args):
+    d = desc._obj
+    seen.append([d.q_row, d.q_col, d.scale_row, d.scale_col])
+    return quantize(desc, *args)
+
+  def mm(desc, *args):
+    d = desc._obj
+    if d.follows_quantize:
+      wrote = [p for p in seen[-1] if p]
+      assert d.contract_groups == 0 and d.b in wrote and d.b_scale in wrote
+      assert d.a not in wrote and d.a_scale not in wrote
+    seen.append(d.follows_quantize)
+    return gemm(desc, *args)
+
+  monkeypatch.setattr(lib, 'aqtb200_block_quantize', q, raising=False)
+  monkeypatch.setattr(lib, 'aqtb200_grouped_gemm', mm, raising=False)
+  x, w, g = (_data((140, 200), torch.bfloat16, 80), _data(
+      (200, 30), torch.bfloat16, 81), _data((140, 30), torch.bfloat16, 82))
+  s = torch.tensor([100, 40], dtype=torch.int32)
+  wg = _data((2, 200, 30), torch.bfloat16, 83)
+  cfg = bs.dot_general_make()
+  flags = lambda: [v for v in seen if not isinstance(v, list)]
+  for run in (lambda: cfg.vjp(x, w, DIMS)[1](g),
+              lambda: cfg.vjp(x, w.t().contiguous(), (((1,), (1,)), ((), ())))[1](g),
+              lambda: rd.ragged_dot_vjp(x, wg, s, cfg=cfg)[1](g)):
+    seen.clear()
+    run()
+    assert flags() == [1, 1, 0]
+  seen.clear()
+  cfg(x, bs.block_quantize(w, 0, square=True), DIMS)
+  rd.ragged_dot(x, bs.block_quantize(wg, 1, square=True), s, cfg=cfg)
+  rd.ragged_dot(x, wg, s)
+  assert flags() == [1, 1, 0]

@@ -397,3 +397,32 @@ def test_step_in_wide_tiles(m, k, n, dtype):
   for name, a, (want, mag, kk) in zip(('out', 'dlhs', 'drhs'), got,
                                       _want(_f32(x), _f32(w), _f32(g))):
     ref.assert_close(_f32(a).astype(np.float64), want, mag, kk, HALF[dtype], name)
+
+
+@pytest.mark.parametrize('m,k,n', [(1, 4096, 512), (16, 8192, 1024),
+                                   (700, 2048, 256), (3000, 1024, 2048)])
+@pytest.mark.parametrize('po2', [False, True])
+def test_products_back_to_back(m, k, n, po2):
+  """A product starts while its operand is still being quantized: queued without
+  a pause, on changing values and memory that is used over and over, each gives
+  what it gives alone. Weights are written anew just before, too."""
+  cfg = bs.dot_general_make(po2_scale=po2)
+  xs = [_data((m, k), torch.bfloat16, 50 + i, 1.0) for i in range(4)]
+  ws = [_data((k, n), torch.bfloat16, 60 + i, 0.3) for i in range(2)]
+  alone = {}
+  for i, x in enumerate(xs):
+    for j, w in enumerate(ws):
+      alone[i, j] = cfg(x, bs.block_quantize(w, 0, square=True), DIMS)
+      _done()
+  x = torch.empty_like(xs[0])
+  got = []
+  for turn in range(40):
+    i, j = turn % 4, turn % 2
+    x.copy_(xs[i])
+    qt = bs.block_quantize(ws[j], 0, square=True)
+    got.append((i, j, cfg(x, qt, DIMS)))
+    x.zero_()  # queued behind the product
+    del qt
+  _done()
+  for i, j, out in got:
+    assert torch.equal(out, alone[i, j]), (i, j)
