@@ -64,21 +64,22 @@ constexpr int GG_BATCH = 4;
 constexpr int GG_SLOTS = 2;                  // batches on their way or in use
 constexpr int GG_SLOT = 256 + 128;           // floats a slab: 256 columns, this CTA's 128 rows
 constexpr int GG_SCALE_BYTES = GG_SLOTS * GG_BATCH * GG_SLOT * 4;
-// Scales on the tensor core (MX): two batches of words in TMEM, behind the columns
-// of the first accumulator. Of each, eight columns for 256 columns of the tile and
+// Scales on the tensor core (MX): two batches of words in TMEM behind the columns
+// of either accumulator. Of each, eight columns for 256 columns of the tile and
 // four for 128 rows.
 constexpr int GG_MX_COLS = 224;
-constexpr int GG_MX_AHEAD = 4;               // batches of f32 scales on their way
+constexpr int GG_MX_AHEAD = 3;               // batches of f32 scales on their way
+constexpr int GG_MX_SLOTS = 4;               // batches of exponents
 // of a slab: 256 columns and 128 rows, each with up to 3 floats more at both ends
 // (whole 16-byte pieces), and how far the first one lies in its piece
 constexpr int GG_MX_ROWS = 264, GG_MX_SHIFTS = GG_MX_ROWS + 136, GG_MX_SLOT = GG_MX_SHIFTS + 4;
 constexpr int GG_STAGE_OUT = 512;            // a warp's staging: 8 columns by 32 rows of bf16,
 constexpr int GG_STAGE_WIDE = 4096;          // or all of its 64 columns
 constexpr int GG_RING_WIDE = 128 * 1024;
+constexpr int GG_RING_MX = 180 * 1024;       // three stages of two slabs for 224 columns
 constexpr size_t GG_SMEM = GG_RING + GG_SCALE_BYTES + 16 * GG_STAGE_OUT + 1024;
-constexpr int GG_MX_BYTES = GG_SLOTS * 3 * 512 + GG_MX_AHEAD * GG_BATCH * GG_MX_SLOT * 4;
-static_assert(GG_MAX_STAGES * (GG_A_STAGE + GG_A_STAGE) + GG_MX_BYTES + 16 * GG_STAGE_OUT + 1024 <= GG_SMEM,
-              "shared memory");
+constexpr int GG_MX_BYTES = GG_MX_SLOTS * 3 * 512 + GG_MX_AHEAD * GG_BATCH * GG_MX_SLOT * 4;
+constexpr size_t GG_SMEM_MX = GG_RING_MX + GG_MX_BYTES + 16 * GG_STAGE_OUT + 1024;
 static_assert(GG_RING_WIDE + GG_SCALE_BYTES + 16 * GG_STAGE_WIDE + 1024 <= GG_SMEM, "shared memory");
 constexpr int GG_MAX_SEG = AQTB200_MAX_GROUPS + 1;
 constexpr int GG_TAIL = 64;                  // k-slab of bf16 elements
@@ -372,7 +373,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                     GGParams P) {
   static_assert(!MX || (FP8 && PAIR && SLICES * COLS > 128), "scales on the tensor core: wide fp8 tiles");
   constexpr bool SUMS = FP8 && !MX;  // the epilogue scales and adds every 128-block
-  constexpr int KS = gg_slabs(FP8, SLICES * COLS);
+  constexpr int KS = MX ? 2 : gg_slabs(FP8, SLICES * COLS);
+  constexpr int SLOTS = MX ? GG_MX_SLOTS : GG_SLOTS;
   // Wide fp8 tiles keep every warp busy with the sums, so their results leave
   // through the TMA unit: written to shared memory (4 KB a warp) and stored from
   // there under the next tile. Stored by the warps themselves they cost 65 us of
@@ -384,8 +386,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   __shared__ __align__(8) uint64_t empty_bar[GG_MAX_STAGES];  // one per CTA
   __shared__ __align__(8) uint64_t tfull_bar[2];              // one per CTA
   __shared__ __align__(8) uint64_t tempty_bar[2];             // used in the pair's even CTA
-  __shared__ __align__(8) uint64_t sfull_bar[GG_SLOTS];       // a batch of scales; one per CTA
-  __shared__ __align__(8) uint64_t sempty_bar[GG_SLOTS];
+  __shared__ __align__(8) uint64_t sfull_bar[SLOTS];       // a batch of scales; one per CTA
+  __shared__ __align__(8) uint64_t sempty_bar[SLOTS];
   __shared__ __align__(8) uint64_t raw_bar[MX ? 2 * GG_MX_AHEAD : 1];  // MX: f32 scales, by warp
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -412,7 +414,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       mbar_init(&tfull_bar[s], 1);
       mbar_init(&tempty_bar[s], CTAS * 4 * SLICES);
     }
-    for (int s = 0; s < GG_SLOTS; ++s) {
+    for (int s = 0; s < SLOTS; ++s) {
       mbar_init(&sfull_bar[s], MX ? 2 * CTAS : 32);
       mbar_init(&sempty_bar[s], MX ? 1 : 4 * SLICES);
     }
@@ -630,7 +632,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             const bool last = kb + 1 == kb1;
             if constexpr (MX) {
               const int j = (kb - kb0) & (GG_BATCH - 1);
-              const uint32_t ts = tmem_base + (P.one_half ? 256u : GG_MX_COLS) + slot * 16u;
+              const uint32_t ts = tmem_base + (P.one_half ? 256u + slot * 16u
+                                                      : GG_MX_COLS + (slot & 1) * 16u + (slot >> 1) * 256u);
               if (j == 0) {
                 if (!warp_wait(&sfull_bar[slot], sphase, abortp)) { fail = 2; break; }
                 tc_fence_after();
@@ -643,7 +646,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                              idesc | (uint32_t)j << 29 | (uint32_t)j << 4, ts + 8, ts, kb > kb0 ? 1u : 0u);
               if (j == GG_BATCH - 1 || last) {
                 gg_commit<PAIR>(elected, sempty0 + slot * 8, lead);
-                if (++slot == GG_SLOTS) { slot = 0; sphase ^= 1u; }
+                if (++slot == SLOTS) { slot = 0; sphase ^= 1u; }
               }
             } else {
               tc_fence_after();
@@ -680,25 +683,32 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       // Warp 2: of the columns; warp 3: of this CTA's rows. GG_MX_AHEAD batches are
       // on their way at once, across tiles, as bulk copies: loaded and waited for
       // one by one a batch took up to 8000 clocks, in 4-byte asynchronous copies
-      // 2100, and its MMAs take 1800.
+      // 2100, and its MMAs take 1800. Four batches of exponents may be ready ahead
+      // (with two 8192 x 8192 x 8192 took 495 us, with none to convert 460).
       const bool rows = warp == 3, square = rows && !A_ROW;
       int slot = 0, cur = 0, issued = 0, done = 0;
       uint32_t phase = 0;
       const uint32_t sfull0 = map_to_cta(smem_u32(&sfull_bar[0]), lead);
       uint64_t* const bars = raw_bar + (rows ? GG_MX_AHEAD : 0);
-      float* const raw = slots + GG_SLOTS * 384 + (rows ? GG_MX_ROWS : 0);
-      int* const shifts = (int*)(slots + GG_SLOTS * 384 + GG_MX_SHIFTS + (rows ? 1 : 0));
+      float* const raw = slots + GG_MX_SLOTS * 384 + (rows ? GG_MX_ROWS : 0);
+      int* const shifts = (int*)(slots + GG_MX_SLOTS * 384 + GG_MX_SHIFTS + (rows ? 1 : 0));
       auto convert = [&]() {
         const int at = (done % GG_MX_AHEAD) * GG_BATCH * GG_MX_SLOT;
         if (!warp_wait(&bars[done % GG_MX_AHEAD], (done / GG_MX_AHEAD) & 1, abortp)) return false;
         uint32_t w[8] = {0};
+        const float* x[GG_BATCH];
 #pragma unroll
-        for (int b = 0; b < GG_BATCH; ++b) {
-          const float* x = raw + at + b * GG_MX_SLOT + (shifts[at + b * GG_MX_SLOT] & 3);
+        for (int b = 0; b < GG_BATCH; ++b)
+          x[b] = raw + at + b * GG_MX_SLOT + (shifts[at + b * GG_MX_SLOT] & 3) + (square ? 0 : lane);
 #pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e < (A_ROW ? 4 : 1) || !rows)
-              w[e] |= (__float_as_uint(x[square ? 0 : e * 32 + lane]) >> 23 & 255u) << (8 * b);
+        for (int e = 0; e < 8; ++e) {
+          if (e < (A_ROW ? 4 : 1) || !rows) {
+            // the exponents are the top bytes once the signs are shifted out
+            uint32_t v[GG_BATCH];
+#pragma unroll
+            for (int b = 0; b < GG_BATCH; ++b) v[b] = __float_as_uint(x[b][e * 32]) << 1;
+            w[e] = __byte_perm(__byte_perm(v[0], v[1], 0x0073), __byte_perm(v[2], v[3], 0x0073), 0x5410);
+          }
         }
         if (square) w[1] = w[2] = w[3] = w[0];
         ++done;
@@ -711,7 +721,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         if (lane == 0)
           asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(sfull0 + slot * 8)
                        : "memory");
-        if (++slot == GG_SLOTS) { slot = 0; phase ^= 1u; }
+        if (++slot == SLOTS) { slot = 0; phase ^= 1u; }
         return true;
       };
       for (int tile = cluster_id; tile < total && !fail; tile += num_clusters) {
@@ -778,7 +788,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(
                            smem_u32(&sfull_bar[slot]))
                        : "memory");
-          if (++slot == GG_SLOTS) { slot = 0; phase ^= 1; }
+          if (++slot == SLOTS) { slot = 0; phase ^= 1; }
         }
       }
       if (fail && lane == 0) {
@@ -1004,7 +1014,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           in_batch += here;
           if (in_batch == GG_BATCH || kb == kb1) {
             if (lane == 0) mbar_arrive(&sempty_bar[slot]);
-            if (++slot == GG_SLOTS) { slot = 0; sphase ^= 1u; }
+            if (++slot == SLOTS) { slot = 0; sphase ^= 1u; }
             in_batch = 0;
           }
         } else {
@@ -1313,8 +1323,8 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   // pass. fp8 hands over an accumulator per 128-block, bf16 one per tile.
   const int64_t want = grouped && P.mode == 0 ? len + len / 2 : len;
   // Scales that are powers of two can be left to the tensor core, which then sums
-  // the whole contraction (8192 x 4096 x 14336: 459 / 446 / 550 us against 588 / 537
-  // / 711; 300 x 4096 x 4096: 22 / 22 / 27 against 29 / 29 / 26). Its sums drop what
+  // the whole contraction (8192 x 4096 x 14336: 432 / 419 / 526 us against 588 / 537
+  // / 711; 8192 x 8192 x 8192: 471 / 469 / 465 against 620 / 615 / 762). Its sums drop what
   // does not fit 24 bits, each step of 32 products less than 2^-23 of the running
   // sum (measured, all products positive: 2^-26 a step, 8e-6 over 14336): nothing
   // beside a bf16 result's rounding of 2^-9 as long as the steps' total stays below
@@ -1331,7 +1341,7 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   };
   // Scales in TMEM leave two accumulators of 224 columns, or one of 256: enough
   // where no CTA pair has a second tile to overlap (1024 x 4096 x 4096, 64 tiles on
-  // 74 pairs and not 80: 25 / 25 / 37 us against 37 / 37 / 36).
+  // 74 pairs and not 80: 25 / 25 / 34 us against 37 / 37 / 36).
   P.one_half = po2 && tiles_of(256) <= units_of(256);
   const int most = po2 && !P.one_half ? GG_MX_COLS : 256;
   // Columns of a tile. A group of `want` rows costs ceil(want / nt) passes over its
@@ -1365,7 +1375,8 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   // with scales: no accumulator type, 8-bit exponents
   if (mx) P.idesc = (P.idesc & ~(1u << 4)) | (1u << 23);
   P.b_stage = P.b_mn ? (P.nt / ctas + 63) / 64 * 8192 : P.nt / ctas * 128;
-  P.stages = std::min(GG_MAX_STAGES, (fp8 && !mx && P.nt > 128 ? GG_RING_WIDE : GG_RING) / (gg_slabs(fp8, P.nt) * (GG_A_STAGE + P.b_stage)));
+  P.stages = std::min(GG_MAX_STAGES, (mx ? GG_RING_MX : fp8 && P.nt > 128 ? GG_RING_WIDE : GG_RING) /
+                                         ((mx ? 2 : gg_slabs(fp8, P.nt)) * (GG_A_STAGE + P.b_stage)));
   P.buf_cols = P.nt <= 64 ? 64 : P.nt <= 128 ? 128 : 256;
   P.half_kb = 256 / P.buf_cols;
   P.a_scale = d->a_scale; P.sa_g = d->a_scale_group_stride; P.sa_k = d->a_scale_k_stride;
@@ -1438,7 +1449,7 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
                            d->out_group_stride);
   }
 
-  const size_t smem = GG_SMEM;
+  const size_t smem = mx ? GG_SMEM_MX : GG_SMEM;
   // Whole tiles round robin: the fewest CTAs that keep the number of rounds.
   const int64_t rounds = (tiles + units - 1) / units;
   const int64_t clusters = P.split > 1 ? tiles
@@ -1464,7 +1475,7 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
     static bool attr_done[64] = {false};                                                           \
     if (!attr_done[dev & 63]) {                                                                    \
       AQT_CUDA_OK(cudaFuncSetAttribute(grouped_gemm_kernel<__VA_ARGS__>,                           \
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)GG_SMEM)); \
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); \
       attr_done[dev & 63] = true;                                                                  \
     }                                                                                              \
     AQT_CUDA_OK(cudaLaunchKernelEx(&cfg, grouped_gemm_kernel<__VA_ARGS__>, tmA, tmB, tmAt, tmBt, P)); \
