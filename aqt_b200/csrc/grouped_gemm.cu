@@ -1204,6 +1204,18 @@ static EncodeTiledFn encode_fn() {
   return fn;
 }
 
+// A thread whose first CUDA call this is (a backward pass runs on one of its own) has
+// no context yet, and the driver call that encodes a map needs one: then the runtime's
+// device is bound. A context that is current already stays so.
+template <class Encode>
+static CUresult with_context(Encode&& encode) {
+  CUresult r = encode();
+  int dev = 0;
+  if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess)
+    r = encode();
+  return r;
+}
+
 // 3-D map [outer][mid][inner] with 128-byte wide boxes of `box_mid` rows.
 static int operand_map(CUtensorMap* tm, const void* ptr, bool fp8, int64_t inner, int64_t mid,
                        int64_t outer, int64_t ld, int64_t s_outer, int box_mid) {
@@ -1219,10 +1231,12 @@ static int operand_map(CUtensorMap* tm, const void* ptr, bool fp8, int64_t inner
   cuuint64_t strides[2] = {(cuuint64_t)(ld * es), (cuuint64_t)(s_outer * es)};
   cuuint32_t box[3] = {(cuuint32_t)(128 / es), (cuuint32_t)box_mid, 1};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = enc(tm, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
-                   const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  const CUresult r = with_context([&] {
+    return enc(tm, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+               const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  });
   AQT_REQUIRE(r == CUDA_SUCCESS, AQTB200_EDRIVER, "cuTensorMapEncodeTiled failed with %d", (int)r);
   return 0;
 }
@@ -1237,9 +1251,11 @@ static bool output_map(CUtensorMap* tm, void* ptr, int64_t r, int64_t t, int64_t
   cuuint64_t strides[2] = {(cuuint64_t)ld * 2, (cuuint64_t)s_group * 2};
   cuuint32_t box[3] = {32, 64, 1};
   cuuint32_t estr[3] = {1, 1, 1};
-  return enc(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, ptr, dims, strides, box, estr,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return with_context([&] {
+           return enc(tm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, ptr, dims, strides, box, estr,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                      CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+         }) == CUDA_SUCCESS;
 }
 
 static bool is_fp8_dtype(int dt) { return dt == AQTB200_E4M3 || dt == AQTB200_E5M2; }
@@ -1392,9 +1408,6 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   AQT_REQUIRE(tiles < lim - 65536, AQTB200_EUNSUPPORTED, "more than 2^31 output tiles");
   int dev = 0;
   AQT_CUDA_OK(cudaGetDevice(&dev));
-  // A thread whose first CUDA call this is (a backward pass runs on one of its own)
-  // has no context yet, and the driver call that encodes a map needs one.
-  AQT_CUDA_OK(cudaSetDevice(dev));
   // Few tiles: the contraction of each is shared by up to four of a cluster, which
   // add their sums through distributed shared memory, in order -- as many as keep
   // every cluster on the device at once (1 x 4096 x 4096 fp8 on CTA pairs: one a
