@@ -332,6 +332,16 @@ def pack(x, group_sizes=None):
   return buf[..., :x.shape[-1]]
 
 
+def as_bf16(x):
+  """x itself, or rounded to bfloat16: torch's work, which a traced step has to
+  be told of, into memory it holds."""
+  if x.dtype == torch.bfloat16:
+    return x
+  out = _empty_out(x.shape, torch.bfloat16, x.device)
+  engine.tape_op(lambda: out.copy_(x))
+  return out
+
+
 def rows_for_tma(x):
   """x [.., R, C] bf16 itself, or a packed copy, with C contiguous."""
   return x if _fits(x, -1, -2) else pack(x)

@@ -137,11 +137,9 @@ def _backward(step, g, grads):
                      f'{(m, n)}')
   dlhs = drhs = None
   if cfg is None:
-    if g.dtype != torch.bfloat16:
-      g = g.to(torch.bfloat16)
     with be.on_device_of(g):
       step.keep.about_to_use()
-      g = be.rows_for_tma(g)
+      g = be.rows_for_tma(be.as_bf16(g))
       if need_l:
         dlhs = be.bf16_rows(g, step.rhs, 2, sizes, step.lhs_dtype)
       if need_r:

@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 import torch
 
+from aqt_b200 import engine
 from aqt_b200.v2 import aqt_dot_general
 from aqt_b200.v2 import aqt_ragged_dot as rd
 from aqt_b200.v2 import block_scaled as bs
@@ -303,3 +304,47 @@ def test_products_that_follow_their_quantizer(monkeypatch):
   rd.ragged_dot(x, bs.block_quantize(wg, 1, square=True), s, cfg=cfg)
   rd.ragged_dot(x, wg, s)
   assert flags() == [1, 1, 0]
+
+
+@pytest.fixture
+def temporaries(monkeypatch):
+  """Conversions torch makes stay allocated, as in the blocks of a caching
+  allocator that nobody has been given yet."""
+  held = []
+  to = torch.Tensor.to
+
+  def hold(t, *args, **kw):
+    held.append(to(t, *args, **kw))
+    return held[-1]
+
+  monkeypatch.setattr(torch.Tensor, 'to', hold)
+  return held
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('layout', [lambda t: t, _off, _flip])
+@pytest.mark.parametrize('q', [False, True])
+def test_traced_ragged_step_reads_the_new_cotangent(temporaries, dtype, layout, q):
+  """A replayed step follows its operands, a float32 cotangent among them, which
+  the bfloat16 products need rounded."""
+  m, k, n = 12, 40, 24
+  x, w, s = (_data((m, k), torch.bfloat16, 90), _data(
+      (3, k, n), torch.bfloat16, 91), torch.tensor([5, 0, 6]))
+  g = layout(_data((m, n), dtype, 92))
+  cfg = bs.dot_general_make() if q else None
+
+  def step(x, w, g):
+    out, bp = rd.ragged_dot_vjp(x, w, s, cfg=cfg, preferred_element_type=dtype)
+    return (out, *bp(g))
+
+  temporaries.clear()
+  traced = engine.TracedStep(step, x, w, g)
+  inside = list(temporaries)
+  for i in range(2):
+    for t, seed in ((x, 93), (w, 94), (g, 95)):
+      t.copy_(_data(t.shape, t.dtype, seed + 10 * i))
+    for t in inside:
+      t.fill_(7)  # handed to somebody else meanwhile
+    got = [t.clone() for t in traced(x, w, g)]
+    for a, b in zip(got, step(x, w, g)):
+      assert torch.equal(a, b)

@@ -443,3 +443,32 @@ def test_step_in_wide_tiles(m, k, n, sizes, q, out):
     _check(got, wt, HALF[got.dtype], name)
   left = sum(sizes)
   assert not y[left:].any() and not dl[left:].any()
+
+
+@pytest.mark.parametrize('q', [False, True])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_traced_step(q, dtype):
+  """Replayed on new operands, after other work has used the memory between."""
+  m, k, n = 130, 136, 77
+  x, w, g = (_data((m, k), torch.bfloat16, 63), _data(
+      (3, k, n), torch.bfloat16, 64, 0.1), _data((m, n), dtype, 65))
+  sizes = _sizes([70, 0, 55])
+  cfg = bs.dot_general_make() if q else None
+
+  def step(x, w, g):
+    out, bp = rd.ragged_dot_vjp(x, w, sizes, cfg=cfg, preferred_element_type=dtype)
+    return (out, *bp(g))
+
+  traced = engine.TracedStep(step, x, w, g)
+  for turn in range(3):
+    for i, t in enumerate((x, w, g)):
+      t.copy_(_data(t.shape, t.dtype, 66 + 3 * turn + i, 0.1))
+    # blocks of every size a temporary of the step may have had
+    junk = [torch.full((1 << b,), float('nan'), dtype=torch.bfloat16, device='cuda')
+            for b in range(5, 21) for _ in range(4)]
+    del junk
+    got = [t.clone() for t in traced(x, w, g)]
+    want = step(x, w, g)
+    _done()
+    for a, b in zip(got, want):
+      assert torch.equal(a, b)
