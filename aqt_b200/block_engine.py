@@ -342,6 +342,15 @@ def as_bf16(x):
   return out
 
 
+def padded_rows(q):
+  """A copy of fp8 [.., R, C] with C contiguous and rows of whole 16 bytes."""
+  n = q.shape[-1]
+  buf = _empty_out((*q.shape[:-1], (n + 15) & -16), torch.uint8, q.device)
+  q8, rows = q.view(torch.uint8), buf[..., :n]
+  engine.tape_op(lambda: (buf.zero_(), rows.copy_(q8)))
+  return rows.view(q.dtype)
+
+
 def rows_for_tma(x):
   """x [.., R, C] bf16 itself, or a packed copy, with C contiguous."""
   return x if _fits(x, -1, -2) else pack(x)

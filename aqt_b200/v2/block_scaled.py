@@ -94,7 +94,7 @@ def frozen(qvalue, scale, contract_axis: int = -2) -> aqt_tensor.QTensor:
   values [K, N] or [G, K, N] and scales [.., ceil(K/128), ceil(N/128)].
 
   The product needs the contraction axis contiguous in memory; values that lie
-  otherwise are copied once, here.
+  otherwise are copied once, here (by a traced step: on every replay).
   """
   be.check_operand(qvalue, 'qvalue', be._FP8)  # pylint: disable=protected-access
   be.check_operand(scale, 'scale', (torch.float32,))
@@ -110,10 +110,7 @@ def frozen(qvalue, scale, contract_axis: int = -2) -> aqt_tensor.QTensor:
   if not _contract_contiguous(qvalue, axis):
     with be.on_device_of(qvalue):
       v = qvalue if axis == -1 else qvalue.transpose(-1, -2)
-      ld = -(-v.shape[-1] // 16) * 16
-      buf = torch.zeros(*v.shape[:-1], ld, dtype=torch.uint8, device=v.device)
-      buf[..., :v.shape[-1]] = v.view(torch.uint8)
-      v = buf[..., :v.shape[-1]].view(qvalue.dtype)
+      v = be.padded_rows(v)
       qvalue = v if axis == -1 else v.transpose(-1, -2)
   return aqt_tensor.QTensor(
       qvalue=qvalue, scale=[scale], scale_t=None, dequant_dtype=None,

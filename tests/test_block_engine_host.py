@@ -348,3 +348,32 @@ def test_traced_ragged_step_reads_the_new_cotangent(temporaries, dtype, layout, 
     got = [t.clone() for t in traced(x, w, g)]
     for a, b in zip(got, step(x, w, g)):
       assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('k,n', [(200, 24), (256, 130)])
+@pytest.mark.parametrize('ragged', [False, True])
+def test_traced_step_that_freezes_weights(monkeypatch, k, n, ragged):
+  """Values of another layout, brought into the product's inside the step."""
+  held = []
+  zeros = torch.zeros
+  monkeypatch.setattr(torch, 'zeros',
+                      lambda *a, **kw: held.append(zeros(*a, **kw)) or held[-1])
+  lead = (2,) if ragged else ()
+  qt = bs.block_quantize(_data((*lead, k, n), torch.bfloat16, 96), -2, square=True)
+  other = bs.block_quantize(_data((*lead, k, n), torch.bfloat16, 97), -2, square=True)
+  values, scales = qt.qvalue.contiguous(), qt.scale[0].clone()
+  x, s = _data((9, k), torch.bfloat16, 98), torch.tensor([4, 4])
+  cfg = bs.dot_general_make()
+
+  def step(x):
+    w = bs.frozen(values, scales)
+    return rd.ragged_dot(x, w, s, cfg=cfg) if ragged else cfg(x, w, DIMS)
+
+  held.clear()
+  traced = engine.TracedStep(step, x)
+  for t in held:
+    t.fill_(9)  # handed to somebody else meanwhile
+  assert torch.equal(traced(x), step(x))
+  values.copy_(other.qvalue)
+  scales.copy_(other.scale[0])
+  assert torch.equal(traced(x), step(x))
