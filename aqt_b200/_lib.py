@@ -177,6 +177,7 @@ SYMBOLS = {
         C.POINTER(GroupedGemmDesc)]),
     'aqtb200_grouped_gemm': (C.c_int, [
         C.POINTER(GroupedGemmDesc), C.c_void_p, C.c_void_p]),
+    'aqtb200_status_words': (C.c_int, [C.POINTER(C.c_void_p)]),
     'aqtb200_pack_bf16': (C.c_int, [
         C.POINTER(View), C.c_void_p, C.c_int64, C.c_void_p]),
     'aqtb200_pack_bf16_groups': (C.c_int, [

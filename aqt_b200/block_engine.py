@@ -238,25 +238,13 @@ def _check(rc, what):
 
 
 def _gemm(desc, device, what):
+  # a product of an earlier call that gave up is reported by the next one
+  words = engine.status_words(device)
+  if words[0]:
+    engine.poll_words(words)
   _check(engine._call(  # pylint: disable=protected-access
-      _lib.load().aqtb200_grouped_gemm, C.byref(desc), _status(device),
-      engine._stream()), what)  # pylint: disable=protected-access
-
-
-def _status(device):
-  """Address of the device's status words. A first call under graph capture goes
-  without: the words would be memory of that graph."""
-  at = _status_at.get(device)
-  if at is None:
-    if (device.type == 'cuda' and str(device) not in engine._status and  # pylint: disable=protected-access
-        torch.cuda.is_current_stream_capturing()):
-      return None
-    # the engine keeps the words for good
-    at = _status_at[device] = engine._status_buf(device).data_ptr()  # pylint: disable=protected-access
-  return at
-
-
-_status_at = {}
+      _lib.load().aqtb200_grouped_gemm, C.byref(desc), words, engine._stream()),  # pylint: disable=protected-access
+         what)
 
 
 def _sizes(group_sizes):

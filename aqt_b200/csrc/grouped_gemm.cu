@@ -194,6 +194,12 @@ __device__ __forceinline__ void tc_copy_scales(uint32_t elected, uint32_t tmem, 
       : "memory");
 }
 
+// Notes that a bounded wait ran out. A plain store, since the words may lie in the
+// host's memory; of several codes either may stay.
+__device__ __forceinline__ void report(int32_t* status, int code) {
+  if (status != nullptr) *(volatile int32_t*)status = code;
+}
+
 // Waits for what a kernel launched before this one wrote; returns at once unless
 // this one was launched early.
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
@@ -590,7 +596,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       if (fail && lane == 0) {
         *abortp = 1;
         st_cluster_u32(peer_abort, 1u);
-        if (P.status) atomicCAS(P.status, 0, 1);
+        report(P.status, 1);
       }
     }
     __syncwarp();
@@ -669,7 +675,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       if (fail && lane == 0) {
         *abortp = 1;
         st_cluster_u32(peer_abort, 1u);
-        if (P.status) atomicCAS(P.status, 0, 2);
+        report(P.status, 2);
       }
     }
     __syncwarp();
@@ -754,7 +760,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       if (fail && lane == 0) {
         *abortp = 1;
         st_cluster_u32(peer_abort, 1u);
-        if (P.status) atomicCAS(P.status, 0, 4);
+        report(P.status, 4);
       }
     }
     if (SUMS && warp == 2) {
@@ -794,7 +800,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       if (fail && lane == 0) {
         *abortp = 1;
         st_cluster_u32(peer_abort, 1u);
-        if (P.status) atomicCAS(P.status, 0, 4);
+        report(P.status, 4);
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
     }
@@ -1060,7 +1066,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     if (fail && lane == 0) {
       *abortp = 1;
       st_cluster_u32(peer_abort, 1u);
-      if (P.status) atomicCAS(P.status, 0, 3);
+      report(P.status, 3);
     }
   }
 

@@ -106,6 +106,20 @@ int aqtb200_d2h(void* dst, const void* src, size_t bytes, void* stream) {
   AQT_CUDA_OK(cudaMemcpyAsync(dst, src, bytes, cudaMemcpyDeviceToHost, (cudaStream_t)stream));
   return 0;
 }
+int aqtb200_status_words(int32_t** out) {
+  AQT_REQUIRE(out != nullptr, AQTB200_EINVAL, "null status words");
+  // an allocation is not work on a stream: allow it beside one that is captured
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  AQT_CUDA_OK(cudaThreadExchangeStreamCaptureMode(&mode));
+  void* p = nullptr;
+  const cudaError_t e = cudaHostAlloc(&p, 4 * sizeof(int32_t), cudaHostAllocPortable | cudaHostAllocMapped);
+  AQT_CUDA_OK(cudaThreadExchangeStreamCaptureMode(&mode));
+  AQT_CUDA_OK(e);
+  memset(p, 0, 4 * sizeof(int32_t));
+  *out = (int32_t*)p;
+  return 0;
+}
+
 int aqtb200_sync(void* stream) {
   AQT_CUDA_OK(cudaStreamSynchronize((cudaStream_t)stream));
   return 0;

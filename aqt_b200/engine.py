@@ -110,8 +110,45 @@ def _status_buf(device):
   return _status[key]
 
 
+_words = {}  # device -> int32[4] that its kernels and the host both address
+
+
+def status_words(device):
+  """The device's status words in host memory its kernels can write.
+
+  A look at them costs the host a load and the stream nothing, and they exist
+  apart from any allocator's pool: a first call under graph capture can have
+  them, and what a replay reports stays readable. Kept for the process's life.
+  """
+  words = _words.get(device)
+  if words is None:
+    if device.type == 'cuda':
+      at = C.c_void_p()
+      _lib.check(_lib.load().aqtb200_status_words(C.byref(at)), 'status_words')
+      words = (C.c_int32 * 4).from_address(at.value)
+    else:
+      words = (C.c_int32 * 4)()
+    words = _words.setdefault(device, words)
+  return words
+
+
+def poll_words(words):
+  """Raises if a kernel has reported there that it gave up; no synchronisation,
+  so a call reports what ended before it."""
+  code = words[0]
+  if code:
+    words[0] = 0
+    raise _lib.AqtB200Error(
+        f'GEMM kernel gave up waiting on a barrier (role {code}); results '
+        'since the last check are incomplete')
+
+
 def check_status():
   """Raises if a kernel reported a bounded wait that ran out (syncs)."""
+  for device, words in _words.items():
+    if device.type == 'cuda':
+      torch.cuda.synchronize(device)
+    poll_words(words)
   for buf in _status.values():
     code = int(buf[0].item())
     if code:
@@ -1801,6 +1838,8 @@ class TracedStep:
           'a traced step runs on the tensors it was traced with')
     assert _stream() == self._stream, (
         'a traced step replays on the stream it was traced on')
+    for words in _words.values():
+      poll_words(words)
     for fn, args in self._tape.ops:
       if args is None:
         fn()

@@ -444,6 +444,11 @@ int aqtb200_dev_memset(void* ptr, int value, size_t bytes, void* stream);
 int aqtb200_h2d(void* dst, const void* src, size_t bytes, void* stream);
 int aqtb200_d2h(void* dst, const void* src, size_t bytes, void* stream);
 int aqtb200_sync(void* stream);
+/* Status words (four, zero) in page-locked host memory that the kernels of the
+ * current device write as well, for aqtb200_grouped_gemm: a host that looks at
+ * them needs no copy and no synchronisation. A new set on every call, never
+ * freed. May be called while a stream is being captured. */
+int aqtb200_status_words(int32_t** out);
 /* Peer memory for the fused exchange: a 64-byte handle of a device allocation
  * (ptr: its base address, e.g. from aqtb200_dev_alloc) that another process on
  * the same node opens as a pointer valid on ITS current device (peer access is
@@ -641,7 +646,7 @@ int aqtb200_block_quantize(const aqtb200_block_quant_desc* desc, void* stream);
  * workspace : contract_groups 1 in bf16 with groups: aqtb200_grouped_gemm_
  *             workspace_bytes() bytes, 256-byte aligned; otherwise unused.
  * out       : F32 | BF16, (t, r) at g*out_group_stride + t*out_ld + r.
- * status    : as for aqtb200_gemm_dequant.
+ * status    : as for aqtb200_gemm_dequant, or words from aqtb200_status_words.
  */
 #define AQTB200_MAX_GROUPS 1024
 typedef struct aqtb200_grouped_gemm_desc {

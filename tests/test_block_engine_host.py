@@ -377,3 +377,47 @@ def test_traced_step_that_freezes_weights(monkeypatch, k, n, ragged):
   values.copy_(other.qvalue)
   scales.copy_(other.scale[0])
   assert torch.equal(traced(x), step(x))
+
+
+@pytest.fixture
+def gives_up(monkeypatch):
+  """Products that report a wait that ran out, as many as the list says."""
+  from aqt_b200 import _lib
+  lib = _lib.load()
+  gemm, left = lib.aqtb200_grouped_gemm, []
+
+  def failing(desc, status, stream):
+    if left:
+      status[0] = left.pop()
+    return gemm(desc, status, stream)
+
+  monkeypatch.setattr(lib, 'aqtb200_grouped_gemm', failing, raising=False)
+  yield left
+  engine._words.clear()  # pylint: disable=protected-access
+
+
+@pytest.mark.parametrize('run', ['dot', 'frozen', 'ragged', 'ragged fp8'])
+def test_a_product_that_gave_up_is_reported(gives_up, run):
+  from aqt_b200 import _lib
+  x, w = _data((9, 40), torch.bfloat16, 100), _data((40, 24), torch.bfloat16, 101)
+  s, cfg = torch.tensor([9]), bs.dot_general_make()
+  call = {'dot': lambda: cfg(x, w, DIMS),
+          'frozen': lambda: cfg(x, bs.block_quantize(w, 0, square=True), DIMS),
+          'ragged': lambda: rd.ragged_dot(x, w[None], s),
+          'ragged fp8': lambda: rd.ragged_dot(x, w[None], s, cfg=cfg)}[run]
+  good = call()
+  gives_up.append(3)
+  call()
+  with pytest.raises(_lib.AqtB200Error, match='role 3'):
+    call()
+  assert torch.equal(call(), good)  # said once
+  gives_up.append(1)
+  call()
+  with pytest.raises(_lib.AqtB200Error, match='role 1'):
+    engine.check_status()
+  engine.check_status()
+  traced = engine.TracedStep(lambda a: call(), x)
+  gives_up.append(2)
+  traced(x)
+  with pytest.raises(_lib.AqtB200Error, match='role 2'):
+    traced(x)
