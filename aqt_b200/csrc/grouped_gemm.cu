@@ -499,7 +499,15 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const int nseg = nseg_s;
   const int total = total_s;
   volatile int* abortp = &abort_flag;
-  const uint32_t peer_abort = map_to_cta(smem_u32(&abort_flag), PAIR ? crank ^ 1u : crank);
+  // A role whose wait ran out: every CTA of the cluster stops waiting, and no part of
+  // a shared contraction is added up (all signals come before the barrier ahead of
+  // the sum).
+  auto give_up = [&](int code) {
+    if (lane != 0) return;
+    const uint32_t flag = smem_u32(&abort_flag);
+    for (int c = 0; c < CTAS * P.split; ++c) st_cluster_u32(map_to_cta(flag, c), 1u);
+    report(P.status, code);
+  };
   const int slab_bytes = GG_A_STAGE + P.b_stage, stage_bytes = KS * slab_bytes;
   float* const slots = (float*)(smem + P.stages * stage_bytes);
   int fail = 0;
@@ -593,11 +601,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           if (++stage == P.stages) { stage = 0; phase ^= 1; }
         }
       }
-      if (fail && lane == 0) {
-        *abortp = 1;
-        st_cluster_u32(peer_abort, 1u);
-        report(P.status, 1);
-      }
+      if (fail) give_up(1);
     }
     __syncwarp();
     if (P.split > 1) cluster_sync_all();
@@ -672,11 +676,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           if (++stage == P.stages) { stage = 0; phase ^= 1; }
         }
       }
-      if (fail && lane == 0) {
-        *abortp = 1;
-        st_cluster_u32(peer_abort, 1u);
-        report(P.status, 2);
-      }
+      if (fail) give_up(2);
     }
     __syncwarp();
     if (P.split > 1) cluster_sync_all();
@@ -757,11 +757,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       }
       while (done < issued && !fail)
         if (!convert()) fail = 4;
-      if (fail && lane == 0) {
-        *abortp = 1;
-        st_cluster_u32(peer_abort, 1u);
-        report(P.status, 4);
-      }
+      if (fail) give_up(4);
     }
     if (SUMS && warp == 2) {
       int slot = 0, cur = 0;
@@ -797,11 +793,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           if (++slot == SLOTS) { slot = 0; phase ^= 1; }
         }
       }
-      if (fail && lane == 0) {
-        *abortp = 1;
-        st_cluster_u32(peer_abort, 1u);
-        report(P.status, 4);
-      }
+      if (fail) give_up(4);
       asm volatile("cp.async.wait_all;" ::: "memory");
     }
     __syncwarp();
@@ -1030,6 +1022,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       if (fail) break;
       if (P.split == 1) store(tile);
     }
+    if (fail) give_up(3);
     if (P.split > 1) {
       // Parts of one tile: parts 1.. leave their sums in their own shared memory
       // (the operand ring is idle by now), part 0 adds them in part order.
@@ -1044,7 +1037,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       }
       __syncwarp();
       cluster_sync_all();
-      if (busy && part == 0) {
+      if (busy && part == 0 && !*abortp) {
         for (int p = 1; p < P.split; ++p) {
           const uint32_t from = map_to_cta(smem_u32(mine), CTAS * p + rank);
           float4 v[GROUPS * 2];
@@ -1063,11 +1056,6 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       }
     }
     if (TMA_OUT && lane == 0) tma_store_wait_read();  // shared memory outlives its last store
-    if (fail && lane == 0) {
-      *abortp = 1;
-      st_cluster_u32(peer_abort, 1u);
-      report(P.status, 3);
-    }
   }
 
   __syncwarp();
