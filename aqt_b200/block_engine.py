@@ -103,6 +103,13 @@ class Side:
     self.scale_k, self.scale_r = scale_k, scale_r
     self.kept, self.keep = kept, keep
 
+  def at(self, base, memory):
+    """This operand with its memory, once at `base`, in `memory` (or in none)."""
+    shift = 0 if memory is None else memory.data_ptr() - base
+    return Side(self.ptr + shift, self.ld, self.group, self.code,
+                self.scale + shift, self.scale_group, self.scale_k, self.scale_r,
+                self.kept, memory)
+
 
 def _align(n):
   return (n + 255) & -256
@@ -398,20 +405,51 @@ def bf16_contract_rows(lhs, g, group_sizes, out_dtype):
 
 
 class Residuals:
-  """Buffers a backward pass reads (tensors, or the memory of Sides). They are torch allocations of the forward
-  pass's stream; used on another one, the allocator is told before they can be
-  handed out again."""
+  """The operands a backward pass reads: Sides, tensors or None.
 
-  __slots__ = ('stream', 'tensors')
+  Their memory is torch allocations of the forward pass's stream; used on
+  another one, the allocator is told before it can be handed out again. On
+  torch's tape the graph keeps it, not this object: release() hands it out for
+  save_for_backward, and regain() takes what the graph gives back, which hooks may
+  have moved.
+  """
 
-  def __init__(self, *of):
-    self.tensors = [s.keep if isinstance(s, Side) else s for s in of
-                    if s is not None]
+  __slots__ = ('lhs', 'rhs', 'stream', 'base')
+
+  def __init__(self, lhs, rhs):
+    self.lhs, self.rhs = lhs, rhs
     self.stream = engine._stream()  # pylint: disable=protected-access
+    self.base = None
+
+  def memory(self):
+    return tuple(s.keep if isinstance(s, Side) else s
+                 for s in (self.lhs, self.rhs))
 
   def about_to_use(self):
     """Called with the operands' device current."""
     if engine._stream() != self.stream:  # pylint: disable=protected-access
-      for t in self.tensors:
-        if t.is_cuda:
+      for t in self.memory():
+        if t is not None and t.is_cuda:
           t.record_stream(torch.cuda.current_stream())
+
+  def release(self):
+    memory = self.memory()
+    self.base = tuple(t if t is None else t.data_ptr() for t in memory)
+    self.lhs, self.rhs = (s.at(0, None) if isinstance(s, Side) else None
+                          for s in (self.lhs, self.rhs))
+    return memory
+
+  def regain(self, *memory):
+    r = object.__new__(Residuals)
+    r.stream, r.base = self.stream, None
+    r.lhs, r.rhs = (_regain(s, base, t) for s, base, t in zip(
+        (self.lhs, self.rhs), self.base, memory))
+    return r
+
+
+def _regain(side, base, t):
+  if side is None or t is None:
+    return t
+  if t.data_ptr() != base and (t.data_ptr() % 256 or not t.is_contiguous()):
+    t = t.clone(memory_format=torch.contiguous_format)  # aligned as at first
+  return side.at(base, t)

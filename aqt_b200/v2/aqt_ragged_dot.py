@@ -60,7 +60,8 @@ def ragged_dot_vjp(lhs, rhs, group_sizes, cfg=None, preferred_element_type=None)
   out_dtype = _check(lhs, rhs, group_sizes, cfg, preferred_element_type)
   out, step = _forward(lhs.detach(), rhs.detach(), group_sizes, cfg, out_dtype,
                        (True, True))
-  return out, lambda g: _backward(step, g.detach(), (True, True))
+  return out, lambda g: _backward(step, step.operands, group_sizes, g.detach(),
+                                  (True, True))
 
 
 def _check(lhs, rhs, group_sizes, cfg, preferred):
@@ -88,8 +89,8 @@ def _check(lhs, rhs, group_sizes, cfg, preferred):
 
 
 class _Step:
-  __slots__ = ('cfg', 'lhs', 'rhs', 'copied', 'sizes', 'keep', 'lhs_dtype',
-               'rhs_dtype', 'shape')
+  __slots__ = ('cfg', 'operands', 'copied', 'device', 'lhs_dtype', 'rhs_dtype',
+               'shape')
 
 
 def _forward(lhs, rhs, sizes, cfg, out_dtype, grads):
@@ -98,7 +99,7 @@ def _forward(lhs, rhs, sizes, cfg, out_dtype, grads):
   with be.on_device_of(lhs):
     if need_l or need_r:
       step = _Step()
-      step.cfg, step.sizes = cfg, sizes
+      step.cfg, step.device = cfg, lhs.device
       step.lhs_dtype, step.rhs_dtype = lhs.dtype, rhs.dtype
       step.shape = (*lhs.shape, rhs.shape[2])
     if cfg is None:
@@ -106,11 +107,9 @@ def _forward(lhs, rhs, sizes, cfg, out_dtype, grads):
       out = be.bf16_rows(l, w, 1, sizes, out_dtype)
       if step is not None:
         # a copy, where one had to be made, serves the backward pass too
-        step.lhs = l if need_r else None
-        step.rhs = w if need_l else None
+        step.operands = be.Residuals(l if need_r else None,
+                                     w if need_l else None)
         step.copied = l is not lhs, w is not rhs
-        step.keep = be.Residuals(*(t for t, c in zip(
-            (step.lhs, step.rhs), step.copied) if c))
       return out, step
     if isinstance(rhs, aqt_tensor.QTensor):
       w, w_n = block_scaled._frozen_operand(rhs, -2), None  # pylint: disable=protected-access
@@ -121,41 +120,42 @@ def _forward(lhs, rhs, sizes, cfg, out_dtype, grads):
     out = be.fp8_rows(l, w, lhs.shape[1], out_dtype, lhs.device, sizes,
                       cfg.po2_scale and not isinstance(rhs, aqt_tensor.QTensor))
     if step is not None:
-      step.lhs, step.rhs = l_t, w_n if need_l else None
-      step.keep = be.Residuals(step.lhs, step.rhs)
+      step.operands = be.Residuals(l_t, w_n if need_l else None)
   return out, step
 
 
-def _backward(step, g, grads):
+def _backward(step, operands, sizes, g, grads):
   need_l, need_r = grads
-  cfg, sizes = step.cfg, step.sizes
+  cfg = step.cfg
   m, k, n = step.shape
   be.check_operand(g, 'the cotangent')
-  be.check_same_device(sizes, g)
+  if g.device != step.device:
+    raise ValueError(
+        f'operands on different devices: {step.device}, {g.device}')
   if tuple(g.shape) != (m, n):
     raise ValueError(f'the cotangent has shape {tuple(g.shape)}, the result '
                      f'{(m, n)}')
   dlhs = drhs = None
   if cfg is None:
     with be.on_device_of(g):
-      step.keep.about_to_use()
+      operands.about_to_use()
       g = be.rows_for_tma(be.as_bf16(g))
       if need_l:
-        dlhs = be.bf16_rows(g, step.rhs, 2, sizes, step.lhs_dtype)
+        dlhs = be.bf16_rows(g, operands.rhs, 2, sizes, step.lhs_dtype)
       if need_r:
-        drhs = be.bf16_contract_rows(step.lhs, g, sizes, step.rhs_dtype)
+        drhs = be.bf16_contract_rows(operands.lhs, g, sizes, step.rhs_dtype)
     return dlhs, drhs
   with be.on_device_of(g):
-    step.keep.about_to_use()
+    operands.about_to_use()
     q, q_t = be.quantize(g, cfg.bwd_dtype, need_l, need_r, False, cfg.po2_scale,
                          sizes if need_r else None)
     if need_l:
-      dlhs = be.fp8_rows(q, step.rhs, n, step.lhs_dtype, g.device, sizes,
+      dlhs = be.fp8_rows(q, operands.rhs, n, step.lhs_dtype, g.device, sizes,
                          cfg.po2_scale)
     if need_r:
       # positions along the groups' padded rows, as both operands were laid out
-      drhs = be.fp8_contract_rows(step.lhs, q_t, step.lhs.ld, m, step.rhs_dtype,
-                                  g.device, sizes, cfg.po2_scale)
+      drhs = be.fp8_contract_rows(operands.lhs, q_t, operands.lhs.ld, m,
+                                  step.rhs_dtype, g.device, sizes, cfg.po2_scale)
   return dlhs, drhs
 
 
@@ -165,17 +165,12 @@ class _RaggedDot(torch.autograd.Function):
   def forward(ctx, lhs, rhs, sizes, cfg, out_dtype):
     out, step = _forward(lhs.detach(), rhs.detach(), sizes, cfg, out_dtype,
                          ctx.needs_input_grad[:2])
+    l, w = step.operands.release()
     if cfg is None:
       # operands themselves: saved the way torch watches for writes into them
-      own = [t is not None and not c
-             for t, c in zip((step.lhs, step.rhs), step.copied)]
-      ctx.save_for_backward(sizes, lhs if own[0] else None,
-                            rhs if own[1] else None)
-      step.lhs = None if own[0] else step.lhs
-      step.rhs = None if own[1] else step.rhs
-    else:
-      ctx.save_for_backward(sizes)
-    step.sizes = None
+      l = lhs if l is not None and not step.copied[0] else l
+      w = rhs if w is not None and not step.copied[1] else w
+    ctx.save_for_backward(sizes, l, w)
     ctx.step = step
     return out
 
@@ -183,12 +178,13 @@ class _RaggedDot(torch.autograd.Function):
   @once_differentiable
   def backward(ctx, g):
     step = ctx.step
-    step.sizes = ctx.saved_tensors[0]
-    copies = step.lhs, step.rhs
+    sizes, lhs, rhs = ctx.saved_tensors
+    # hooks on saved tensors may give them back in other strides
+    sizes = sizes.contiguous()
     if step.cfg is None:
-      _, lhs, rhs = ctx.saved_tensors
-      step.lhs = step.lhs if lhs is None else lhs.detach()
-      step.rhs = step.rhs if rhs is None else rhs.detach()
-    dlhs, drhs = _backward(step, g, ctx.needs_input_grad[:2])
-    step.lhs, step.rhs = copies
+      with be.on_device_of(sizes):
+        lhs = None if lhs is None else be.rows_for_tma(lhs.detach())
+        rhs = None if rhs is None else be.matrices_for_tma(rhs.detach(), sizes)
+    dlhs, drhs = _backward(step, step.operands.regain(lhs, rhs), sizes, g,
+                           ctx.needs_input_grad[:2])
     return dlhs, drhs, None, None, None

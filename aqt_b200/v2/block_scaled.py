@@ -169,7 +169,7 @@ _CODES = {torch.float8_e4m3fn: _lib.E4M3, torch.float8_e5m2: _lib.E5M2}
 class _Step:
   """One forward product's operands, as its backward pass needs them."""
 
-  __slots__ = ('lhs', 'rhs', 'keep', 'rows', 'k', 'n', 'lhs_shape', 'lhs_axis',
+  __slots__ = ('operands', 'device', 'rows', 'k', 'n', 'lhs_shape', 'lhs_axis',
                'rhs_axis', 'lhs_dtype', 'rhs_dtype')
 
 
@@ -209,7 +209,8 @@ class BlockScaledDotGeneral:
     out_dtype = _out_dtype(preferred_element_type, lhs)
     out, step = self._forward(lhs.detach(), rhs.detach(), dims, out_dtype,
                               (True, True))
-    return out, lambda g: self._backward(step, g.detach(), (True, True))
+    return out, lambda g: self._backward(step, step.operands, g.detach(),
+                                         (True, True))
 
   def _forward(self, lhs, rhs, dims, out_dtype, grads):
     lhs_axis, rhs_axis = dims
@@ -233,8 +234,8 @@ class BlockScaledDotGeneral:
       step = None
       if need_l or need_r:
         step = _Step()
-        step.lhs, step.rhs = l_t, w_t if need_l else None
-        step.keep = be.Residuals(step.lhs, step.rhs)
+        step.operands = be.Residuals(l_t, w_t if need_l else None)
+        step.device = device
         step.rows, step.k, step.n = m, k, w.kept
         step.lhs_shape, step.lhs_axis, step.rhs_axis = lhs.shape, lhs_axis, rhs_axis
         step.lhs_dtype, step.rhs_dtype = lhs.dtype, rhs.dtype
@@ -242,11 +243,13 @@ class BlockScaledDotGeneral:
       out = out.view(*lhs.shape[:-1], w.kept)
     return out, step
 
-  def _backward(self, step, g, grads):
+  def _backward(self, step, operands, g, grads):
     need_l, need_r = grads
     m, k, n = step.rows, step.k, step.n
     be.check_operand(g, 'the cotangent')
-    be.check_same_device(step.keep.tensors[0], g)
+    if g.device != step.device:
+      raise ValueError(
+          f'operands on different devices: {step.device}, {g.device}')
     want = ((*step.lhs_shape[:-1], n) if step.lhs_axis == -1 else (m, n))
     if tuple(g.shape) != want:
       raise ValueError(f'the cotangent has shape {tuple(g.shape)}, the result '
@@ -255,15 +258,16 @@ class BlockScaledDotGeneral:
     gm = _as_matrix(g, -1)
     dlhs = drhs = None
     with be.on_device_of(g):
-      step.keep.about_to_use()
+      operands.about_to_use()
       q, q_t = be.quantize(gm, self.bwd_dtype, need_l, need_r, False,
                            self.po2_scale)
       if need_l:
-        dlhs = be.fp8_rows(q, step.rhs, n, step.lhs_dtype, device,
+        dlhs = be.fp8_rows(q, operands.rhs, n, step.lhs_dtype, device,
                            po2=self.po2_scale)
       if need_r:
         # [K, N] as rhs lies: its last axis is the output's contiguous one
-        b, a = (step.lhs, q_t) if step.rhs_axis == -2 else (q_t, step.lhs)
+        b, a = ((operands.lhs, q_t) if step.rhs_axis == -2 else
+                (q_t, operands.lhs))
         drhs = be.fp8_contract_rows(b, a, m, m, step.rhs_dtype, device,
                                     po2=self.po2_scale)
     if need_l:
@@ -282,13 +286,15 @@ class _BlockDot(torch.autograd.Function):
     ctx.cfg = cfg
     out, ctx.step = cfg._forward(  # pylint: disable=protected-access
         lhs.detach(), rhs.detach(), dims, out_dtype, ctx.needs_input_grad[:2])
+    ctx.save_for_backward(*ctx.step.operands.release())
     return out
 
   @staticmethod
   @once_differentiable
   def backward(ctx, g):
     dlhs, drhs = ctx.cfg._backward(  # pylint: disable=protected-access
-        ctx.step, g, ctx.needs_input_grad[:2])
+        ctx.step, ctx.step.operands.regain(*ctx.saved_tensors), g,
+        ctx.needs_input_grad[:2])
     return dlhs, drhs, None, None, None
 
 

@@ -421,3 +421,98 @@ def test_a_product_that_gave_up_is_reported(gives_up, run):
   traced(x)
   with pytest.raises(_lib.AqtB200Error, match='role 2'):
     traced(x)
+
+
+def _graphs():
+  """name -> (leaves, cotangent, product of the leaves)."""
+  m, k, n, s = 12, 41, 24, torch.tensor([5, 0, 6])
+  cfg = bs.dot_general_make()
+  x, g = _data((m, k), torch.bfloat16, 110), _data((m, n), torch.bfloat16, 111)
+  w = _data((3, k, n), torch.bfloat16, 112)
+  return {
+      'dot': ([x, w[0]], g, lambda a, b: cfg(a, b, DIMS)),
+      'ragged': ([x, w], g, lambda a, b: rd.ragged_dot(a, b, s)),
+      'ragged own': ([x[:, :40], w[:, :40]], g,
+                     lambda a, b: rd.ragged_dot(a, b, s)),
+      'ragged fp8': ([x, w], g, lambda a, b: rd.ragged_dot(a, b, s, cfg=cfg)),
+  }
+
+
+GRAPHS = ['dot', 'ragged', 'ragged own', 'ragged fp8']
+
+
+def _leaves(tensors):
+  return [t.clone().contiguous().requires_grad_() for t in tensors]
+
+
+@pytest.mark.parametrize('name', GRAPHS)
+def test_a_graph_is_used_up_by_its_backward_pass(name):
+  """As torch's own products: a second pass needs retain_graph, and what was kept
+  for the first goes with it although the result lives on."""
+  import gc
+  import weakref
+  from aqt_b200 import block_engine as be
+  tensors, g, run = _graphs()[name]
+  leaves = _leaves(tensors)
+  made = []
+
+  def watch(f):
+    def made_one(*args):
+      t = f(*args)
+      made.append(weakref.ref(t))
+      return t
+    return made_one
+
+  real = {f: getattr(be, f) for f in ('_scratch', '_empty_out')}
+  try:
+    for f in real:
+      setattr(be, f, watch(real[f]))
+    y = run(*leaves)
+  finally:
+    for f in real:
+      setattr(be, f, real[f])
+  gc.collect()
+  y.backward(g, retain_graph=True)
+  once = [t.grad.clone() for t in leaves]
+  for t in leaves:
+    t.grad = None
+  y.backward(g)
+  assert all(torch.equal(t.grad, o) for t, o in zip(leaves, once))
+  gc.collect()
+  left = [r() for r in made if r() is not None and r() is not y]
+  assert not left
+  with pytest.raises(RuntimeError, match='second time'):
+    y.backward(g)
+
+
+@pytest.mark.parametrize('name', GRAPHS)
+@pytest.mark.parametrize('strided', [False, True])
+def test_hooks_on_saved_tensors_see_the_residuals(name, strided):
+  """Offloading and the like: what the hooks give back is what is read."""
+  tensors, g, run = _graphs()[name]
+  a = _leaves(tensors)
+  run(*a).backward(g)
+  b = _leaves(tensors)
+  packed = []
+
+  def pack(t):
+    packed.append(t)
+    return t.detach().clone()
+
+  def unpack(t):
+    if not strided:
+      return t
+    wide = torch.zeros(*t.shape, 2, dtype=t.dtype)
+    wide[..., 0] = t
+    return wide[..., 0]  # the same values, elements apart
+
+  with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+    y = run(*b)
+  own = {leaf.data_ptr() for leaf in b}
+  for t in packed:
+    if t.data_ptr() not in own and t.dtype in (torch.uint8, torch.bfloat16):
+      t.detach().zero_()  # its memory is somebody else's from here on
+  y.backward(g)
+  assert len(packed) >= 2
+  for s, t in zip(a, b):
+    assert torch.equal(s.grad, t.grad)

@@ -472,3 +472,39 @@ def test_traced_step(q, dtype):
     _done()
     for a, b in zip(got, want):
       assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize('q', [False, True])
+@pytest.mark.parametrize('k', [136, 133])
+def test_checkpointed_and_offloaded(q, k):
+  """Residuals that torch computes anew, or keeps in host memory meanwhile."""
+  from torch.utils.checkpoint import checkpoint
+  x, w, g = (_data((130, k), torch.bfloat16, 80), _data(
+      (3, k, 77), torch.bfloat16, 81, 0.1), _data((130, 77), torch.bfloat16, 82))
+  sizes = _sizes([70, 0, 55])
+  cfg = bs.dot_general_make() if q else None
+  dense = bs.dot_general_make()
+  dims = (((1,), (0,)), ((), ()))
+
+  def layer(a, b):
+    y = rd.ragged_dot(a, b, sizes, cfg=cfg)
+    return dense(y, b[0].t(), dims).mul(0.1) + a
+
+  def step(run):
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+    y = run(a, b)
+    filler = [torch.full((1 << i,), float('nan'), device='cuda') for i in range(5, 20)]
+    del filler
+    y.backward(x)
+    return y.detach(), a.grad, b.grad
+
+  def offloaded(a, b):
+    with torch.autograd.graph.save_on_cpu(pin_memory=True):
+      return layer(a, b)
+
+  want = step(layer)
+  for run in (offloaded, lambda a, b: checkpoint(layer, a, b, use_reentrant=False)):
+    got = step(run)
+    _done()
+    for s, t in zip(got, want):
+      assert torch.equal(s, t)
