@@ -24,6 +24,7 @@ import contextlib
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from aqt_b200 import _lib
 from aqt_b200 import engine
@@ -68,6 +69,10 @@ def check_operand(x, name, dtypes=_FLOATS):
     raise NotImplementedError(
         f'{name} has dtype {x.dtype}; handled here: '
         + ', '.join(str(d) for d in dtypes))
+  if forward_ad.unpack_dual(x).tangent is not None:
+    raise NotImplementedError(
+        f'{name} carries a forward-mode tangent; these products have gradients '
+        '(backward) only')
 
 
 def check_same_device(*tensors):

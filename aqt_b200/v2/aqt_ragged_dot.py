@@ -60,7 +60,7 @@ def ragged_dot_vjp(lhs, rhs, group_sizes, cfg=None, preferred_element_type=None)
   out_dtype = _check(lhs, rhs, group_sizes, cfg, preferred_element_type)
   out, step = _forward(lhs.detach(), rhs.detach(), group_sizes, cfg, out_dtype,
                        (True, True))
-  return out, lambda g: _backward(step, step.operands, group_sizes, g.detach(),
+  return out, lambda g: _backward(step, step.operands, group_sizes, g,
                                   (True, True))
 
 
@@ -129,6 +129,7 @@ def _backward(step, operands, sizes, g, grads):
   cfg = step.cfg
   m, k, n = step.shape
   be.check_operand(g, 'the cotangent')
+  g = g.detach()
   if g.device != step.device:
     raise ValueError(
         f'operands on different devices: {step.device}, {g.device}')

@@ -209,8 +209,7 @@ class BlockScaledDotGeneral:
     out_dtype = _out_dtype(preferred_element_type, lhs)
     out, step = self._forward(lhs.detach(), rhs.detach(), dims, out_dtype,
                               (True, True))
-    return out, lambda g: self._backward(step, step.operands, g.detach(),
-                                         (True, True))
+    return out, lambda g: self._backward(step, step.operands, g, (True, True))
 
   def _forward(self, lhs, rhs, dims, out_dtype, grads):
     lhs_axis, rhs_axis = dims
@@ -247,6 +246,7 @@ class BlockScaledDotGeneral:
     need_l, need_r = grads
     m, k, n = step.rows, step.k, step.n
     be.check_operand(g, 'the cotangent')
+    g = g.detach()
     if g.device != step.device:
       raise ValueError(
           f'operands on different devices: {step.device}, {g.device}')

@@ -246,3 +246,30 @@ def test_cotangent_on_another_device(monkeypatch, q):
   for back in backs:
     with pytest.raises(ValueError, match='different devices'):
       back(torch.zeros(4, 8, dtype=BF, device='meta'))
+
+
+def test_forward_mode_tangents(monkeypatch):
+  """Refused, not dropped: with or without a leaf that wants a gradient."""
+  from torch.autograd import forward_ad
+  from tests import fake_block_lib
+  fake_block_lib.install(monkeypatch)
+  cfg = bs.dot_general_make()
+  x, w = torch.ones(4, 128, dtype=BF), torch.ones(2, 128, 8, dtype=BF)
+  s = torch.tensor([2, 2], dtype=torch.int32)
+  qt, g = bs.block_quantize(w[0], 0, square=True), torch.ones(4, 8, dtype=BF)
+  backs = [cfg.vjp(x, w[0], DIMS)[1], rd.ragged_dot_vjp(x, w, s)[1]]
+  dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+  with forward_ad.dual_level():
+    calls = [lambda: cfg(dual(x), w[0], DIMS), lambda: cfg(x, dual(w[0]), DIMS),
+             lambda: cfg(dual(x), w[0].clone().requires_grad_(), DIMS),
+             lambda: cfg(dual(x), qt, DIMS), lambda: cfg.vjp(dual(x), w[0], DIMS),
+             lambda: bs.block_quantize(dual(x)),
+             lambda: rd.ragged_dot(dual(x), w, s),
+             lambda: rd.ragged_dot(x, dual(w), s, cfg=cfg),
+             lambda: rd.ragged_dot_vjp(dual(x), w, s, cfg=cfg)]
+    calls += [lambda back=back: back(dual(g)) for back in backs]
+    for i, call in enumerate(calls):
+      with pytest.raises(NotImplementedError, match='tangent'):
+        call()
+        pytest.fail(f'call {i} was not refused')
+    cfg(x, w[0], DIMS)  # a level without tangents of its operands
