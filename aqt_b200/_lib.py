@@ -93,6 +93,7 @@ class BlockQuantDesc(C.Structure):
       ('q_row', C.c_void_p), ('ld_row', C.c_int64), ('scale_row', C.c_void_p),
       ('q_col', C.c_void_p), ('ld_col', C.c_int64), ('scale_col', C.c_void_p),
       ('group_sizes', C.c_void_p), ('groups', C.c_int64),
+      ('far_row', C.c_void_p), ('far_col', C.c_void_p),
   ]
 
 
@@ -113,6 +114,10 @@ class GroupedGemmDesc(C.Structure):
       ('group_sizes', C.c_void_p), ('groups', C.c_int64),
       ('out', C.c_void_p), ('out_ld', C.c_int64), ('out_group_stride', C.c_int64),
       ('workspace', C.c_void_p), ('workspace_bytes', C.c_size_t),
+      ('a_far', C.c_void_p), ('a_far_k_stride', C.c_int64),
+      ('a_far_r_stride', C.c_int64),
+      ('b_far', C.c_void_p), ('b_far_k_stride', C.c_int64),
+      ('b_far_t_stride', C.c_int64), ('b_far_padded', C.c_int32),
   ]
 
 

@@ -13,6 +13,9 @@ quantized operand of this library; scales with the kept index contiguous):
                     col   q [C][ld], scale [R/128][C]     blocks along R
                     square: both orders of q, ONE scale [R/128][C/128]
 
+Row and col scales come with marks on those that f32 products have to be careful
+with (aqtb200_block_quantize's far_row, far_col); the products read them.
+
 The calls here are short next to their kernels' launches, so what a product
 needs between its kernels is one torch allocation, addressed by offsets, and
 operands travel as (address, stride) numbers rather than as tensor views.
@@ -99,21 +102,25 @@ class Side:
   """One operand of a product: values with the contraction contiguous and their
   scales, as addresses and strides. `keep` holds the memory."""
   __slots__ = ('ptr', 'ld', 'group', 'code', 'scale', 'scale_group', 'scale_k',
-               'scale_r', 'kept', 'keep')
+               'scale_r', 'kept', 'keep', 'far', 'far_k', 'far_kept',
+               'far_padded')
 
   def __init__(self, ptr, ld, group, code, scale, scale_group, scale_k, scale_r,
-               kept, keep):
+               kept, keep, far=None, far_k=0, far_kept=0, far_padded=0):
     self.ptr, self.ld, self.group, self.code = ptr, ld, group, code
     self.scale, self.scale_group = scale, scale_group
     self.scale_k, self.scale_r = scale_k, scale_r
     self.kept, self.keep = kept, keep
+    self.far, self.far_k, self.far_kept = far, far_k, far_kept
+    self.far_padded = far_padded
 
   def at(self, base, memory):
     """This operand with its memory, once at `base`, in `memory` (or in none)."""
     shift = 0 if memory is None else memory.data_ptr() - base
     return Side(self.ptr + shift, self.ld, self.group, self.code,
                 self.scale + shift, self.scale_group, self.scale_k, self.scale_r,
-                self.kept, memory)
+                self.kept, memory, None if self.far is None else self.far + shift,
+                self.far_k, self.far_kept, self.far_padded)
 
 
 def _align(n):
@@ -157,7 +164,7 @@ def quantize(x, dtype, row=True, col=False, square=False, po2=False,
     row_blocks = r // BLOCK + min(groups, r)
     int64 = int(group_sizes.dtype == torch.int64)
     sizes_ptr = group_sizes.data_ptr()
-  at_q_row = at_s_row = at_q_col = at_s_col = end = 0
+  at_q_row = at_s_row = at_q_col = at_s_col = at_f_row = at_f_col = end = 0
   if row:
     ld_row = (c + 15) & -16
     end = _align(batch * r * ld_row)
@@ -174,6 +181,14 @@ def quantize(x, dtype, row=True, col=False, square=False, po2=False,
     if not square:
       at_s_col = end
       end += _align(batch * row_blocks * c * 4)
+  marks = not square and batch == 1
+  if marks:
+    if row:
+      at_f_row = end
+      end += _align(row_blocks * nc * 8)
+    if col:
+      at_f_col = end
+      end += _align(row_blocks * nc * 8)
   ws = _scratch(end, x.device)
   base = ws.data_ptr()
   desc = _lib.BlockQuantDesc(
@@ -182,7 +197,9 @@ def quantize(x, dtype, row=True, col=False, square=False, po2=False,
       base + at_q_row if row else None, ld_row,
       base + at_s_row if row or square else None,
       base + at_q_col if col else None, ld_col,
-      base + at_s_col if col and not square else None, sizes_ptr, groups)
+      base + at_s_col if col and not square else None, sizes_ptr, groups,
+      base + at_f_row if marks and row else None,
+      base + at_f_col if marks and col else None)
   _check(engine._call(  # pylint: disable=protected-access
       _lib.load().aqtb200_block_quantize, C.byref(desc), engine._stream()),  # pylint: disable=protected-access
          'block_quantize')
@@ -191,11 +208,13 @@ def quantize(x, dtype, row=True, col=False, square=False, po2=False,
   if row:
     s = ((base + at_s_row, nr * nc, 1, nc) if square else
          (base + at_s_row, nc * r, r, 1))
-    a = Side(base + at_q_row, ld_row, r * ld_row, q, *s, r, ws)
+    a = Side(base + at_q_row, ld_row, r * ld_row, q, *s, r, ws,
+             base + at_f_row if marks else None, 1, nc, group_sizes is not None)
   if col:
     s = ((base + at_s_row, nr * nc, nc, 1) if square else
          (base + at_s_col, row_blocks * c, c, 1))
-    b = Side(base + at_q_col, ld_col, c * ld_col, q, *s, c, ws)
+    b = Side(base + at_q_col, ld_col, c * ld_col, q, *s, c, ws,
+             base + at_f_col if marks else None, nc, 1)
   return (b, a) if swap else (a, b)
 
 
@@ -283,7 +302,8 @@ def fp8_rows(tokens, a, k, out_dtype, device, group_sizes=None, po2=False):
       a.ptr, a.ld, a.group, tokens.ptr, tokens.ld, 0, 0, 1, int64, po2, 1,
       a.scale, a.scale_group, a.scale_k, a.scale_r,
       tokens.scale, tokens.scale_k, sizes, groups,
-      out.data_ptr(), r, 0, None, 0), device, 'block-scaled product')
+      out.data_ptr(), r, 0, None, 0, None, 0, 0, tokens.far, tokens.far_k,
+      tokens.far_kept, tokens.far_padded), device, 'block-scaled product')
   return out
 
 
@@ -299,7 +319,8 @@ def fp8_contract_rows(b, a, k, rows, out_dtype, device, group_sizes=None,
       1, a.code, b.code, engine._TORCH_CODE[out_dtype], r, t, k, rows,  # pylint: disable=protected-access
       a.ptr, a.ld, 0, b.ptr, b.ld, 0, 0, 0, int64, po2, 0,
       a.scale, 0, a.scale_k, 1, b.scale, b.scale_k, sizes, groups,
-      out.data_ptr(), r, t * r, None, 0), device, 'block-scaled product')
+      out.data_ptr(), r, t * r, None, 0, a.far, a.far_k, a.far_kept), device,
+        'block-scaled product')
   return out
 
 

@@ -18,6 +18,7 @@ SOURCES = ['quantize.cu', 'gemm.cu', 'block_quantize.cu', 'grouped_gemm.cu',
            'xla_ffi.cc']
 HEADERS = [os.path.join(CSRC, 'common.cuh'),
            os.path.join(CSRC, 'tcgen05.cuh'), os.path.join(CSRC, 'groups.cuh'),
+           os.path.join(CSRC, 'block_scales.cuh'),
            os.path.join(HERE, '..', 'include', 'aqt_b200.h')]
 NVCC_FLAGS = [
     '-gencode', 'arch=compute_100a,code=sm_100a', '-O3', '-lineinfo',

@@ -32,11 +32,13 @@
 // shared memory) and finds its tiles from that, so no call waits for the host.
 #include <cuda.h>
 #include <cudaTypedefs.h>
+#include <cuda_fp8.h>
 
 #include <algorithm>
 #include <atomic>
 #include <cstring>
 
+#include "block_scales.cuh"
 #include "groups.cuh"
 #include "tcgen05.cuh"
 
@@ -103,6 +105,15 @@ struct GGParams {
   int64_t sa_g, sa_k, sa_r;
   const float* b_scale;
   int64_t sb_k;
+  // marks of the quantizer on a's rows (row scales) or b's, eight bytes for 128 of them and
+  // a slab, or none; far_padded: by 128 rows of each group
+  const uint64_t* far;
+  int64_t far_k, far_t;
+  int far_padded;
+  // fp8 operands as far_tile reads them
+  const uint8_t *a, *b;
+  int64_t a_ld, a_g, b_ld;
+  int k, a_e5, b_e5;
   void* out;
   int out_f32;
   int out_staged;  // bf16 rows of whole 16-byte pieces
@@ -372,15 +383,150 @@ __device__ __forceinline__ int share_of(int nkb, int part, int split) {
   return (int)((int64_t)nkb * part / split);
 }
 
+// A block's sum times its two scales, where a factor or a product on the way leaves
+// f32's range and the result does not. |sum| is zero or between 2^-32 and 2^39 (128
+// products of e5m2 values), so the epilogue's one multiplication ahead of its add is
+// right with
+//   weights' blocks  the two scales' product as the factor, where that is normal
+//   row scales       the sum times the row's scale, where that lies in ROW_MIN .. ROW_MAX
+// Elements with a block of other scales are computed again, by far_tile, when all is
+// stored. (Nothing of this is in the epilogue's loop or between its tiles: choosing
+// slab by slab cost 2 to 5 %, a verdict on each tile 1 to 2 %, and a look at the scales
+// ahead of their use up to 20 % of a decode.)
+constexpr float GG_MIN_NORMAL = 0x1p-126f;
+constexpr float GG_ROW_MIN = 0x1p-94f, GG_ROW_MAX = 0x1p89f;
+template <bool A_ROW>
+__device__ __forceinline__ bool is_far(float ra, float s) {
+  if (!finite_nonzero(ra)) return false;
+  if constexpr (A_ROW) return fabsf(ra) < GG_ROW_MIN || fabsf(ra) > GG_ROW_MAX;
+  const float p = fabsf(s * ra);
+  return finite_nonzero(s) && (p < GG_MIN_NORMAL || p > SCALE_MAX_FLOAT);
+}
+// acc + sum * ra * s. Part of a far factor goes to the sum first; a far row scale is
+// brought 2^40 nearer to 1 for both products and sent back in the add.
+template <bool A_ROW>
+__device__ __forceinline__ float far_add(float acc, float sum, float ra, float s) {
+  const bool far = is_far<A_ROW>(ra, s);
+  if constexpr (A_ROW) {
+    if (!far) return fmaf(sum * ra, s, acc);
+    const bool small = fabsf(ra) < GG_ROW_MIN;
+    return fmaf(sum * (ra * (small ? 0x1p40f : 0x1p-40f)) * s, small ? 0x1p-40f : 0x1p40f, acc);
+  }
+  if (!far) return fmaf(sum, s * ra, acc);
+  if (fabsf(s * ra) < 1.f) return fmaf(sum * 0x1p-90f, (s * 0x1p45f) * (ra * 0x1p45f), acc);
+  return fmaf(sum * 0x1p120f, (s * 0x1p-60f) * (ra * 0x1p-60f), acc);
+}
+__device__ __forceinline__ float2 fp8_pair(uint32_t v, int e5) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)v, e5 ? __NV_E5M2 : __NV_E4M3);
+  return __half22float2(*(const __half2*)&h);
+}
+// Whether some of slabs kb0 .. kb1 of a CTA's tile, rows from row0 on, may be far: by the
+// scales of the weights' blocks, and by the quantizer's marks on the others.
+__device__ __forceinline__ const float* tile_a_scale(const GGParams& P, const TileAt& T, int row) {
+  return P.a_scale + (P.mode == 0 ? (int64_t)T.seg * P.sa_g : 0) + (int64_t)(T.k0 / 128) * P.sa_k +
+         (int64_t)row * P.sa_r;
+}
+__device__ __forceinline__ bool far_blocks(const GGParams& P, const TileAt& T, int kb0, int kb1, int row0,
+                                           int lane) {
+  const float* sa = tile_a_scale(P, T, min(row0, P.r - 1) >> 7);
+  bool may = false;
+  for (int kb = kb0 + lane; kb < kb1; kb += 32) may |= may_be_far(sa[kb * P.sa_k]);
+  return may;
+}
+template <bool A_ROW>
+__device__ __forceinline__ bool far_marks(const GGParams& P, const Segments& S, const TileAt& T, int kb0,
+                                          int kb1, int row0, int lane) {
+  if (P.far == nullptr) return false;
+  int first = min(row0, P.r - 1) / 128, last = first;  // blocks of 128 with a mark each
+  if constexpr (!A_ROW) {
+    int t = T.t0, before = 0;
+    if (P.far_padded) {
+      t -= S.off[T.seg];
+      for (int g = lane; g < T.seg; g += 32) before += (S.off[g + 1] - S.off[g] + 127) / 128;
+      before = __reduce_add_sync(0xffffffffu, before);
+    }
+    first = before + t / 128;
+    last = before + (t + T.tvalid - 1) / 128;
+  }
+  bool may = false;
+  for (int x = first; x <= last; ++x)
+    for (int kb = kb0 + lane; kb < kb1; kb += 32) may |= P.far[(T.k0 / 128 + kb) * P.far_k + x * P.far_t] != 0;
+  return may;
+}
+// Whether one is: every pair is tried.
+template <bool A_ROW>
+__device__ __forceinline__ bool far_scales(const GGParams& P, const TileAt& T, int kb0, int kb1, int row0,
+                                           int lane) {
+  const float* sa = tile_a_scale(P, T, A_ROW ? row0 : min(row0, P.r - 1) >> 7);
+  const float* sb = P.b_scale + (int64_t)(T.k0 / 128) * P.sb_k + T.t0;
+  const int count = A_ROW ? min(128, P.r - row0) : T.tvalid;
+  bool far = false;
+  for (int kb = kb0; kb < kb1; ++kb)
+    for (int c = lane; c < count; c += 32) {
+      const float v = A_ROW ? sa[c * P.sa_r + kb * P.sa_k] : sb[kb * P.sb_k + c];
+      far |= is_far<A_ROW>(A_ROW ? v : sa[kb * P.sa_k], v);
+    }
+  return __any_sync(0xffffffffu, far);
+}
+
+// Writes the elements of a warp's part of a tile -- rows from r0 on, `n` columns from c0
+// on -- that have a far block, from the operands in global memory. Other elements keep
+// their value, so that no result depends on its neighbours. A call of its own, off the
+// epilogue's registers.
+template <bool A_ROW, bool PAIR>
+__device__ __noinline__ void far_tile(const GGParams& P, const Segments& S, int nseg, int tile, int r0, int c0,
+                                      int n, int lane) {
+  int cur = 0;
+  const TileAt T = gg_tile<true, PAIR>(P, S, nseg, tile, cur);
+  const int row0 = T.r0 + r0, rows = P.r - row0, col0 = T.t0 + c0, cols = T.tvalid - c0;
+  const int64_t g = P.mode == 0 ? T.seg : 0;
+  for (int e = lane; e < 32 * n; e += 32) {
+    const int r = e & 31, c = e >> 5;
+    if (c >= cols || r >= rows) continue;
+    const float* sa = P.a_scale + g * P.sa_g + (int64_t)(A_ROW ? row0 + r : (row0 + r) >> 7) * P.sa_r;
+    const float* sb = P.b_scale + col0 + c;
+    bool far = false;
+    for (int kb = 0; kb < T.nkb && !far; ++kb) {
+      const int64_t at = T.k0 / 128 + kb;
+      far = is_far<A_ROW>(sa[at * P.sa_k], sb[at * P.sb_k]);
+    }
+    if (!far) continue;
+    const uint8_t* a = P.a + g * P.a_g + (int64_t)(row0 + r) * P.a_ld;
+    const uint8_t* b = P.b + (int64_t)(col0 + c) * P.b_ld;
+    float total = 0.f;
+    for (int kb = 0; kb < T.nkb; ++kb) {
+      const int first = T.k0 + kb * 128, end = min(first + 128, P.k);
+      float sum = 0.f;
+      for (int k = first; k < end; k += 16) {
+        const uint4 va = *(const uint4*)(a + k), vb = *(const uint4*)(b + k);
+        const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+          const float2 x = fp8_pair(wa[q >> 1] >> (16 * (q & 1)) & 0xffffu, P.a_e5);
+          const float2 y = fp8_pair(wb[q >> 1] >> (16 * (q & 1)) & 0xffffu, P.b_e5);
+          if (k + 2 * q < end) sum = fmaf(x.x, y.x, sum);
+          if (k + 2 * q + 1 < end) sum = fmaf(x.y, y.y, sum);
+        }
+      }
+      const int64_t at = T.k0 / 128 + kb;
+      total = far_add<A_ROW>(total, sum, sa[at * P.sa_k], sb[at * P.sb_k]);
+    }
+    const int64_t o = (P.mode == 1 ? (int64_t)T.seg * P.o_g : 0) + (int64_t)(col0 + c) * P.o_ld + row0 + r;
+    if (P.out_f32) ((float*)P.out)[o] = total;
+    else ((__nv_bfloat16*)P.out)[o] = __float2bfloat16_rn(total);
+  }
+}
+
 template <bool FP8, bool A_ROW, bool PAIR, int SLICES, int COLS, bool MX = false>
 __global__ void __launch_bounds__(gg_threads(SLICES), 1)
 grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmAt, const __grid_constant__ CUtensorMap tmBt,
-                    GGParams P) {
+                    const __grid_constant__ GGParams P) {
   static_assert(!MX || (FP8 && PAIR && SLICES * COLS > 128), "scales on the tensor core: wide fp8 tiles");
   constexpr bool SUMS = FP8 && !MX;  // the epilogue scales and adds every 128-block
   constexpr int KS = MX ? 2 : gg_slabs(FP8, SLICES * COLS);
   constexpr int SLOTS = MX ? GG_MX_SLOTS : GG_SLOTS;
+  constexpr bool SHARES = SLICES * COLS <= 128;  // a contraction may be shared (P.split)
   // Wide fp8 tiles keep every warp busy with the sums, so their results leave
   // through the TMA unit: written to shared memory (4 KB a warp) and stored from
   // there under the next tile. Stored by the warps themselves they cost 65 us of
@@ -395,6 +541,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   __shared__ __align__(8) uint64_t sfull_bar[SLOTS];       // a batch of scales; one per CTA
   __shared__ __align__(8) uint64_t sempty_bar[SLOTS];
   __shared__ __align__(8) uint64_t raw_bar[MX ? 2 * GG_MX_AHEAD : 1];  // MX: f32 scales, by warp
+  __shared__ int far_flag;  // some tile has far scales
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   __shared__ int nseg_s;
@@ -426,6 +573,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
     if constexpr (MX)
       for (int s = 0; s < 2 * GG_MX_AHEAD; ++s) mbar_init(&raw_bar[s], 1);
+    far_flag = 0;
     abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -759,9 +907,26 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         if (!convert()) fail = 4;
       if (fail) give_up(4);
     }
+    // A look at the range of a tile's scales, for which nothing waits. Wide tiles: by
+    // warp 3 (by warp 2 a prompt of 2047 took 2 % longer). Narrow ones: by warp 2 once
+    // the tile's scales are on their way (by warp 3 a token took 1.0 us longer, for the
+    // instructions it fetched beside the first tile's; so 0.4 us of 12). Read from the
+    // slots, or scale by scale, it took longer than the products.
+    auto look = [&](const TileAt& T, int kb0, int kb1) {
+      const int row0 = T.r0 + (int)rank * 128;
+      bool may = far_marks<A_ROW>(P, S, T, kb0, kb1, row0, lane);
+      if constexpr (!A_ROW) may |= far_blocks(P, T, kb0, kb1, row0, lane);
+      if (!__any_sync(0xffffffffu, may)) return false;
+      return far_scales<A_ROW>(P, T, kb0, kb1, row0, lane);
+    };
+    auto tell = [&]() {  // the CTA that stores the tile
+      if (lane == 0) st_cluster_u32(map_to_cta(smem_u32(&far_flag), P.split > 1 ? rank : crank), 1u);
+    };
+    bool arrived = false;  // at the barrier ahead of the sum of a shared contraction
     if (SUMS && warp == 2) {
       int slot = 0, cur = 0;
       uint32_t phase = 0;
+      bool far = false;
       for (int tile = cluster_id; tile < total && !fail; tile += num_clusters) {
         const TileAt T = gg_tile<FP8, PAIR>(P, S, nseg, tile, cur);
         const int kb0 = share_of(T.nkb, part, P.split), kb1 = share_of(T.nkb, part + 1, P.split);
@@ -792,12 +957,31 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                        : "memory");
           if (++slot == SLOTS) { slot = 0; phase ^= 1; }
         }
+        if (fail) break;
+        if (SHARES && P.split > 1) {
+          cluster_arrive();
+          arrived = true;
+        }
+        if (SHARES && !far) far = look(T, kb0, kb1);
       }
+      if (far) tell();
       if (fail) give_up(4);
       asm volatile("cp.async.wait_all;" ::: "memory");
     }
+    if (SUMS && !SHARES && warp == 3) {
+      bool far = false;
+      int cur = 0;
+      for (int tile = cluster_id; tile < total && !far; tile += num_clusters) {
+        const TileAt T = gg_tile<FP8, PAIR>(P, S, nseg, tile, cur);
+        far = look(T, 0, T.nkb);
+      }
+      if (far) tell();
+    }
     __syncwarp();
-    if (P.split > 1) cluster_sync_all();
+    if (P.split > 1) {
+      if (!arrived) cluster_arrive();
+      cluster_wait();
+    }
   }
   } else {
     // ---------------- epilogue (every CTA, its own 128 rows) ----------------
@@ -1020,10 +1204,10 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
       }
       if (fail) break;
-      if (P.split == 1) store(tile);
+      if (!SHARES || P.split == 1) store(tile);
     }
     if (fail) give_up(3);
-    if (P.split > 1) {
+    if (SHARES && P.split > 1) {
       // Parts of one tile: parts 1.. leave their sums in their own shared memory
       // (the operand ring is idle by now), part 0 adds them in part order.
       float4* mine = (float4*)smem + (warp - 4) * (GROUPS * 2 * 32) + lane;
@@ -1067,6 +1251,15 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   tc_fence_before();
   __syncthreads();
   if (PAIR || P.split > 1) cluster_sync_all();
+  if constexpr (SUMS) {
+    if (warp >= 4 && part == 0 && *(volatile int*)&far_flag && !*abortp) {
+      if (TMA_OUT && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      __syncwarp();  // behind every lane's stores
+      for (int tile = cluster_id; tile < total; tile += num_clusters)
+        far_tile<A_ROW, PAIR>(P, S, nseg, tile, (int)rank * 128 + (warp & 3) * 32, ((warp - 4) >> 2) * COLS, COLS,
+                              lane);
+    }
+  }
   if (warp == 1) {
     tc_fence_after();
     if constexpr (PAIR)
@@ -1392,6 +1585,13 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   P.a_scale = d->a_scale; P.sa_g = d->a_scale_group_stride; P.sa_k = d->a_scale_k_stride;
   P.sa_r = d->a_scale_r_stride;
   P.b_scale = d->b_scale; P.sb_k = d->b_scale_k_stride;
+  P.far = (const uint64_t*)(a_row ? d->a_far : d->b_far);
+  P.far_k = a_row ? d->a_far_k_stride : d->b_far_k_stride;
+  P.far_t = a_row ? d->a_far_r_stride : d->b_far_t_stride;
+  P.far_padded = P.mode == 0 && grouped && d->b_far_padded;
+  P.a = (const uint8_t*)d->a; P.a_ld = d->a_ld; P.a_g = d->a_group_stride;
+  P.b = (const uint8_t*)d->b; P.b_ld = d->b_ld;
+  P.k = (int)k; P.a_e5 = d->a_dtype == AQTB200_E5M2; P.b_e5 = d->b_dtype == AQTB200_E5M2;
   P.out = d->out; P.out_f32 = d->out_dtype == AQTB200_F32;
   P.o_ld = d->out_ld; P.o_g = d->out_group_stride;
   P.out_staged = !P.out_f32 && ((uintptr_t)d->out & 15) == 0 && d->out_ld % 8 == 0 &&

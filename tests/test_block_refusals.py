@@ -273,3 +273,13 @@ def test_forward_mode_tangents(monkeypatch):
         call()
         pytest.fail(f'call {i} was not refused')
     cfg(x, w[0], DIMS)  # a level without tangents of its operands
+
+
+def test_abi_marks(lib):
+  """Marks are of one matrix with 1 x 128 blocks, eight bytes each."""
+  call = lambda d: lib.aqtb200_block_quantize(C.byref(d), None)
+  assert call(_quant_desc(far_row=260)) == -2
+  assert call(_quant_desc(far_row=256, square=1)) == -2
+  d = _quant_desc(far_row=256)
+  d.x.b0 = 2
+  assert call(d) == -2

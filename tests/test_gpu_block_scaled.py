@@ -426,3 +426,101 @@ def test_products_back_to_back(m, k, n, po2):
   _done()
   for i, j, out in got:
     assert torch.equal(out, alone[i, j]), (i, j)
+
+
+# Exponents of the operands' magnitudes: the block scales' product (about 2^17.6
+# less) lies below f32's normal numbers, at zero or above its range, or one scale
+# alone takes a block's sum out of it, where the results do not.
+EXPONENTS = [(-60, -62), (-70, -66), (-100, 20), (100, -60), (-60, 100), (-108, 90),
+             (110, -100), (-45, -97)]
+
+
+def _far(shape, dtype, seed, exponent):
+  """Values whose blocks' maxima are all the same size, times 2^exponent; the
+  rounding to 8 bits is then the same for every exponent but for the scale."""
+  rng = np.random.default_rng(seed)
+  x = rng.integers(-15, 16, shape).astype(np.float64)
+  x = np.ldexp(x + (x == 0), exponent)
+  return torch.from_numpy(x.astype(np.float32)).to(dtype).cuda()
+
+
+@pytest.mark.parametrize('m,k,n', [(3, 640, 70), (200, 300, 129),
+                                   (2048, 384, 2560)])
+@pytest.mark.parametrize('a,b', EXPONENTS)
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('rhs_axis', [0, 1])
+def test_scales_whose_product_leaves_the_range(m, k, n, a, b, dtype, rhs_axis):
+  x, w, g = (_far((m, k), dtype, 70, a), _far((k, n), dtype, 71, b),
+             _far((m, n), dtype, 72, -a // 2))
+  v = w.t().contiguous() if rhs_axis else w
+  out, bp = bs.dot_general_make('e4m3', 'e4m3').vjp(x, v, (((1,), (rhs_axis,)),
+                                                           ((), ())))
+  dl, dr = bp(g)
+  _done()
+  dr = dr.t() if rhs_axis else dr
+  for name, got, (want, mag, kk) in zip(
+      ('out', 'dlhs', 'drhs'), (out, dl, dr),
+      _want(_f32(x), _f32(w), _f32(g), False, 'e4m3', 'e4m3')):
+    _check_in_range(got, want, mag, kk, HALF[dtype], name)
+
+
+def _check_in_range(got, want, mag, k, half, name):
+  """What f32 holds on the way is right; what it cannot hold is not finite. (Sums
+  between the two may overflow in one order and not in another, and two partial
+  sums of either sign past the range add up to a NaN.)"""
+  got = _f32(got).astype(np.float64)
+  held = mag < 2.0 ** 127
+  ref.assert_close(got[held], want[held], mag[held], k, half, name)
+  past = np.abs(want) - (k + 3) * 2.0 ** -22 * mag >= 2.0 ** 128
+  assert not np.isfinite(got[past]).any(), name
+
+
+@pytest.mark.parametrize('m,n', [(3, 70), (2048, 2560)])
+@pytest.mark.parametrize('e', [60, 72, 100])
+def test_large_scales_on_operands_that_hardly_meet(m, n, e):
+  """Each operand's large values meet the other's zeros, its small ones each
+  other: the scales' product is past f32's range, the results are not."""
+  k = 256
+  x = torch.zeros(m, k, device='cuda')
+  w = torch.zeros(k, n, device='cuda')
+  x[:, 0::8], w[1::8, :] = 2.0 ** e, 2.0 ** e      # scales near 2^(e - 8.8)
+  x[:, 2::16] = 2.0 ** (e - 15)                    # 2^-6 in units of a scale
+  w[2::16, ::3] = 2.0 ** (e - 15)
+  qt = bs.block_quantize(w, 0, square=True)
+  (want, mag, kk), = _want(_f32(x), _f32(w), None)
+  cfg = bs.dot_general_make()
+  for q in (w, qt):
+    out = cfg(x, q, DIMS)
+    _done()
+    got = _f32(out)
+    assert not got[:, 1::3].any() and not got[:, 2::3].any()
+    _check_in_range(out, want, mag, kk, 2.0 ** -24, '')
+
+
+def test_far_scales_leave_other_rows_alone():
+  """Rows that need the careful products change no bit of the others."""
+  x, w = _data((300, 384), torch.bfloat16, 73, 1.0), _data((384, 200),
+                                                         torch.bfloat16, 74, 0.3)
+  cfg = bs.dot_general_make()
+  w[:128] *= 2.0 ** -60
+  out, bp = cfg.vjp(x, w, DIMS)
+  g = _data((300, 200), torch.bfloat16, 75, 1.0)
+  dl, dr = bp(g)
+  x2, g2 = x.clone(), g.clone()
+  x2[7] *= 2.0 ** -75
+  g2[9] *= 2.0 ** -90
+  g2[:, 5] *= 2.0 ** -110
+  x2[:, 3] *= 2.0 ** 60
+  rest = [i for i in range(300) if i not in (7, 9)]
+  out2 = cfg.vjp(x2, w, DIMS)[0]
+  x3 = x.clone()
+  x3[7] *= 2.0 ** -75
+  assert torch.equal(cfg.vjp(x3, w, DIMS)[0][rest], out[rest])
+  assert torch.isfinite(out2.float()).all()
+  dr3 = cfg.vjp(x, w, DIMS)[1](g)[1]
+  g3 = g.clone()
+  g3[:, 5] *= 2.0 ** -110
+  dr4 = cfg.vjp(x, w, DIMS)[1](g3)[1]
+  _done()
+  cols = [i for i in range(200) if i != 5]
+  assert torch.equal(dr3, dr) and torch.equal(dr4[:, cols], dr[:, cols])

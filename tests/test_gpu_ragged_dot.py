@@ -508,3 +508,73 @@ def test_checkpointed_and_offloaded(q, k):
     _done()
     for s, t in zip(got, want):
       assert torch.equal(s, t)
+
+
+@pytest.mark.parametrize('m,k,n,sizes', [
+    (60, 640, 72, [10, 0, 7, 20, 3]),
+    (700, 300, 264, [257, 130, 1, 0, 300]),
+    (5000, 384, 1800, [700, 2000, 0, 129, 2100])])
+@pytest.mark.parametrize('out', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('frozen', [False, True])
+def test_scales_whose_product_leaves_the_range(m, k, n, sizes, out, frozen):
+  """Each expert has a magnitude of its own, and so have its rows: some products of
+  two block scales are below f32's normal numbers, some above all of them."""
+  rng = np.random.default_rng(90)
+
+  def values(shape, exponents):  # one exponent for each of the first axis
+    v = rng.integers(-15, 16, shape).astype(np.float64)
+    v = np.ldexp(v + (v == 0), np.asarray(exponents).reshape(-1, *[1] * (v.ndim - 1)))
+    return torch.from_numpy(v.astype(np.float32)).cuda()
+
+  rows, cots = np.zeros(m, int), np.zeros(m, int)
+  of_x, of_w, of_g = (-70, 30, -20, 0, 100), (-64, 5, 60, 0, -95), (-66, 20, -120, 0, 60)
+  for e, (a, b) in enumerate(ref.spans(sizes, m)):
+    rows[a:b], cots[a:b] = of_x[e], of_g[e]
+  rows[::9] += 3
+  x, w, g = values((m, k), rows), values((len(sizes), k, n), of_w), values((m, n), cots)
+  cfg = bs.dot_general_make('e4m3', 'e4m3')
+  want = _want(_f32(x), _f32(w), _f32(g), sizes, True, False, 'e4m3', 'e4m3')
+  if frozen:
+    y = rd.ragged_dot(x, bs.block_quantize(w, 1, square=True), _sizes(sizes), cfg=cfg,
+                      preferred_element_type=out)
+    got, want = (y,), want[:1]
+  else:
+    y, bp = rd.ragged_dot_vjp(x, w, _sizes(sizes), cfg=cfg, preferred_element_type=out)
+    got = (y, *bp(g))
+  _done()
+  for name, t, (value, mag, kk) in zip(('out', 'dlhs', 'drhs'), got, want):
+    t, half = _f32(t).astype(np.float64), HALF[t.dtype]
+    held = mag < 2.0 ** 127  # the others pass f32's range, in sum or on the way
+    ref.assert_close(t[held], value[held], mag[held], kk, half, name)
+    past = np.abs(value) - (kk + 3) * 2.0 ** -22 * mag >= 2.0 ** 128
+    assert not np.isfinite(t[past]).any(), name
+
+
+@pytest.mark.parametrize('sizes', [[5, 0, 11], [300, 129, 200]])
+def test_far_scales_leave_other_groups_alone(sizes):
+  """What a far group or row needs changes no bit of the others."""
+  m = sum(sizes)
+  x, w, g = (_data((m, 384), torch.bfloat16, 91), _data(
+      (3, 384, 200), torch.bfloat16, 92, 0.1), _data((m, 200), torch.bfloat16, 93))
+  w[0] *= 2.0 ** -60
+  cfg = bs.dot_general_make()
+
+  def step(x, g):
+    out, bp = rd.ragged_dot_vjp(x, w, _sizes(sizes), cfg=cfg)
+    return (out, *bp(g))
+
+  out, dl, dr = step(x, g)
+  x2, g2 = x.clone(), g.clone()
+  x2[2] *= 2.0 ** -75
+  g2[3] *= 2.0 ** -90
+  out2, dl2, _ = step(x2, g2)
+  rest = [i for i in range(m) if i not in (2, 3)]
+  assert torch.equal(out[rest], out2[rest]) and torch.equal(dl[rest], dl2[rest])
+  assert torch.equal(out[3], out2[3]) and torch.equal(dl[2], dl2[2])
+  g3 = g.clone()
+  g3[:sizes[0], 7] *= 2.0 ** -110
+  _, _, dr3 = step(x, g3)
+  _done()
+  cols = [i for i in range(200) if i != 7]
+  assert torch.equal(dr[0][:, cols], dr3[0][:, cols])
+  assert torch.equal(dr[1:], dr3[1:])
