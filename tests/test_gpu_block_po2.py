@@ -257,3 +257,29 @@ def test_captured_and_replayed():
     graph.replay()
     _done()
     _check_step(x, w, g, got)
+
+
+@pytest.mark.parametrize('a,b', [(-60, -62), (-70, -66), (100, -60), (-60, 100),
+                                 (-108, 90), (110, -100), (-45, -97), (60, 40)])
+@pytest.mark.parametrize('m,k,n', [(2048, 384, 2560), (200, 300, 129)])
+def test_far_exponents(m, k, n, a, b):
+  """Scales whose product f32 does not hold, results that it does."""
+  rng = np.random.default_rng(76)
+
+  def values(shape, e):
+    v = rng.integers(-15, 16, shape).astype(np.float64)
+    return torch.from_numpy(np.ldexp(v + (v == 0), e).astype(np.float32)).to(
+        torch.bfloat16).cuda()
+
+  x, w, g = values((m, k), a), values((k, n), b), values((m, n), -a // 2)
+  out, bp = bs.dot_general_make('e4m3', 'e4m3', po2_scale=True).vjp(x, w, DIMS)
+  got = (out, *bp(g))
+  _done()
+  f = lambda t, br, bc: ref.fake(t.float().cpu().numpy(), br, bc, 'e4m3', True)
+  w_ = f(w, 128, 128)
+  for name, t, (p, q) in zip(('out', 'dlhs', 'drhs'), got, (
+      (f(x, 1, 128), w_), (f(g, 1, 128), w_.T), (f(x, 128, 1).T, f(g, 128, 1)))):
+    want, mag = p @ q, np.abs(p) @ np.abs(q)
+    held = mag < 2.0 ** 127  # the others pass f32's range, in sum or on the way
+    t = t.float().cpu().numpy().astype(np.float64)
+    ref.assert_close(t[held], want[held], mag[held], p.shape[1], 2.0 ** -8, name)
