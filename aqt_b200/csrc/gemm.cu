@@ -1722,7 +1722,8 @@ struct ExchangeArgs {
 
 static int g_gemm_impl = 0;
 static int g_sm_budget = 0;
-static int gemm_sms() {
+// SMs a persistent GEMM grid may take.
+int gemm_sms() {
   int n = sm_count();
   return (g_sm_budget > 0 && g_sm_budget < n) ? g_sm_budget : n;
 }

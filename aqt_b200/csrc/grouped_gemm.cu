@@ -45,6 +45,7 @@
 namespace aqtb200 {
 
 int sm_count();
+int gemm_sms();
 
 // Epilogue warps: SLICES for each TMEM lane quarter, COLS columns each; a tile is
 // up to SLICES * COLS columns wide. Four more warps carry the other roles.
@@ -1535,7 +1536,7 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   const bool po2 = fp8 && d->scales_po2 && d->out_dtype == AQTB200_BF16 && P.num_kb * 4 <= 1 << 13 &&
                    (d->a_scale_square || d->a_scale_r_stride == 1);
   const auto ctas_of = [&](int nt) { return !fp8 || (nt <= 128 ? GG_PAIR_NARROW : GG_PAIR_WIDE) ? 2 : 1; };
-  const auto units_of = [&](int nt) { return std::max(1, sm_count() / ctas_of(nt)); };
+  const auto units_of = [&](int nt) { return std::max(1, gemm_sms() / ctas_of(nt)); };
   // Tiles, or the most there can be: groups that end inside a tile add one each.
   const auto tiles_of = [&](int nt) {
     const int64_t per = (d->t + nt - 1) / nt, rows = 128 * ctas_of(nt);

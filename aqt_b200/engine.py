@@ -203,7 +203,8 @@ def set_gemm_impl(name: str):
 
 
 def set_gemm_sm_budget(max_sms: int):
-  """Caps the SMs the persistent GEMM grids take (0 = all)."""
+  """Caps the SMs the persistent GEMM grids take (0 = all), those of block-scaled
+  and grouped products among them."""
   _lib.check(_call(_lib.load().aqtb200_set_gemm_sm_budget, int(max_sms)),
              'set_gemm_sm_budget')
 

@@ -501,7 +501,8 @@ int64_t aqtb200_kernel_launch_count(void);
  * single CTAs; 3 = always 256 x 256 CTA pairs; 4 = always 256 x 512 CTA
  * pairs. */
 int aqtb200_set_gemm_impl(int impl);
-/* Caps the number of SMs the persistent GEMM kernels occupy (0 = all of them).
+/* Caps the number of SMs the persistent GEMM kernels occupy (0 = all of them;
+ * aqtb200_grouped_gemm: one CTA pair at least; quantizers are not capped).
  * A caller that runs a collective concurrently with a GEMM leaves it room
  * this way: a persistent grid that fills every SM would otherwise make the
  * collective's kernel (or the GEMM's last CTAs) wait for a free SM. */

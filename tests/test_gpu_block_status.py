@@ -59,3 +59,42 @@ def test_first_call_under_capture():
   with pytest.raises(_lib.AqtB200Error, match='role 4'):
     rd.ragged_dot(x, w, sizes)
   engine.check_status()
+
+
+@pytest.mark.parametrize('kind', ['bf16', 'fp8', 'po2', 'decode'])
+def test_the_sm_budget_caps_these_products_too(kind):
+  """A caller that keeps SMs free for a collective beside the products."""
+  m = 16 if kind == 'decode' else 2048
+  x, w = _data((m, 2048), 5), _data((2048, 8192), 6)
+  if kind == 'bf16':
+    sizes = torch.tensor([m], device='cuda')
+    run = lambda: rd.ragged_dot(x, w[None], sizes)
+  else:
+    cfg = bs.dot_general_make(po2_scale=kind == 'po2')
+    w = bs.block_quantize(w, 0, square=True) if kind == 'decode' else w
+    run = lambda: cfg(x, w, DIMS)
+
+  def products():
+    """Results, and microseconds of the product kernels alone."""
+    out = run()
+    torch.cuda.synchronize()
+    with torch.profiler.profile(
+        activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+      for _ in range(3):
+        run()
+      torch.cuda.synchronize()
+    return out, min(e.device_time_total for e in prof.events()
+                    if 'grouped_gemm' in e.name)
+
+  out, free = products()
+  engine.set_gemm_sm_budget(8)
+  try:
+    capped, slow = products()
+  finally:
+    engine.set_gemm_sm_budget(0)
+  engine.check_status()
+  # 8 of 148 SMs: 18 times the work an SM; a decode stops at the memory's rate and
+  # loses less
+  assert slow > (2 if kind == 'decode' else 4) * free
+  assert torch.allclose(out.float(), capped.float(), rtol=2.0 ** -7,
+                        atol=float(out.abs().max()) * 2.0 ** -8)
