@@ -1680,11 +1680,11 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   cfg.numAttrs = fp8 && P.mode == 0 && k > 0 && d->follows_quantize ? 2 : 1;
 #define AQT_GG(...)                                                                                \
   do {                                                                                             \
-    static bool attr_done[64] = {false};                                                           \
-    if (!attr_done[dev & 63]) {                                                                    \
+    static std::atomic<bool> attr_done[64]; /* calls come from several threads */                  \
+    if (!attr_done[dev & 63].load(std::memory_order_acquire)) {                                    \
       AQT_CUDA_OK(cudaFuncSetAttribute(grouped_gemm_kernel<__VA_ARGS__>,                           \
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); \
-      attr_done[dev & 63] = true;                                                                  \
+      attr_done[dev & 63].store(true, std::memory_order_release);                                  \
     }                                                                                              \
     AQT_CUDA_OK(cudaLaunchKernelEx(&cfg, grouped_gemm_kernel<__VA_ARGS__>, tmA, tmB, tmAt, tmBt, P)); \
   } while (0)

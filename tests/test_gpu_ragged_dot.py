@@ -578,3 +578,36 @@ def test_far_scales_leave_other_groups_alone(sizes):
   cols = [i for i in range(200) if i != 7]
   assert torch.equal(dr[0][:, cols], dr3[0][:, cols])
   assert torch.equal(dr[1:], dr3[1:])
+
+
+def test_first_calls_of_many_threads_at_once():
+  """Every kind of product, each from four threads on streams of their own."""
+  import threading
+  x, w, g = (_data((300, 200), torch.bfloat16, 94), _data(
+      (3, 200, 136), torch.bfloat16, 95, 0.1), _data((300, 136), torch.bfloat16, 96))
+  sizes = _sizes([150, 20, 100])
+  kinds = (None, bs.dot_general_make(), bs.dot_general_make(po2_scale=True))
+
+  def run(cfg):
+    out, bp = rd.ragged_dot_vjp(x, w, sizes, cfg=cfg)
+    return (out, *bp(g))
+
+  want = [run(cfg) for cfg in kinds]
+  _done()
+  got, start = {}, threading.Barrier(12)
+
+  def work(i):
+    stream = torch.cuda.Stream()
+    start.wait()
+    with torch.cuda.stream(stream):
+      got[i] = run(kinds[i % 3])
+    stream.synchronize()
+
+  threads = [threading.Thread(target=work, args=(i,)) for i in range(12)]
+  for t in threads:
+    t.start()
+  for t in threads:
+    t.join()
+  _done()
+  for i in range(12):
+    assert all(torch.equal(a, b) for a, b in zip(got[i], want[i % 3])), i
