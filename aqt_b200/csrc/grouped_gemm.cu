@@ -1498,6 +1498,9 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   const bool grouped = d->group_sizes != nullptr;
   AQT_REQUIRE(!grouped || (d->groups >= 1 && d->groups <= AQTB200_MAX_GROUPS), AQTB200_EUNSUPPORTED,
               "between 1 and %d groups (got %lld)", AQTB200_MAX_GROUPS, (long long)d->groups);
+  // such a copy's first column is a group's first row, and has to be a multiple of eight
+  AQT_REQUIRE(!(grouped && d->contract_groups == 0 && d->b_mn_major), AQTB200_EUNSUPPORTED,
+              "grouped rows of b are contiguous along k");
   const int64_t groups = grouped ? d->groups : 1;
   if (grouped && d->contract_groups == 1)
     // the groups' positions are worked out from the sizes and `rows` alone

@@ -634,7 +634,8 @@ int aqtb200_block_quantize(const aqtb200_block_quant_desc* desc, void* stream);
  *             aqtb200_block_quantize).
  * a, b      : element (r, k) of group g at g*a_group_stride + r*a_ld + k, or
  *             with a_mn_major at g*a_group_stride + k*a_ld + r (bf16 only; b
- *             alike). 16-byte aligned, strides multiples of 16 bytes.
+ *             alike, but not with groups and contract_groups 0). 16-byte aligned,
+ *             strides multiples of 16 bytes.
  * a_scale   : fp8 only. f32 of (r, block kb) at g*a_scale_group_stride +
  *             kb*a_scale_k_stride + (a_scale_square ? r/128 : r)*a_scale_r_stride.
  * b_scale   : f32 of (t, kb) at kb*b_scale_k_stride + t.

@@ -275,6 +275,14 @@ def test_forward_mode_tangents(monkeypatch):
     cfg(x, w[0], DIMS)  # a level without tangents of its operands
 
 
+def test_abi_gemm_columns_of_groups(lib):
+  """With b's columns contiguous a group's tiles would start at any column, where
+  no tiled copy may: refused before anything is launched."""
+  call = lambda d: lib.aqtb200_grouped_gemm(C.byref(d), None, None)
+  assert call(_gemm_desc(b_mn_major=1, b_ld=8, group_sizes=256, groups=2,
+                         a_group_stride=4096)) == -2
+
+
 def test_abi_marks(lib):
   """Marks are of one matrix with 1 x 128 blocks, eight bytes each."""
   call = lambda d: lib.aqtb200_block_quantize(C.byref(d), None)
