@@ -989,6 +989,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     if constexpr (SLICES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     else if constexpr (SUMS) asm volatile("setmaxnreg.inc.sync.aligned.u32 112;");
     else asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    // rows behind the last group are zeros that wait for no operand: nothing is stored
+    // before what was put on the stream last has ended, be it torch filling the result
+    if constexpr (FP8) grid_wait();
     // A warp reads its 32 rows by COLS columns with 16x256b loads: a thread then
     // holds, of every 8 columns, two neighbouring ones in four rows,
     //   acc[g][h][i]: column 8 g + 2 (lane % 4) + i % 2, row 16 h + lane / 4 + 8 (i / 2),

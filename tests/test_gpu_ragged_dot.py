@@ -611,3 +611,23 @@ def test_first_calls_of_many_threads_at_once():
   _done()
   for i in range(12):
     assert all(torch.equal(a, b) for a, b in zip(got[i], want[i % 3])), i
+
+
+def test_results_that_torch_fills_first():
+  """Deterministic algorithms: torch fills every new tensor with NaN, between the
+  quantizer and the product that is launched beside it."""
+  x, w = _data((400, 384), torch.bfloat16, 97), _data((4, 384, 200), torch.bfloat16, 98,
+                                                      0.1)
+  qt = bs.block_quantize(w, 1, square=True)
+  cfg = bs.dot_general_make()
+  sizes = _sizes([20, 0, 30, 5])  # most rows lie behind the last group
+  want = rd.ragged_dot(x, qt, sizes, cfg=cfg)
+  _done()
+  torch.use_deterministic_algorithms(True)
+  try:
+    got = [rd.ragged_dot(x, qt, sizes, cfg=cfg) for _ in range(50)]
+  finally:
+    torch.use_deterministic_algorithms(False)
+  _done()
+  assert not want[55:].any()
+  assert all(torch.equal(t, want) for t in got)
