@@ -392,8 +392,7 @@ __device__ __forceinline__ int share_of(int nkb, int part, int split) {
 //   row scales       the sum times the row's scale, where that lies in ROW_MIN .. ROW_MAX
 // Elements with a block of other scales are computed again, by far_tile, when all is
 // stored. (Nothing of this is in the epilogue's loop or between its tiles: choosing
-// slab by slab cost 2 to 5 %, a verdict on each tile 1 to 2 %, and a look at the scales
-// ahead of their use up to 20 % of a decode.)
+// slab by slab cost 2 to 5 %, and a verdict on each tile 1 to 2 %.)
 constexpr float GG_MIN_NORMAL = 0x1p-126f;
 constexpr float GG_ROW_MIN = 0x1p-94f, GG_ROW_MAX = 0x1p89f;
 template <bool A_ROW>
@@ -427,33 +426,55 @@ __device__ __forceinline__ const float* tile_a_scale(const GGParams& P, const Ti
   return P.a_scale + (P.mode == 0 ? (int64_t)T.seg * P.sa_g : 0) + (int64_t)(T.k0 / 128) * P.sa_k +
          (int64_t)row * P.sa_r;
 }
-__device__ __forceinline__ bool far_blocks(const GGParams& P, const TileAt& T, int kb0, int kb1, int row0,
-                                           int lane) {
-  const float* sa = tile_a_scale(P, T, min(row0, P.r - 1) >> 7);
-  bool may = false;
-  for (int kb = kb0 + lane; kb < kb1; kb += 32) may |= may_be_far(sa[kb * P.sa_k]);
-  return may;
-}
+// In two steps, so that the reads of the first 32 slabs are on their way meanwhile.
 template <bool A_ROW>
-__device__ __forceinline__ bool far_marks(const GGParams& P, const Segments& S, const TileAt& T, int kb0,
-                                          int kb1, int row0, int lane) {
-  if (P.far == nullptr) return false;
-  int first = min(row0, P.r - 1) / 128, last = first;  // blocks of 128 with a mark each
-  if constexpr (!A_ROW) {
-    int t = T.t0, before = 0;
-    if (P.far_padded) {
-      t -= S.off[T.seg];
-      for (int g = lane; g < T.seg; g += 32) before += (S.off[g + 1] - S.off[g] + 127) / 128;
-      before = __reduce_add_sync(0xffffffffu, before);
+struct FarLook {
+  const float* a;      // scales of the weights' blocks
+  const uint64_t* m0;  // marks of the first and the last block of 128
+  const uint64_t* m1;
+  float a_first;
+  uint64_t m0_first, m1_first;
+
+  __device__ __forceinline__ void begin(const GGParams& P, const Segments& S, const TileAt& T, int kb0, int kb1,
+                                        int row0, int lane) {
+    row0 = min(row0, P.r - 1);
+    a = tile_a_scale(P, T, row0 >> 7);
+    int first = row0 >> 7, last = first;
+    if constexpr (!A_ROW) {
+      int t = T.t0, before = 0;
+      if (P.far_padded) {
+        t -= S.off[T.seg];
+        for (int g = lane; g < T.seg; g += 32) before += (S.off[g + 1] - S.off[g] + 127) >> 7;
+        before = __reduce_add_sync(0xffffffffu, before);
+      }
+      first = before + (t >> 7);
+      last = before + ((t + T.tvalid - 1) >> 7);
     }
-    first = before + t / 128;
-    last = before + (t + T.tvalid - 1) / 128;
+    m0 = P.far + (int64_t)(T.k0 >> 7) * P.far_k + first * P.far_t;
+    m1 = m0 + (last - first) * P.far_t;
+    a_first = 0.f;
+    m0_first = m1_first = 0;
+    const int kb = kb0 + lane;
+    if (kb < kb1) {
+      if constexpr (!A_ROW) a_first = a[kb * P.sa_k];
+      if (P.far != nullptr) {
+        m0_first = m0[kb * P.far_k];
+        if constexpr (!A_ROW) m1_first = m1[kb * P.far_k];
+      }
+    }
   }
-  bool may = false;
-  for (int x = first; x <= last; ++x)
-    for (int kb = kb0 + lane; kb < kb1; kb += 32) may |= P.far[(T.k0 / 128 + kb) * P.far_k + x * P.far_t] != 0;
-  return may;
-}
+  __device__ __forceinline__ bool finish(const GGParams& P, int kb0, int kb1, int lane) const {
+    bool may = may_be_far(a_first) || (m0_first | m1_first) != 0;
+    for (int kb = kb0 + 32 + lane; kb < kb1; kb += 32) {
+      if constexpr (!A_ROW) may |= may_be_far(a[kb * P.sa_k]);
+      if (P.far != nullptr) {
+        may |= m0[kb * P.far_k] != 0;
+        if constexpr (!A_ROW) may |= m1[kb * P.far_k] != 0;
+      }
+    }
+    return __any_sync(0xffffffffu, may);
+  }
+};
 // Whether one is: every pair is tried.
 template <bool A_ROW>
 __device__ __forceinline__ bool far_scales(const GGParams& P, const TileAt& T, int kb0, int kb1, int row0,
@@ -913,13 +934,12 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     // the tile's scales are on their way (by warp 3 a token took 1.0 us longer, for the
     // instructions it fetched beside the first tile's; so 0.4 us of 12). Read from the
     // slots, or scale by scale, it took longer than the products.
-    auto look = [&](const TileAt& T, int kb0, int kb1) {
-      const int row0 = T.r0 + (int)rank * 128;
-      bool may = far_marks<A_ROW>(P, S, T, kb0, kb1, row0, lane);
-      if constexpr (!A_ROW) may |= far_blocks(P, T, kb0, kb1, row0, lane);
-      if (!__any_sync(0xffffffffu, may)) return false;
-      return far_scales<A_ROW>(P, T, kb0, kb1, row0, lane);
-    };
+    // The range of a tile's scales is looked at beside the products; nothing but the
+    // kernel's end waits for it. Wide tiles: by warp 3 (by warp 2 a prompt of 2047 x 4096
+    // x 14336 took 2 % longer). Narrow ones: by warp 2, around the copies of the tile's
+    // scales: one token of 4096 x 4096 takes 12.4 us with its quantizer, 12.1 without the
+    // look, 13.1 with warp 3 doing it, for the instructions it fetches beside the first
+    // tile's. Read from the slots, or scale by scale, it took longer than the products.
     auto tell = [&]() {  // the CTA that stores the tile
       if (lane == 0) st_cluster_u32(map_to_cta(smem_u32(&far_flag), P.split > 1 ? rank : crank), 1u);
     };
@@ -937,6 +957,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                           (int64_t)(A_ROW ? row : row >> 7) * P.sa_r;
         const float* pb = P.b_scale + kabs * P.sb_k + T.t0;
         const int rows = A_ROW ? min(128, P.r - row) : 1;
+        FarLook<A_ROW> look;
+        if (SHARES) look.begin(P, S, T, kb0, kb1, T.r0 + (int)rank * 128, lane);
         for (int kb = kb0; kb < kb1; kb += GG_BATCH) {
           const int ok = mbar_wait(&sempty_bar[slot], phase ^ 1, abortp) ? 1 : 0;
           if (!__all_sync(0xffffffffu, ok)) { fail = 4; break; }
@@ -963,7 +985,8 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           cluster_arrive();
           arrived = true;
         }
-        if (SHARES && !far) far = look(T, kb0, kb1);
+        if (SHARES && !far && look.finish(P, kb0, kb1, lane))
+          far = far_scales<A_ROW>(P, T, kb0, kb1, T.r0 + (int)rank * 128, lane);
       }
       if (far) tell();
       if (fail) give_up(4);
@@ -974,7 +997,10 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       int cur = 0;
       for (int tile = cluster_id; tile < total && !far; tile += num_clusters) {
         const TileAt T = gg_tile<FP8, PAIR>(P, S, nseg, tile, cur);
-        far = look(T, 0, T.nkb);
+        FarLook<A_ROW> look;
+        look.begin(P, S, T, 0, T.nkb, T.r0 + (int)rank * 128, lane);
+        far = look.finish(P, 0, T.nkb, lane) &&
+              far_scales<A_ROW>(P, T, 0, T.nkb, T.r0 + (int)rank * 128, lane);
       }
       if (far) tell();
     }
