@@ -524,3 +524,37 @@ def test_far_scales_leave_other_rows_alone():
   _done()
   cols = [i for i in range(200) if i != 5]
   assert torch.equal(dr3, dr) and torch.equal(dr4[:, cols], dr[:, cols])
+
+
+def test_projection_stack_product_by_product():
+  """Each projection of a micro-step gets its own product's gradient, and those of
+  the keys and values are the definition's for the operands they got."""
+  from aqt_b200 import layer_stack
+  cfg, seen = bs.dot_general_make(), []
+
+  class Watched:
+
+    def vjp(self, x, w, dims):
+      out, bp = cfg.vjp(x, w, dims)
+      at = {'x': x.clone(), 'w': w, 'out': out.clone()}
+      seen.append(at)
+
+      def back(g):
+        at['g'] = g.clone()
+        at['dl'], at['dr'] = bp(g)
+        return at['dl'], at['dr'].clone()
+
+      return out, back
+
+  stack = layer_stack.ProjectionStack('cuda', layers=1, cfg=Watched())
+  stack.micro_step(_data((130, layer_stack.D_MODEL), torch.bfloat16, 29, 0.0))
+  _done()
+  names = [n for n, _, _ in layer_stack.PROJ]
+  assert len(seen) == len(names)
+  for name, at in zip(names, seen):
+    assert torch.equal(stack.grad[0][name], at['dr']), name
+    if name in ('wk', 'wv'):
+      for what, (want, mag, kk) in zip(('out', 'dl', 'dr'), _want(
+          _f32(at['x']), _f32(at['w']), _f32(at['g']))):
+        ref.assert_close(_f32(at[what]).astype(np.float64), want, mag, kk,
+                         2.0 ** -8, f'{name} {what}')

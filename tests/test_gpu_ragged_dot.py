@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 import torch
 
+from aqt_b200 import block_engine as be
 from aqt_b200 import engine
 from aqt_b200.v2 import aqt_ragged_dot as rd
 from aqt_b200.v2 import block_scaled as bs
@@ -631,3 +632,82 @@ def test_results_that_torch_fills_first():
   _done()
   assert not want[55:].any()
   assert all(torch.equal(t, want) for t in got)
+
+
+@pytest.mark.parametrize('index', [torch.int32, torch.int64])
+def test_matrices_of_empty_experts_are_not_read(monkeypatch, index):
+  """The packed copy's memory holds NaN before it is written, and only the matrices
+  of experts with rows are filled in."""
+  g, k, n = 40, 133, 77
+  sizes = [0] * g
+  sizes[3], sizes[17], sizes[39] = 5, 1, 2
+  x, w, ct = (_data((9, k), torch.bfloat16, 50), _data(
+      (g, k, n), torch.bfloat16, 51, 0.1), _data((9, n), torch.bfloat16, 52))
+  copies = []
+  empty = be._empty_out  # pylint: disable=protected-access
+
+  def poisoned(shape, dtype, device):
+    t = empty(shape, dtype, device)
+    if dtype == torch.bfloat16:
+      t.fill_(float('nan'))
+      if tuple(t.shape) == (g, k, 80):
+        copies.append(t)
+    return t
+
+  monkeypatch.setattr(be, '_empty_out', poisoned)
+  out, bp = rd.ragged_dot_vjp(x, w, _sizes(sizes, index))
+  dl, dr = bp(ct)
+  _done()
+  assert len(copies) == 1
+  left = torch.isnan(copies[0].float()).flatten(1).all(1)
+  assert left.tolist() == [v == 0 for v in sizes]
+  for got, wt in zip((out, dl, dr), _want(_f32(x), _f32(w), _f32(ct), sizes, False)):
+    _check(got, wt, 2.0 ** -8, '')
+
+
+@pytest.mark.parametrize('po2', [False, True])
+def test_expert_layer_in_fp8_product_by_product(po2):
+  """The layer of test_expert_layer in fp8, each product against the definition on
+  the operands and the cotangent that it got."""
+  tokens, d, f, e, top = 200, 264, 392, 6, 2
+  x = _data((tokens, d), torch.bfloat16, 83)
+  router = _data((d, e), torch.float32, 84, 0.2)
+  ws = [_data((e, d, f), torch.bfloat16, 85, 0.1), _data(
+      (e, d, f), torch.bfloat16, 86, 0.1), _data((e, f, d), torch.bfloat16, 87, 0.1)]
+  p, chosen = torch.softmax(x.float() @ router, -1).topk(top, -1)
+  order = chosen.reshape(-1).argsort(stable=True)
+  sizes = torch.bincount(chosen.reshape(-1), minlength=e).to(torch.int32)
+  row, weight = order // top, p.reshape(-1)[order]
+  cfg = bs.dot_general_make('e4m3', 'e5m2', po2_scale=po2)
+  leaf = x.clone().requires_grad_()
+  weights = [w.clone().requires_grad_() for w in ws]
+  seen = []
+
+  def product(a, w):
+    y = rd.ragged_dot(a, w, sizes, cfg=cfg)
+    at = {'a': a.detach().clone(), 'w': w, 'y': y.detach().clone()}
+    y.register_hook(lambda g: at.__setitem__('g', g.clone()))
+    seen.append(at)
+    return y
+
+  rows = leaf[row]
+  hidden = (torch.nn.functional.silu(product(rows, weights[0]).float()) *
+            product(rows, weights[1]).float()).bfloat16()
+  down = product(hidden, weights[2]).float() * weight[:, None]
+  y = torch.zeros(tokens, d, device='cuda').index_add(0, row, down)
+  (y * _data((tokens, d), torch.float32, 88)).sum().backward()
+  _done()
+  assert len(seen) == 3
+  for at, w in zip(seen, weights):
+    out, dl, dr = _want(_f32(at['a']), _f32(w.detach()), _f32(at['g']), sizes.tolist(), True, po2)
+    _check(at['y'], out, 2.0 ** -8, 'out')
+    _check(w.grad, dr, 2.0 ** -8, 'drhs')
+    at['dl'], at['mag'] = dl[0], dl[1]
+  # the tokens' gradient: two products' rows, summed over the experts of a token;
+  # rounded to bfloat16 by either product, in their sum, and in each of the sums
+  want, mag = np.zeros((tokens, d)), np.zeros((tokens, d))
+  for at in seen[:2]:
+    np.add.at(want, row.cpu().numpy(), at['dl'])
+    np.add.at(mag, row.cpu().numpy(), at['mag'])
+  tol = (2 + top) * 2.0 ** -8 * mag + f * 2.0 ** -23 * mag
+  assert (np.abs(_f32(leaf.grad) - want) <= tol).all()
