@@ -114,10 +114,8 @@ class GroupedGemmDesc(C.Structure):
       ('group_sizes', C.c_void_p), ('groups', C.c_int64),
       ('out', C.c_void_p), ('out_ld', C.c_int64), ('out_group_stride', C.c_int64),
       ('workspace', C.c_void_p), ('workspace_bytes', C.c_size_t),
-      ('a_far', C.c_void_p), ('a_far_k_stride', C.c_int64),
-      ('a_far_r_stride', C.c_int64),
-      ('b_far', C.c_void_p), ('b_far_k_stride', C.c_int64),
-      ('b_far_t_stride', C.c_int64), ('b_far_padded', C.c_int32),
+      ('far', C.c_void_p), ('far_k_stride', C.c_int64),
+      ('far_stride', C.c_int64), ('far_padded', C.c_int32),
   ]
 
 

@@ -36,6 +36,8 @@ BLOCK = 128
 _FLOATS = (torch.float32, torch.bfloat16)
 _FP8 = (torch.float8_e4m3fn, torch.float8_e5m2)
 _NULL_CONTEXT = contextlib.nullcontext()
+_NO_MARKS = ()
+_AD_LEVEL = hasattr(forward_ad, '_current_level')
 
 
 def fp8_dtype(bits) -> torch.dtype:
@@ -64,7 +66,7 @@ def on_device_of(x):
 def check_operand(x, name, dtypes=_FLOATS):
   if not isinstance(x, torch.Tensor):
     raise TypeError(f'{name} must be a torch tensor (got {type(x).__name__})')
-  if not engine._on_device(x):  # pylint: disable=protected-access
+  if not (x.is_cuda or engine._on_device(x)):  # pylint: disable=protected-access
     raise _lib.AqtB200Error(f'{name} must be a CUDA tensor (no CPU path)')
   if x.dtype == torch.float16 and x.dtype not in dtypes:
     engine._code(x.dtype)  # raises with the reason  pylint: disable=protected-access
@@ -72,7 +74,9 @@ def check_operand(x, name, dtypes=_FLOATS):
     raise NotImplementedError(
         f'{name} has dtype {x.dtype}; handled here: '
         + ', '.join(str(d) for d in dtypes))
-  if forward_ad.unpack_dual(x).tangent is not None:
+  # (torch's note of the open level first: unpacking takes longer than these checks)
+  if ((not _AD_LEVEL or forward_ad._current_level >= 0) and  # pylint: disable=protected-access
+      forward_ad.unpack_dual(x).tangent is not None):
     raise NotImplementedError(
         f'{name} carries a forward-mode tangent; these products have gradients '
         '(backward) only')
@@ -102,25 +106,22 @@ class Side:
   """One operand of a product: values with the contraction contiguous and their
   scales, as addresses and strides. `keep` holds the memory."""
   __slots__ = ('ptr', 'ld', 'group', 'code', 'scale', 'scale_group', 'scale_k',
-               'scale_r', 'kept', 'keep', 'far', 'far_k', 'far_kept',
-               'far_padded')
+               'scale_r', 'kept', 'keep', 'far')
 
   def __init__(self, ptr, ld, group, code, scale, scale_group, scale_k, scale_r,
-               kept, keep, far=None, far_k=0, far_kept=0, far_padded=0):
+               kept, keep, far=_NO_MARKS):
     self.ptr, self.ld, self.group, self.code = ptr, ld, group, code
     self.scale, self.scale_group = scale, scale_group
     self.scale_k, self.scale_r = scale_k, scale_r
     self.kept, self.keep = kept, keep
-    self.far, self.far_k, self.far_kept = far, far_k, far_kept
-    self.far_padded = far_padded
+    self.far = far  # marks: address, strides of a block of k and of 128 kept, padded
 
   def at(self, base, memory):
     """This operand with its memory, once at `base`, in `memory` (or in none)."""
     shift = 0 if memory is None else memory.data_ptr() - base
     return Side(self.ptr + shift, self.ld, self.group, self.code,
                 self.scale + shift, self.scale_group, self.scale_k, self.scale_r,
-                self.kept, memory, None if self.far is None else self.far + shift,
-                self.far_k, self.far_kept, self.far_padded)
+                self.kept, memory, self.far and (self.far[0] + shift, *self.far[1:]))
 
 
 def _align(n):
@@ -183,12 +184,13 @@ def quantize(x, dtype, row=True, col=False, square=False, po2=False,
       end += _align(batch * row_blocks * c * 4)
   marks = not square and batch == 1
   if marks:
+    nbytes = _align(row_blocks * nc * 8)
     if row:
       at_f_row = end
-      end += _align(row_blocks * nc * 8)
+      end += nbytes
     if col:
       at_f_col = end
-      end += _align(row_blocks * nc * 8)
+      end += nbytes
   ws = _scratch(end, x.device)
   base = ws.data_ptr()
   desc = _lib.BlockQuantDesc(
@@ -200,21 +202,20 @@ def quantize(x, dtype, row=True, col=False, square=False, po2=False,
       base + at_s_col if col and not square else None, sizes_ptr, groups,
       base + at_f_row if marks and row else None,
       base + at_f_col if marks and col else None)
-  _check(engine._call(  # pylint: disable=protected-access
-      _lib.load().aqtb200_block_quantize, C.byref(desc), engine._stream()),  # pylint: disable=protected-access
-         'block_quantize')
+  _run('block_quantize', _lib.load().aqtb200_block_quantize, C.byref(desc),
+       engine._stream())  # pylint: disable=protected-access
   q = code[dtype]
   a = b = None
   if row:
     s = ((base + at_s_row, nr * nc, 1, nc) if square else
          (base + at_s_row, nc * r, r, 1))
     a = Side(base + at_q_row, ld_row, r * ld_row, q, *s, r, ws,
-             base + at_f_row if marks else None, 1, nc, group_sizes is not None)
+             (base + at_f_row, 1, nc, sizes_ptr != 0) if marks else _NO_MARKS)
   if col:
     s = ((base + at_s_row, nr * nc, nc, 1) if square else
          (base + at_s_col, row_blocks * c, c, 1))
     b = Side(base + at_q_col, ld_col, c * ld_col, q, *s, c, ws,
-             base + at_f_col if marks else None, nc, 1)
+             (base + at_f_col, nc, 1, 0) if marks else _NO_MARKS)
   return (b, a) if swap else (a, b)
 
 
@@ -248,9 +249,8 @@ def quantize_tensors(x, dtype, axis, square, po2):
       code[dtype], po2, square, 0, qp if row else None, ld,
       sp if row or square else None, None if row else qp, ld,
       None if row or square else sp, None, 0)
-  _check(engine._call(  # pylint: disable=protected-access
-      _lib.load().aqtb200_block_quantize, C.byref(desc), engine._stream()),  # pylint: disable=protected-access
-         'block_quantize')
+  _run('block_quantize', _lib.load().aqtb200_block_quantize, C.byref(desc),
+       engine._stream())  # pylint: disable=protected-access
   # back to x's axes: values lie [kept][contracted], row scales [block][kept]
   if axis == -2:
     view = view.transpose(-1, -2)
@@ -263,19 +263,22 @@ def quantize_tensors(x, dtype, axis, square, po2):
   return view, s
 
 
-def _check(rc, what):
+def _run(what, fn, *args):
+  """engine._call and the check of its answer, in one frame."""
+  rc = fn(*args)
+  if engine._tape is not None:  # pylint: disable=protected-access
+    engine._tape.ops.append((fn, args))  # pylint: disable=protected-access
   if rc:
     _lib.check(rc, what)
 
 
 def _gemm(desc, device, what):
   # a product of an earlier call that gave up is reported by the next one
-  words = engine.status_words(device)
+  words = engine._words.get(device) or engine.status_words(device)  # pylint: disable=protected-access
   if words[0]:
     engine.poll_words(words)
-  _check(engine._call(  # pylint: disable=protected-access
-      _lib.load().aqtb200_grouped_gemm, C.byref(desc), words, engine._stream()),  # pylint: disable=protected-access
-         what)
+  _run(what, _lib.load().aqtb200_grouped_gemm, C.byref(desc), words.address,
+       engine._stream())  # pylint: disable=protected-access
 
 
 def _sizes(group_sizes):
@@ -302,8 +305,7 @@ def fp8_rows(tokens, a, k, out_dtype, device, group_sizes=None, po2=False):
       a.ptr, a.ld, a.group, tokens.ptr, tokens.ld, 0, 0, 1, int64, po2, 1,
       a.scale, a.scale_group, a.scale_k, a.scale_r,
       tokens.scale, tokens.scale_k, sizes, groups,
-      out.data_ptr(), r, 0, None, 0, None, 0, 0, tokens.far, tokens.far_k,
-      tokens.far_kept, tokens.far_padded), device, 'block-scaled product')
+      out.data_ptr(), r, 0, None, 0, *tokens.far), device, 'block-scaled product')
   return out
 
 
@@ -319,8 +321,7 @@ def fp8_contract_rows(b, a, k, rows, out_dtype, device, group_sizes=None,
       1, a.code, b.code, engine._TORCH_CODE[out_dtype], r, t, k, rows,  # pylint: disable=protected-access
       a.ptr, a.ld, 0, b.ptr, b.ld, 0, 0, 0, int64, po2, 0,
       a.scale, 0, a.scale_k, 1, b.scale, b.scale_k, sizes, groups,
-      out.data_ptr(), r, t * r, None, 0, a.far, a.far_k, a.far_kept), device,
-        'block-scaled product')
+      out.data_ptr(), r, t * r, None, 0, *a.far), device, 'block-scaled product')
   return out
 
 
@@ -347,9 +348,8 @@ def pack(x, group_sizes=None):
   v = _lib.View(x.data_ptr(), _lib.BF16, 0, batch, 1, x.shape[-2], x.shape[-1],
                 x.stride(0) if x.ndim == 3 else 0, 0, x.stride(-2), x.stride(-1))
   sizes, _, int64 = _sizes(group_sizes)
-  _check(engine._call(  # pylint: disable=protected-access
-      _lib.load().aqtb200_pack_bf16_groups, C.byref(v), sizes, int64,
-      buf.data_ptr(), ld, engine._stream()), 'pack_bf16')  # pylint: disable=protected-access
+  _run('pack_bf16', _lib.load().aqtb200_pack_bf16_groups, C.byref(v), sizes, int64,
+       buf.data_ptr(), ld, engine._stream())  # pylint: disable=protected-access
   return buf[..., :x.shape[-1]]
 
 

@@ -1618,10 +1618,8 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   P.a_scale = d->a_scale; P.sa_g = d->a_scale_group_stride; P.sa_k = d->a_scale_k_stride;
   P.sa_r = d->a_scale_r_stride;
   P.b_scale = d->b_scale; P.sb_k = d->b_scale_k_stride;
-  P.far = (const uint64_t*)(a_row ? d->a_far : d->b_far);
-  P.far_k = a_row ? d->a_far_k_stride : d->b_far_k_stride;
-  P.far_t = a_row ? d->a_far_r_stride : d->b_far_t_stride;
-  P.far_padded = P.mode == 0 && grouped && d->b_far_padded;
+  P.far = (const uint64_t*)d->far; P.far_k = d->far_k_stride; P.far_t = d->far_stride;
+  P.far_padded = P.mode == 0 && grouped && d->far_padded;
   P.a = (const uint8_t*)d->a; P.a_ld = d->a_ld; P.a_g = d->a_group_stride;
   P.b = (const uint8_t*)d->b; P.b_ld = d->b_ld;
   P.k = (int)k; P.a_e5 = d->a_dtype == AQTB200_E5M2; P.b_e5 = d->b_dtype == AQTB200_E5M2;

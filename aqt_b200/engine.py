@@ -110,7 +110,11 @@ def _status_buf(device):
   return _status[key]
 
 
-_words = {}  # device -> int32[4] that its kernels and the host both address
+class _Words(C.c_int32 * 4):
+  """Status words; `address` as a number, quicker to hand over than the array."""
+
+
+_words = {}  # device -> _Words that its kernels and the host both address
 
 
 def status_words(device):
@@ -125,9 +129,10 @@ def status_words(device):
     if device.type == 'cuda':
       at = C.c_void_p()
       _lib.check(_lib.load().aqtb200_status_words(C.byref(at)), 'status_words')
-      words = (C.c_int32 * 4).from_address(at.value)
+      words = _Words.from_address(at.value)
     else:
-      words = (C.c_int32 * 4)()
+      words = _Words()
+    words.address = C.addressof(words)
     words = _words.setdefault(device, words)
   return words
 

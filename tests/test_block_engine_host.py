@@ -382,13 +382,14 @@ def test_traced_step_that_freezes_weights(monkeypatch, k, n, ragged):
 @pytest.fixture
 def gives_up(monkeypatch):
   """Products that report a wait that ran out, as many as the list says."""
+  import ctypes as C
   from aqt_b200 import _lib
   lib = _lib.load()
   gemm, left = lib.aqtb200_grouped_gemm, []
 
   def failing(desc, status, stream):
     if left:
-      status[0] = left.pop()
+      (C.c_int32 * 4).from_address(status)[0] = left.pop()
     return gemm(desc, status, stream)
 
   monkeypatch.setattr(lib, 'aqtb200_grouped_gemm', failing, raising=False)
