@@ -426,12 +426,14 @@ __device__ __forceinline__ const float* tile_a_scale(const GGParams& P, const Ti
   return P.a_scale + (P.mode == 0 ? (int64_t)T.seg * P.sa_g : 0) + (int64_t)(T.k0 / 128) * P.sa_k +
          (int64_t)row * P.sa_r;
 }
-// In two steps, so that the reads of the first 32 slabs are on their way meanwhile.
+// In two steps, so that the reads of the first 32 slabs are on their way meanwhile (but
+// for those of a block of 128 between the first and the last that the tile touches).
 template <bool A_ROW>
 struct FarLook {
   const float* a;      // scales of the weights' blocks
   const uint64_t* m0;  // marks of the first and the last block of 128
   const uint64_t* m1;
+  int blocks;
   float a_first;
   uint64_t m0_first, m1_first;
 
@@ -452,6 +454,7 @@ struct FarLook {
     }
     m0 = P.far + (int64_t)(T.k0 >> 7) * P.far_k + first * P.far_t;
     m1 = m0 + (last - first) * P.far_t;
+    blocks = last - first + 1;
     a_first = 0.f;
     m0_first = m1_first = 0;
     const int kb = kb0 + lane;
@@ -472,6 +475,10 @@ struct FarLook {
         if constexpr (!A_ROW) may |= m1[kb * P.far_k] != 0;
       }
     }
+    if constexpr (!A_ROW)
+      if (P.far != nullptr)
+        for (int x = 1; x < blocks - 1; ++x)
+          for (int kb = kb0 + lane; kb < kb1; kb += 32) may |= m0[kb * P.far_k + x * P.far_t] != 0;
     return __any_sync(0xffffffffu, may);
   }
 };
@@ -929,15 +936,10 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         if (!convert()) fail = 4;
       if (fail) give_up(4);
     }
-    // A look at the range of a tile's scales, for which nothing waits. Wide tiles: by
-    // warp 3 (by warp 2 a prompt of 2047 took 2 % longer). Narrow ones: by warp 2 once
-    // the tile's scales are on their way (by warp 3 a token took 1.0 us longer, for the
-    // instructions it fetched beside the first tile's; so 0.4 us of 12). Read from the
-    // slots, or scale by scale, it took longer than the products.
     // The range of a tile's scales is looked at beside the products; nothing but the
     // kernel's end waits for it. Wide tiles: by warp 3 (by warp 2 a prompt of 2047 x 4096
     // x 14336 took 2 % longer). Narrow ones: by warp 2, around the copies of the tile's
-    // scales: one token of 4096 x 4096 takes 12.4 us with its quantizer, 12.1 without the
+    // scales: one token of 4096 x 4096 takes 12.5 us with its quantizer, 12.0 without the
     // look, 13.1 with warp 3 doing it, for the instructions it fetches beside the first
     // tile's. Read from the slots, or scale by scale, it took longer than the products.
     auto tell = [&]() {  // the CTA that stores the tile
@@ -1544,6 +1546,7 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   const int64_t k = d->k;
   AQT_REQUIRE(k == 0 || !fp8 || (d->a_scale != nullptr && d->b_scale != nullptr), AQTB200_EINVAL,
               "fp8 operands need their scales");
+  AQT_REQUIRE(((uintptr_t)d->far & 7) == 0, AQTB200_EINVAL, "marks are eight bytes each, 8-byte aligned");
 
   GGParams P{};
   P.mode = d->contract_groups;
@@ -1563,7 +1566,7 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   // / 711; 8192 x 8192 x 8192: 471 / 469 / 465 against 620 / 615 / 762). Its sums drop what
   // does not fit 24 bits, each step of 32 products less than 2^-23 of the running
   // sum (measured, all products positive: 2^-26 a step, 8e-6 over 14336): nothing
-  // beside a bf16 result's rounding of 2^-9 as long as the steps' total stays below
+  // beside a bf16 result's rounding of 2^-8 as long as the steps' total stays below
   // 2^-10. f32 results keep the f32 registers.
   const bool po2 = fp8 && d->scales_po2 && d->out_dtype == AQTB200_BF16 && P.num_kb * 4 <= 1 << 13 &&
                    (d->a_scale_square || d->a_scale_r_stride == 1);
@@ -1584,8 +1587,13 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   // weights, and an MMA's time goes with its columns.
   P.nt = want <= most ? (int)std::max<int64_t>(32, (want + 31) / 32 * 32) : most;
   if (want > most && !grouped) {
-    // all sizes known: the width whose rounds cost least in total; each tile has a
-    // cost of its own besides, larger where the epilogue adds every 128-block
+    // The width whose rounds cost least in total; each tile has a cost of its own
+    // besides, in columns: 80 where the epilogue adds every 128-block, 8 otherwise. With
+    // f32 scales 2047 x 4096 x 14336 takes 174 us at 80 or 160 and 242 at 0 or 8, 4096 x
+    // 4096 x 4096 109 and 128, 3300 x 4096 x 3500 87 and 113, 700 x 4096 x 20000 103 and
+    // 123; on the tensor core 0, 8 and 80 give the same to 1 % but for the last but one
+    // (86, 86, 77 us). Products with groups are left out: the number of their tiles, or
+    // how long each group's contraction is, is known on the device only.
     const int extra = po2 || !fp8 ? 8 : 80;
     int64_t least = INT64_MAX;
     for (int nt = most; nt >= 160; nt -= 32) {

@@ -291,3 +291,5 @@ def test_abi_marks(lib):
   d = _quant_desc(far_row=256)
   d.x.b0 = 2
   assert call(d) == -2
+  d = _gemm_desc(a_dtype=_lib.E4M3, b_dtype=_lib.E4M3, a_scale=256, b_scale=256, far=260)
+  assert lib.aqtb200_grouped_gemm(C.byref(d), None, None) == -1

@@ -558,3 +558,33 @@ def test_projection_stack_product_by_product():
           _f32(at['x']), _f32(at['w']), _f32(at['g']))):
         ref.assert_close(_f32(at[what]).astype(np.float64), want, mag, kk,
                          2.0 ** -8, f'{name} {what}')
+
+
+@pytest.mark.parametrize('m,n', [(1500, 5120), (2047, 7168), (3300, 3500), (700, 12000),
+                                 (130, 200)])
+@pytest.mark.parametrize('rows', [128, 1])
+def test_far_rows_wherever_they_lie(m, n, rows):
+  """Tiles of any width: rows that need care lie in any one of the blocks of 128 that
+  a tile covers, its middle one too."""
+  k = 256
+  x, w = _data((m, k), torch.float32, 76, 1.0), _data((k, n), torch.float32, 77, 0.3)
+  w *= 2.0 ** -50  # scales that alone are no reason for care
+  cfg = bs.dot_general_make()
+  qt = bs.block_quantize(w, 0, square=True)
+  assert float(qt.scale[0].min()) > 2.0 ** -63
+  base = cfg(x, qt, DIMS)
+  mag = cfg(x.abs(), bs.frozen(qt.qvalue.float().abs().to(torch.float8_e4m3fn),
+                               qt.scale[0]), DIMS).double()
+  for first in range(0, m, 128):
+    at = slice(first + (17 if rows == 1 and first + 17 < m else 0), None)
+    at = slice(at.start, min(at.start + rows, m))
+    far = x.clone()
+    far[at] *= 2.0 ** -75
+    out = cfg(far, qt, DIMS)
+    # two sums of the same products, each off by k 2^-23 of their magnitudes
+    off = (out[at].double() * 2.0 ** 75 - base[at].double()).abs()
+    assert (off <= 2 * (k + 9) * 2.0 ** -23 * mag[at]).all(), first
+    same = torch.ones(m, dtype=torch.bool, device='cuda')
+    same[at] = False
+    assert torch.equal(out[same], base[same]), first
+  _done()

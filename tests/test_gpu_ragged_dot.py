@@ -711,3 +711,35 @@ def test_expert_layer_in_fp8_product_by_product(po2):
     np.add.at(mag, row.cpu().numpy(), at['mag'])
   tol = (2 + top) * 2.0 ** -8 * mag + f * 2.0 ** -23 * mag
   assert (np.abs(_f32(leaf.grad) - want) <= tol).all()
+
+
+@pytest.mark.parametrize('m,n,sizes', [(1700, 6000, [100, 900, 0, 655]),
+                                       (300, 264, [33, 200, 0, 60])])
+def test_far_rows_wherever_they_lie(m, n, sizes):
+  """Rows that need care lie in any block of 128 that a tile of a group covers,
+  counted from the first row (serving) or from the group's (training)."""
+  k = 256
+  x, w = _data((m, k), torch.float32, 100), _data((4, k, n), torch.float32, 101,
+                                                 0.3 * 2.0 ** -50)
+  cfg = bs.dot_general_make()
+  s, qt = _sizes(sizes), bs.block_quantize(w, 1, square=True)
+  assert float(qt.scale[0].min()) > 2.0 ** -63
+  leaf = lambda t: t.clone().requires_grad_()
+  runs = (lambda t: rd.ragged_dot(t, qt, s, cfg=cfg),
+          lambda t: rd.ragged_dot(leaf(t), leaf(w), s, cfg=cfg).detach())
+  base = runs[0](x)
+  assert torch.equal(base, runs[1](x))
+  mag = rd.ragged_dot(x.abs(), bs.frozen(qt.qvalue.float().abs().to(
+      torch.float8_e4m3fn), qt.scale[0]), s, cfg=cfg).double()
+  for first in range(0, sum(sizes), 61):
+    at = slice(first, min(first + 3, m))
+    far = x.clone()
+    far[at] *= 2.0 ** -75
+    for run in runs:
+      out = run(far)
+      off = (out[at].double() * 2.0 ** 75 - base[at].double()).abs()
+      assert (off <= 2 * (k + 9) * 2.0 ** -23 * mag[at]).all(), first
+      same = torch.ones(m, dtype=torch.bool, device='cuda')
+      same[at] = False
+      assert torch.equal(out[same], base[same]), first
+  _done()
