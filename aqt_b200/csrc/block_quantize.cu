@@ -18,6 +18,8 @@
 // of the copy bandwidth), the transposed one 62 us, both 88 us (0.81), square in
 // both orders 79 us; four blocks a SM, since with three the instructions, not the
 // memory, are the bound (61, 71, 97, 88 us). 8192 x 7168 f32: 47, 53, 67, 61 us.
+// Each warp can also mark whether one of its scales lies outside 2^-63 .. 2^63: a byte
+// of its own, written whatever it says, so that no call has to clear it first.
 #include <algorithm>
 
 #include "block_scales.cuh"

@@ -16,6 +16,7 @@
 //   warp 0      TMA producer, 128-byte k-slabs, 128-byte swizzle, no multicast
 //   warp 1      MMA issuer (of a pair: in its even CTA)
 //   warp 2      first the scan of the groups, then scales (fp8; MX: warp 3 too)
+//   warp 3      of wide fp8 tiles, not MX: a look at the scales' range (narrow: warp 2)
 //   warps 4-    epilogue: two or four per TMEM lane quarter, up to 64 columns each
 // Warps 0 and 1 run whole, with one elected lane issuing. bf16 accumulates the
 // whole contraction in TMEM (two 256-column accumulators: the epilogue of one tile
@@ -706,9 +707,9 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       const uint32_t ring = smem_u32(smem);
       // The weights of the first stages are asked for while the quantizer of the
       // other operand may still run (see `follows_quantize`); what reads its results
-      // waits for it, in every CTA, so that this grid ends after it. In a graph: 1 x
-      // 4096 x 4096 13.7 -> 12.2 us with the quantizer, 16 x 8192 x 28672 47.8 ->
-      // 46.0, 257 rows of 64 experts 2048 x 1408 42.4 -> 38.1.
+      // waits for it, in every CTA, so that this grid ends after it. In a graph it took
+      // 1.5 us off the 13.7 of 1 x 4096 x 4096 with its quantizer, 1.8 off the 47.8 of
+      // 16 x 8192 x 28672, 4.3 off the 42.4 of 257 rows of 64 experts 2048 x 1408.
       int ahead = 0;
       if constexpr (FP8) {
         if (P.mode == 0 && cluster_id < total) {

@@ -20,7 +20,8 @@ weights serves the forward product and dlhs:
 
 A block: a = max|x|, s = max((a or 1) / bound, 2^-126) in f32 [, up to a power of
 two], q = fp8(x * (1 / s)); products of 128 are summed on the tensor core, scaled
-and added in f32, and the result is rounded once to the output's dtype. With
+and added in f32, and the result is rounded once to the output's dtype -- for any
+scales, also where the product of two is no f32 number and the result is one. With
 po2_scale and a bfloat16 result the tensor core scales and sums large products by
 itself, 1.3 times as fast; its sums drop what does not fit 24 bits (up to 2^-23 of
 the running sum for each 32 products). A NaN or an infinity in a block makes that
