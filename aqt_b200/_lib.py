@@ -93,7 +93,7 @@ class BlockQuantDesc(C.Structure):
       ('q_row', C.c_void_p), ('ld_row', C.c_int64), ('scale_row', C.c_void_p),
       ('q_col', C.c_void_p), ('ld_col', C.c_int64), ('scale_col', C.c_void_p),
       ('group_sizes', C.c_void_p), ('groups', C.c_int64),
-      ('far_row', C.c_void_p), ('far_col', C.c_void_p),
+      ('note_row', C.c_void_p), ('note_col', C.c_void_p),
   ]
 
 
@@ -114,8 +114,8 @@ class GroupedGemmDesc(C.Structure):
       ('group_sizes', C.c_void_p), ('groups', C.c_int64),
       ('out', C.c_void_p), ('out_ld', C.c_int64), ('out_group_stride', C.c_int64),
       ('workspace', C.c_void_p), ('workspace_bytes', C.c_size_t),
-      ('far', C.c_void_p), ('far_k_stride', C.c_int64),
-      ('far_stride', C.c_int64), ('far_padded', C.c_int32),
+      ('note', C.c_void_p), ('note_k_stride', C.c_int64),
+      ('note_stride', C.c_int64), ('note_padded', C.c_int32),
   ]
 
 

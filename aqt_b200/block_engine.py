@@ -13,8 +13,8 @@ quantized operand of this library; scales with the kept index contiguous):
                     col   q [C][ld], scale [R/128][C]     blocks along R
                     square: both orders of q, ONE scale [R/128][C/128]
 
-Row and col scales come with marks on those that f32 products have to be careful
-with (aqtb200_block_quantize's far_row, far_col); the products read them.
+Row and col scales come with notes on their range (aqtb200_block_quantize's note_row,
+note_col), by which the products find those that f32 has to be careful with.
 
 The calls here are short next to their kernels' launches, so what a product
 needs between its kernels is one torch allocation, addressed by offsets, and
@@ -36,7 +36,7 @@ BLOCK = 128
 _FLOATS = (torch.float32, torch.bfloat16)
 _FP8 = (torch.float8_e4m3fn, torch.float8_e5m2)
 _NULL_CONTEXT = contextlib.nullcontext()
-_NO_MARKS = ()
+_NO_NOTES = ()
 _AD_LEVEL = hasattr(forward_ad, '_current_level')
 
 
@@ -106,22 +106,22 @@ class Side:
   """One operand of a product: values with the contraction contiguous and their
   scales, as addresses and strides. `keep` holds the memory."""
   __slots__ = ('ptr', 'ld', 'group', 'code', 'scale', 'scale_group', 'scale_k',
-               'scale_r', 'kept', 'keep', 'far')
+               'scale_r', 'kept', 'keep', 'note')
 
   def __init__(self, ptr, ld, group, code, scale, scale_group, scale_k, scale_r,
-               kept, keep, far=_NO_MARKS):
+               kept, keep, note=_NO_NOTES):
     self.ptr, self.ld, self.group, self.code = ptr, ld, group, code
     self.scale, self.scale_group = scale, scale_group
     self.scale_k, self.scale_r = scale_k, scale_r
     self.kept, self.keep = kept, keep
-    self.far = far  # marks: address, strides of a block of k and of 128 kept, padded
+    self.note = note  # address, strides of a block of k and of 128 kept, padded
 
   def at(self, base, memory):
     """This operand with its memory, once at `base`, in `memory` (or in none)."""
     shift = 0 if memory is None else memory.data_ptr() - base
     return Side(self.ptr + shift, self.ld, self.group, self.code,
                 self.scale + shift, self.scale_group, self.scale_k, self.scale_r,
-                self.kept, memory, self.far and (self.far[0] + shift, *self.far[1:]))
+                self.kept, memory, self.note and (self.note[0] + shift, *self.note[1:]))
 
 
 def _align(n):
@@ -165,7 +165,7 @@ def quantize(x, dtype, row=True, col=False, square=False, po2=False,
     row_blocks = r // BLOCK + min(groups, r)
     int64 = int(group_sizes.dtype == torch.int64)
     sizes_ptr = group_sizes.data_ptr()
-  at_q_row = at_s_row = at_q_col = at_s_col = at_f_row = at_f_col = end = 0
+  at_q_row = at_s_row = at_q_col = at_s_col = at_n_row = at_n_col = end = 0
   if row:
     ld_row = (c + 15) & -16
     end = _align(batch * r * ld_row)
@@ -182,14 +182,14 @@ def quantize(x, dtype, row=True, col=False, square=False, po2=False,
     if not square:
       at_s_col = end
       end += _align(batch * row_blocks * c * 4)
-  marks = not square and batch == 1
-  if marks:
-    nbytes = _align(row_blocks * nc * 8)
+  notes = not square and batch == 1
+  if notes:
+    nbytes = _align(row_blocks * nc * 16)
     if row:
-      at_f_row = end
+      at_n_row = end
       end += nbytes
     if col:
-      at_f_col = end
+      at_n_col = end
       end += nbytes
   ws = _scratch(end, x.device)
   base = ws.data_ptr()
@@ -200,8 +200,8 @@ def quantize(x, dtype, row=True, col=False, square=False, po2=False,
       base + at_s_row if row or square else None,
       base + at_q_col if col else None, ld_col,
       base + at_s_col if col and not square else None, sizes_ptr, groups,
-      base + at_f_row if marks and row else None,
-      base + at_f_col if marks and col else None)
+      base + at_n_row if notes and row else None,
+      base + at_n_col if notes and col else None)
   _run('block_quantize', _lib.load().aqtb200_block_quantize, C.byref(desc),
        engine._stream())  # pylint: disable=protected-access
   q = code[dtype]
@@ -210,12 +210,12 @@ def quantize(x, dtype, row=True, col=False, square=False, po2=False,
     s = ((base + at_s_row, nr * nc, 1, nc) if square else
          (base + at_s_row, nc * r, r, 1))
     a = Side(base + at_q_row, ld_row, r * ld_row, q, *s, r, ws,
-             (base + at_f_row, 1, nc, sizes_ptr != 0) if marks else _NO_MARKS)
+             (base + at_n_row, 1, nc, sizes_ptr != 0) if notes else _NO_NOTES)
   if col:
     s = ((base + at_s_row, nr * nc, nc, 1) if square else
          (base + at_s_col, row_blocks * c, c, 1))
     b = Side(base + at_q_col, ld_col, c * ld_col, q, *s, c, ws,
-             (base + at_f_col, nc, 1, 0) if marks else _NO_MARKS)
+             (base + at_n_col, nc, 1, 0) if notes else _NO_NOTES)
   return (b, a) if swap else (a, b)
 
 
@@ -305,7 +305,7 @@ def fp8_rows(tokens, a, k, out_dtype, device, group_sizes=None, po2=False):
       a.ptr, a.ld, a.group, tokens.ptr, tokens.ld, 0, 0, 1, int64, po2, 1,
       a.scale, a.scale_group, a.scale_k, a.scale_r,
       tokens.scale, tokens.scale_k, sizes, groups,
-      out.data_ptr(), r, 0, None, 0, *tokens.far), device, 'block-scaled product')
+      out.data_ptr(), r, 0, None, 0, *tokens.note), device, 'block-scaled product')
   return out
 
 
@@ -321,7 +321,7 @@ def fp8_contract_rows(b, a, k, rows, out_dtype, device, group_sizes=None,
       1, a.code, b.code, engine._TORCH_CODE[out_dtype], r, t, k, rows,  # pylint: disable=protected-access
       a.ptr, a.ld, 0, b.ptr, b.ld, 0, 0, 0, int64, po2, 0,
       a.scale, 0, a.scale_k, 1, b.scale, b.scale_k, sizes, groups,
-      out.data_ptr(), r, t * r, None, 0, *a.far), device, 'block-scaled product')
+      out.data_ptr(), r, t * r, None, 0, *a.note), device, 'block-scaled product')
   return out
 
 

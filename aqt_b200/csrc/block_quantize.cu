@@ -18,8 +18,8 @@
 // of the copy bandwidth), the transposed one 62 us, both 88 us (0.81), square in
 // both orders 79 us; four blocks a SM, since with three the instructions, not the
 // memory, are the bound (61, 71, 97, 88 us). 8192 x 7168 f32: 47, 53, 67, 61 us.
-// Each warp can also mark whether one of its scales lies outside 2^-63 .. 2^63: a byte
-// of its own, written whatever it says, so that no call has to clear it first.
+// Each warp can also note the range of its scales, in bytes of its own (block_scales.cuh)
+// that are written whatever they say, so that no call has to clear them first.
 #include <algorithm>
 
 #include "block_scales.cuh"
@@ -39,7 +39,7 @@ struct BqParams {
   uint8_t* q_col;
   int64_t ld_col;
   float* s_col;
-  uint8_t *far_row, *far_col;  // optional marks, a byte for each warp and tile
+  uint16_t *note_row, *note_col;  // optional notes on the scales, of each warp and tile
   int64_t row_tiles, col_tiles;
   const void* sizes;  // optional: rows fall into groups, row blocks start anew in each
   int sizes64;
@@ -306,9 +306,9 @@ __global__ void __launch_bounds__(BQ_THREADS, BF16 ? 4 : 2) block_quantize_kerne
       const float inv = __fdiv_rn(1.f, s);
       const int64_t r = row + ((lane >> 1) & 7);
       if ((lane & 1) == 0 && r < row_end) P.s_row[(b * P.col_tiles + ct) * P.rows + r] = s;
-      if (P.far_row != nullptr) {
-        const bool far = __any_sync(0xffffffffu, may_be_far(s));
-        if (lane == 0) P.far_row[(rt * P.col_tiles + ct) * 8 + warp] = far;
+      if (P.note_row != nullptr) {
+        const uint16_t note = scale_note(s);
+        if (lane == 0) P.note_row[(rt * P.col_tiles + ct) * 8 + warp] = note;
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) inv_r[i] = __shfl_sync(0xffffffffu, inv, (lane & 16) | (i << 1));
@@ -325,7 +325,7 @@ __global__ void __launch_bounds__(BQ_THREADS, BF16 ? 4 : 2) block_quantize_kerne
       }
       *(uint4*)&red[warp][c8 * 8 + (upper ? 4 : 0)] = make_uint4(m[0], m[1], m[2], m[3]);
       __syncthreads();
-      bool far = false;
+      float scale = 0.f;
       if (tid < QB) {
         uint32_t top = 0;
 #pragma unroll
@@ -334,11 +334,11 @@ __global__ void __launch_bounds__(BQ_THREADS, BF16 ? 4 : 2) block_quantize_kerne
         col_inv[tid] = __fdiv_rn(1.f, s);
         if (ct * QB + tid < P.cols)
           P.s_col[(b * P.row_tiles + rt) * P.cols + ct * QB + tid] = s;
-        far = may_be_far(s);
+        scale = s;
       }
-      if (P.far_col != nullptr) {
-        far = __any_sync(0xffffffffu, far);
-        if (lane == 0) P.far_col[(rt * P.col_tiles + ct) * 8 + warp] = far;
+      if (P.note_col != nullptr) {
+        const uint16_t note = scale_note(scale);
+        if (lane == 0) P.note_col[(rt * P.col_tiles + ct) * 8 + warp] = note;
       }
       __syncthreads();
 #pragma unroll
@@ -409,16 +409,16 @@ int aqtb200_block_quantize(const aqtb200_block_quant_desc* d, void* stream) {
                            (d->q_col == nullptr || d->scale_col != nullptr)),
               AQTB200_EINVAL, "an output has no place for its scales");
   AQT_REQUIRE(v.ptr != nullptr, AQTB200_EINVAL, "null input");
-  AQT_REQUIRE((d->far_row == nullptr && d->far_col == nullptr) ||
-                  (batch == 1 && !d->square && (((uintptr_t)d->far_row | (uintptr_t)d->far_col) & 7) == 0),
-              AQTB200_EUNSUPPORTED, "marks: of one matrix in blocks of 1 x 128, 8-byte aligned");
+  AQT_REQUIRE((d->note_row == nullptr && d->note_col == nullptr) ||
+                  (batch == 1 && !d->square && (((uintptr_t)d->note_row | (uintptr_t)d->note_col) & 15) == 0),
+              AQTB200_EUNSUPPORTED, "notes on scales: of one matrix in blocks of 1 x 128, 16-byte aligned");
   BqParams P{};
   P.x = v.ptr;
   P.rows = v.rows; P.cols = v.cols; P.b1 = v.b1;
   P.bs0 = v.b0_stride; P.bs1 = v.b1_stride; P.rs = v.row_stride; P.cs = v.col_stride;
   P.q_row = (uint8_t*)d->q_row; P.ld_row = d->ld_row; P.s_row = d->scale_row;
   P.q_col = (uint8_t*)d->q_col; P.ld_col = d->ld_col; P.s_col = d->scale_col;
-  P.far_row = (uint8_t*)d->far_row; P.far_col = (uint8_t*)d->far_col;
+  P.note_row = (uint16_t*)d->note_row; P.note_col = (uint16_t*)d->note_col;
   P.po2 = d->po2_scale; P.square = d->square;
   P.bound = d->qdtype == AQTB200_E4M3 ? 448.f : 57344.f;
   P.col_tiles = (v.cols + QB - 1) / QB;

@@ -107,11 +107,11 @@ struct GGParams {
   int64_t sa_g, sa_k, sa_r;
   const float* b_scale;
   int64_t sb_k;
-  // marks of the quantizer on a's rows (row scales) or b's, eight bytes for 128 of them and
-  // a slab, or none; far_padded: by 128 rows of each group
-  const uint64_t* far;
-  int64_t far_k, far_t;
-  int far_padded;
+  // the quantizer's notes on a's rows (row scales) or b's, one for 128 of them and a
+  // slab, or none; note_padded: by 128 rows of each group
+  const uint4* note;
+  int64_t note_k, note_t;
+  int note_padded;
   // fp8 operands as far_tile reads them
   const uint8_t *a, *b;
   int64_t a_ld, a_g, b_ld;
@@ -393,15 +393,16 @@ __device__ __forceinline__ int share_of(int nkb, int part, int split) {
 //   row scales       the sum times the row's scale, where that lies in ROW_MIN .. ROW_MAX
 // Elements with a block of other scales are computed again, by far_tile, when all is
 // stored. (Nothing of this is in the epilogue's loop or between its tiles: choosing
-// slab by slab cost 2 to 5 %, and a verdict on each tile 1 to 2 %.)
-constexpr float GG_MIN_NORMAL = 0x1p-126f;
+// slab by slab cost 2 to 5 %, and a verdict on each tile 1 to 2 %.) 8192 x 4096 x 14336
+// with operands of 2^-60 and 2^-62, all of it: 82 ms in place of 0.6; cotangents of
+// 2^-95, where it only looks: 5.0 ms backward in place of 1.3.
 constexpr float GG_ROW_MIN = 0x1p-94f, GG_ROW_MAX = 0x1p89f;
 template <bool A_ROW>
 __device__ __forceinline__ bool is_far(float ra, float s) {
   if (!finite_nonzero(ra)) return false;
   if constexpr (A_ROW) return fabsf(ra) < GG_ROW_MIN || fabsf(ra) > GG_ROW_MAX;
   const float p = fabsf(s * ra);
-  return finite_nonzero(s) && (p < GG_MIN_NORMAL || p > SCALE_MAX_FLOAT);
+  return finite_nonzero(s) && (p < SCALE_MIN_NORMAL || p > SCALE_MAX_FLOAT);
 }
 // acc + sum * ra * s. Part of a far factor goes to the sum first; a far row scale is
 // brought 2^40 nearer to 1 for both products and sent back in the add.
@@ -417,35 +418,29 @@ __device__ __forceinline__ float far_add(float acc, float sum, float ra, float s
   if (fabsf(s * ra) < 1.f) return fmaf(sum * 0x1p-90f, (s * 0x1p45f) * (ra * 0x1p45f), acc);
   return fmaf(sum * 0x1p120f, (s * 0x1p-60f) * (ra * 0x1p-60f), acc);
 }
-__device__ __forceinline__ float2 fp8_pair(uint32_t v, int e5) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)v, e5 ? __NV_E5M2 : __NV_E4M3);
-  return __half22float2(*(const __half2*)&h);
-}
-// Whether some of slabs kb0 .. kb1 of a CTA's tile, rows from row0 on, may be far: by the
-// scales of the weights' blocks, and by the quantizer's marks on the others.
-__device__ __forceinline__ const float* tile_a_scale(const GGParams& P, const TileAt& T, int row) {
-  return P.a_scale + (P.mode == 0 ? (int64_t)T.seg * P.sa_g : 0) + (int64_t)(T.k0 / 128) * P.sa_k +
-         (int64_t)row * P.sa_r;
-}
-// In two steps, so that the reads of the first 32 slabs are on their way meanwhile (but
-// for those of a block of 128 between the first and the last that the tile touches).
+// A look at the range of slabs kb0 .. kb1 of a CTA's tile, rows from row0 on: whether a
+// pair of scales may be far, by the quantizer's notes and, weights' blocks, their own
+// scales. In two steps, so that the reads of the first 32 slabs are on their way
+// meanwhile (but for those of a block of 128 between the first and the last that the
+// tile touches).
 template <bool A_ROW>
 struct FarLook {
-  const float* a;      // scales of the weights' blocks
-  const uint64_t* m0;  // marks of the first and the last block of 128
-  const uint64_t* m1;
+  const float* a;   // scales of the weights' blocks
+  const uint4* m0;  // notes on the first and the last block of 128
+  const uint4* m1;
   int blocks;
   float a_first;
-  uint64_t m0_first, m1_first;
+  uint4 m0_first, m1_first;
 
   __device__ __forceinline__ void begin(const GGParams& P, const Segments& S, const TileAt& T, int kb0, int kb1,
                                         int row0, int lane) {
     row0 = min(row0, P.r - 1);
-    a = tile_a_scale(P, T, row0 >> 7);
+    a = P.a_scale + (P.mode == 0 ? (int64_t)T.seg * P.sa_g : 0) + (int64_t)(T.k0 >> 7) * P.sa_k +
+        (int64_t)(row0 >> 7) * P.sa_r;
     int first = row0 >> 7, last = first;
     if constexpr (!A_ROW) {
       int t = T.t0, before = 0;
-      if (P.far_padded) {
+      if (P.note_padded) {
         t -= S.off[T.seg];
         for (int g = lane; g < T.seg; g += 32) before += (S.off[g + 1] - S.off[g] + 127) >> 7;
         before = __reduce_add_sync(0xffffffffu, before);
@@ -453,97 +448,190 @@ struct FarLook {
       first = before + (t >> 7);
       last = before + ((t + T.tvalid - 1) >> 7);
     }
-    m0 = P.far + (int64_t)(T.k0 >> 7) * P.far_k + first * P.far_t;
-    m1 = m0 + (last - first) * P.far_t;
+    m0 = P.note + (int64_t)(T.k0 >> 7) * P.note_k + first * P.note_t;
+    m1 = m0 + (last - first) * P.note_t;
     blocks = last - first + 1;
     a_first = 0.f;
-    m0_first = m1_first = 0;
+    m0_first = m1_first = make_uint4(0, 0, 0, 0);
     const int kb = kb0 + lane;
     if (kb < kb1) {
       if constexpr (!A_ROW) a_first = a[kb * P.sa_k];
-      if (P.far != nullptr) {
-        m0_first = m0[kb * P.far_k];
-        if constexpr (!A_ROW) m1_first = m1[kb * P.far_k];
+      if (P.note != nullptr) {
+        m0_first = m0[kb * P.note_k];
+        if constexpr (!A_ROW) m1_first = m1[kb * P.note_k];
       }
     }
   }
+  static __device__ __forceinline__ bool may_be_far(float a, uint32_t note) {
+    const float least = note_least(note), most = note_most(note);
+    if constexpr (A_ROW) return (least > 0.f && least < GG_ROW_MIN) || most > GG_ROW_MAX;
+    return finite_nonzero(a) && most > 0.f &&
+           (least * fabsf(a) < SCALE_MIN_NORMAL || most * fabsf(a) > SCALE_MAX_FLOAT);
+  }
   __device__ __forceinline__ bool finish(const GGParams& P, int kb0, int kb1, int lane) const {
-    bool may = may_be_far(a_first) || (m0_first | m1_first) != 0;
+    const bool noted = P.note != nullptr;
+    bool may = kb0 + lane < kb1 &&
+               may_be_far(a_first, noted ? __vmaxu4(join_notes(m0_first), join_notes(m1_first)) : NOTE_ORDINARY);
     for (int kb = kb0 + 32 + lane; kb < kb1; kb += 32) {
-      if constexpr (!A_ROW) may |= may_be_far(a[kb * P.sa_k]);
-      if (P.far != nullptr) {
-        may |= m0[kb * P.far_k] != 0;
-        if constexpr (!A_ROW) may |= m1[kb * P.far_k] != 0;
+      float s = 0.f;
+      uint32_t note = NOTE_ORDINARY;
+      if constexpr (!A_ROW) s = a[kb * P.sa_k];
+      if (noted) {
+        note = join_notes(m0[kb * P.note_k]);
+        if constexpr (!A_ROW) note = __vmaxu4(note, join_notes(m1[kb * P.note_k]));
       }
+      may |= may_be_far(s, note);
     }
     if constexpr (!A_ROW)
-      if (P.far != nullptr)
+      if (noted)
         for (int x = 1; x < blocks - 1; ++x)
-          for (int kb = kb0 + lane; kb < kb1; kb += 32) may |= m0[kb * P.far_k + x * P.far_t] != 0;
+          for (int kb = kb0 + lane; kb < kb1; kb += 32)
+            may |= may_be_far(a[kb * P.sa_k], join_notes(m0[kb * P.note_k + x * P.note_t]));
     return __any_sync(0xffffffffu, may);
   }
 };
-// Whether one is: every pair is tried.
-template <bool A_ROW>
-__device__ __forceinline__ bool far_scales(const GGParams& P, const TileAt& T, int kb0, int kb1, int row0,
-                                           int lane) {
-  const float* sa = tile_a_scale(P, T, A_ROW ? row0 : min(row0, P.r - 1) >> 7);
-  const float* sb = P.b_scale + (int64_t)(T.k0 / 128) * P.sb_k + T.t0;
-  const int count = A_ROW ? min(128, P.r - row0) : T.tvalid;
-  bool far = false;
-  for (int kb = kb0; kb < kb1; ++kb)
-    for (int c = lane; c < count; c += 32) {
-      const float v = A_ROW ? sa[c * P.sa_r + kb * P.sa_k] : sb[kb * P.sb_k + c];
-      far |= is_far<A_ROW>(A_ROW ? v : sa[kb * P.sa_k], v);
+
+// Sixteen fp8 values, zeros from the `left`-th on.
+__device__ __forceinline__ uint4 fp8_piece(const uint8_t* p, int left) {
+  if (left <= 0) return make_uint4(0, 0, 0, 0);
+  uint4 v = *(const uint4*)p;
+  if (left < 16) {
+    uint32_t* w = (uint32_t*)&v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = left - 4 * i;
+      w[i] = n <= 0 ? 0u : n < 4 ? w[i] & ((1u << (8 * n)) - 1u) : w[i];
     }
-  return __any_sync(0xffffffffu, far);
+  }
+  return v;
+}
+// Two of them as f16, which holds both formats exactly.
+__device__ __forceinline__ uint32_t fp8_pair(uint32_t v, int e5) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)v, e5 ? __NV_E5M2 : __NV_E4M3);
+  return (uint32_t)h.x | (uint32_t)h.y << 16;
+}
+__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                        uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Writes the elements of a warp's part of a tile -- rows from r0 on, `n` columns from c0
-// on -- that have a far block, from the operands in global memory. Other elements keep
-// their value, so that no result depends on its neighbours. A call of its own, off the
-// epilogue's registers.
+// Writes the elements of a warp's part of a tile -- 32 rows from r0 on, `n` columns from
+// c0 on -- that a far block may have spoilt, from the operands in global memory. Other
+// elements keep their value, so that no result depends on its neighbours. A call of its
+// own, off the epilogue's registers.
+//
+// A far block has spoilt nothing where the stored value is finite (what overflows on the
+// way stays infinite or NaN) and large beside all that may have been lost below the
+// normal numbers, for each block at most 2^-150, half the smallest of them, times the
+// column's scale (row scales) or the sum of at most 2^39 (a product of scales): less
+// than 2^-24 of the value. So it is with small cotangents beside ordinary activations.
+//
+// Eight columns at a time, each 128-block's sum by the warp's own MMAs on f16 copies of
+// the values. A thread's sixteen bytes of a row serve four MMAs: the order of the
+// positions is the same in both operands, and no other than any other.
 template <bool A_ROW, bool PAIR>
 __device__ __noinline__ void far_tile(const GGParams& P, const Segments& S, int nseg, int tile, int r0, int c0,
                                       int n, int lane) {
   int cur = 0;
   const TileAt T = gg_tile<true, PAIR>(P, S, nseg, tile, cur);
-  const int row0 = T.r0 + r0, rows = P.r - row0, col0 = T.t0 + c0, cols = T.tvalid - c0;
-  const int64_t g = P.mode == 0 ? T.seg : 0;
-  for (int e = lane; e < 32 * n; e += 32) {
-    const int r = e & 31, c = e >> 5;
-    if (c >= cols || r >= rows) continue;
-    const float* sa = P.a_scale + g * P.sa_g + (int64_t)(A_ROW ? row0 + r : (row0 + r) >> 7) * P.sa_r;
-    const float* sb = P.b_scale + col0 + c;
-    bool far = false;
-    for (int kb = 0; kb < T.nkb && !far; ++kb) {
-      const int64_t at = T.k0 / 128 + kb;
-      far = is_far<A_ROW>(sa[at * P.sa_k], sb[at * P.sb_k]);
-    }
-    if (!far) continue;
-    const uint8_t* a = P.a + g * P.a_g + (int64_t)(row0 + r) * P.a_ld;
-    const uint8_t* b = P.b + (int64_t)(col0 + c) * P.b_ld;
-    float total = 0.f;
+  const int row0 = T.r0 + r0, rows = min(32, P.r - row0), col0 = T.t0 + c0, cols = min(n, T.tvalid - c0);
+  if (rows <= 0) return;
+  const int64_t g = P.mode == 0 ? T.seg : 0, at = T.k0 / 128;
+  const int lr = lane >> 2, lq = lane & 3;
+  const float* sa = P.a_scale + g * P.sa_g + at * P.sa_k;
+  const float* sb = P.b_scale + at * P.sb_k + col0;
+  // this thread's elements: rows lr + 8 h, columns first + 2 lq + x
+  const auto a_scale = [&](int kb, int h) {
+    const int row = row0 + min(lr + 8 * h, rows - 1);
+    return sa[kb * P.sa_k + (int64_t)(A_ROW ? row : row >> 7) * P.sa_r];
+  };
+  const auto place = [&](int h, int c) {
+    return (P.mode == 1 ? (int64_t)T.seg * P.o_g : 0) + (int64_t)(col0 + c) * P.o_ld + row0 + lr + 8 * h;
+  };
+  for (int first = 0; first < cols; first += 8) {
+    const int c[2] = {first + 2 * lq, first + 2 * lq + 1};
+    uint32_t far = 0;  // bit 2 h + x
+    float most[2] = {0.f, 0.f};
+#pragma unroll 2
     for (int kb = 0; kb < T.nkb; ++kb) {
-      const int first = T.k0 + kb * 128, end = min(first + 128, P.k);
-      float sum = 0.f;
-      for (int k = first; k < end; k += 16) {
-        const uint4 va = *(const uint4*)(a + k), vb = *(const uint4*)(b + k);
-        const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
+      float s[2];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
-          const float2 x = fp8_pair(wa[q >> 1] >> (16 * (q & 1)) & 0xffffu, P.a_e5);
-          const float2 y = fp8_pair(wb[q >> 1] >> (16 * (q & 1)) & 0xffffu, P.b_e5);
-          if (k + 2 * q < end) sum = fmaf(x.x, y.x, sum);
-          if (k + 2 * q + 1 < end) sum = fmaf(x.y, y.y, sum);
+      for (int x = 0; x < 2; ++x) {
+        s[x] = sb[kb * P.sb_k + min(c[x], cols - 1)];
+        most[x] = fmaxf(most[x], fabsf(s[x]));
+      }
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const float ra = a_scale(kb, h);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) far |= (uint32_t)is_far<A_ROW>(ra, s[x]) << (2 * h + x);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const uint32_t bit = 1u << (2 * h + x);
+        if (lr + 8 * h >= rows || c[x] >= cols) far &= ~bit;
+        if (!(far & bit)) continue;
+        const int64_t o = place(h, c[x]);
+        const float have =
+            fabsf(P.out_f32 ? ((const float*)P.out)[o] : __bfloat162float(((const __nv_bfloat16*)P.out)[o]));
+        if (have <= SCALE_MAX_FLOAT && have >= (float)T.nkb * (A_ROW ? 0x1p-126f * most[x] : 0x1p-87f))
+          far &= ~bit;
+      }
+    if (!__any_sync(0xffffffffu, far != 0)) continue;
+    float total[4][2] = {};
+#pragma unroll 1
+    for (int kb = 0; kb < T.nkb; ++kb) {
+      const int begin = T.k0 + kb * 128, end = min(begin + 128, P.k);
+      float sum[2][4] = {};
+#pragma unroll 1
+      for (int k = begin + 16 * lq; k < begin + 128; k += 64) {
+        uint4 va[4];
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+          va[h] = fp8_piece(P.a + g * P.a_g + (int64_t)(row0 + lr + 8 * h) * P.a_ld + k,
+                            lr + 8 * h < rows ? end - k : 0);
+        const uint4 vb = fp8_piece(P.b + (int64_t)(col0 + first + lr) * P.b_ld + k, first + lr < cols ? end - k : 0);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t a[4][2];
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const uint32_t v = ((const uint32_t*)&va[h])[w];
+            a[h][0] = fp8_pair(v & 0xffffu, P.a_e5);
+            a[h][1] = fp8_pair(v >> 16, P.a_e5);
+          }
+          const uint32_t v = ((const uint32_t*)&vb)[w];
+          const uint32_t b0 = fp8_pair(v & 0xffffu, P.b_e5), b1 = fp8_pair(v >> 16, P.b_e5);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            mma_f16(sum[i], a[2 * i][0], a[2 * i + 1][0], a[2 * i][1], a[2 * i + 1][1], b0, b1);
         }
       }
-      const int64_t at = T.k0 / 128 + kb;
-      total = far_add<A_ROW>(total, sum, sa[at * P.sa_k], sb[at * P.sb_k]);
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        const float ra = a_scale(kb, h);
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          total[h][x] = far_add<A_ROW>(total[h][x], sum[h >> 1][2 * (h & 1) + x], ra,
+                                       sb[kb * P.sb_k + min(c[x], cols - 1)]);
+      }
     }
-    const int64_t o = (P.mode == 1 ? (int64_t)T.seg * P.o_g : 0) + (int64_t)(col0 + c) * P.o_ld + row0 + r;
-    if (P.out_f32) ((float*)P.out)[o] = total;
-    else ((__nv_bfloat16*)P.out)[o] = __float2bfloat16_rn(total);
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        if (far >> (2 * h + x) & 1u) {
+          const int64_t o = place(h, c[x]);
+          if (P.out_f32) ((float*)P.out)[o] = total[h][x];
+          else ((__nv_bfloat16*)P.out)[o] = __float2bfloat16_rn(total[h][x]);
+        }
   }
 }
 
@@ -988,8 +1076,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           cluster_arrive();
           arrived = true;
         }
-        if (SHARES && !far && look.finish(P, kb0, kb1, lane))
-          far = far_scales<A_ROW>(P, T, kb0, kb1, T.r0 + (int)rank * 128, lane);
+        if (SHARES && !far) far = look.finish(P, kb0, kb1, lane);
       }
       if (far) tell();
       if (fail) give_up(4);
@@ -1002,8 +1089,7 @@ grouped_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         const TileAt T = gg_tile<FP8, PAIR>(P, S, nseg, tile, cur);
         FarLook<A_ROW> look;
         look.begin(P, S, T, 0, T.nkb, T.r0 + (int)rank * 128, lane);
-        far = look.finish(P, 0, T.nkb, lane) &&
-              far_scales<A_ROW>(P, T, 0, T.nkb, T.r0 + (int)rank * 128, lane);
+        far = look.finish(P, 0, T.nkb, lane);
       }
       if (far) tell();
     }
@@ -1547,7 +1633,7 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   const int64_t k = d->k;
   AQT_REQUIRE(k == 0 || !fp8 || (d->a_scale != nullptr && d->b_scale != nullptr), AQTB200_EINVAL,
               "fp8 operands need their scales");
-  AQT_REQUIRE(((uintptr_t)d->far & 7) == 0, AQTB200_EINVAL, "marks are eight bytes each, 8-byte aligned");
+  AQT_REQUIRE(((uintptr_t)d->note & 15) == 0, AQTB200_EINVAL, "notes on scales: 16-byte aligned");
 
   GGParams P{};
   P.mode = d->contract_groups;
@@ -1627,8 +1713,8 @@ static int grouped_gemm(const aqtb200_grouped_gemm_desc* d, int32_t* status, cud
   P.a_scale = d->a_scale; P.sa_g = d->a_scale_group_stride; P.sa_k = d->a_scale_k_stride;
   P.sa_r = d->a_scale_r_stride;
   P.b_scale = d->b_scale; P.sb_k = d->b_scale_k_stride;
-  P.far = (const uint64_t*)d->far; P.far_k = d->far_k_stride; P.far_t = d->far_stride;
-  P.far_padded = P.mode == 0 && grouped && d->far_padded;
+  P.note = (const uint4*)d->note; P.note_k = d->note_k_stride; P.note_t = d->note_stride;
+  P.note_padded = P.mode == 0 && grouped && d->note_padded;
   P.a = (const uint8_t*)d->a; P.a_ld = d->a_ld; P.a_g = d->a_group_stride;
   P.b = (const uint8_t*)d->b; P.b_ld = d->b_ld;
   P.k = (int)k; P.a_e5 = d->a_dtype == AQTB200_E5M2; P.b_e5 = d->b_dtype == AQTB200_E5M2;

@@ -588,10 +588,10 @@ int aqtb200_mma_peak(int32_t is_int, int64_t mmas_per_sm, int32_t* status, void*
  *             min(groups, rows)). Negative sizes count as 0, and the running sum
  *             is cut at `rows`. Rows behind the last group are not read and their
  *             places in q_row and scale_row are left as they were.
- * far_row, far_col: optional, without b0 / b1 and `square`: marks of eight bytes for
- *             each tile of 128 rows (with groups: of the padded order) and 128
- *             columns, [row tile][ceil(cols/128)], not zero where one of the tile's
- *             scales in scale_row / scale_col lies outside 2^-63 .. 2^63.
+ * note_row, note_col: optional, without b0 / b1 and `square`: notes for
+ *             aqtb200_grouped_gemm on the range of scale_row / scale_col, sixteen bytes
+ *             for each tile of 128 rows (with groups: of the padded order) and 128
+ *             columns, [row tile][ceil(cols/128)], 16-byte aligned.
  */
 typedef struct aqtb200_block_quant_desc {
   aqtb200_view x;
@@ -607,8 +607,8 @@ typedef struct aqtb200_block_quant_desc {
   float* scale_col;
   const void* group_sizes;
   int64_t groups;
-  void* far_row;
-  void* far_col;
+  void* note_row;
+  void* note_col;
 } aqtb200_block_quant_desc;
 
 int aqtb200_block_quantize(const aqtb200_block_quant_desc* desc, void* stream);
@@ -624,7 +624,7 @@ int aqtb200_block_quantize(const aqtb200_block_quant_desc* desc, void* stream);
  *   contract_groups 1: out[g][t][r] = sum_{k in group g} b[t][k] a[r][k]   drhs
  *       k: the grouped rows; an empty group gives zeros.
  * fp8:  every 128 products are summed on the tensor core, times a_scale times
- *       b_scale, and added in f32 (right to its rounding for any scales, see far).
+ *       b_scale, and added in f32 (right to its rounding for any scales, see note).
  *       bf16: one f32 sum.
  *
  * r         : extent of the output's contiguous index; t: of its row index.
@@ -639,13 +639,13 @@ int aqtb200_block_quantize(const aqtb200_block_quant_desc* desc, void* stream);
  * a_scale   : fp8 only. f32 of (r, block kb) at g*a_scale_group_stride +
  *             kb*a_scale_k_stride + (a_scale_square ? r/128 : r)*a_scale_r_stride.
  * b_scale   : f32 of (t, kb) at kb*b_scale_k_stride + t.
- * far       : optional marks of aqtb200_block_quantize on b's scales, or with
- *             a_scale_square 0 on a's: eight bytes of (block of 128 t or r, kb) at
- *             kb*far_k_stride + block*far_stride (in marks); far_padded: blocks count
- *             from each group's first row. A product of a block's two scales, or of its
- *             sum and one of them, that leaves f32's range where the result does not is
- *             found by them, and what it enters is computed with care. NULL: those
- *             scales lie within 2^-63 .. 2^63, or are zero.
+ * note      : optional notes of aqtb200_block_quantize on b's scales, or with
+ *             a_scale_square 0 on a's: that of (block of 128 t or r, kb) at
+ *             kb*note_k_stride + block*note_stride (counted in notes); note_padded:
+ *             blocks count from each group's first row. A product of a block's two
+ *             scales, or of its sum and one of them, that leaves f32's range where the
+ *             result does not is found by them, and what it enters is computed with
+ *             care. NULL: those scales lie within 2^-63 .. 2^63, or are zero.
  * scales_po2: fp8: every scale is a power of two (po2_scale of
  *             aqtb200_block_quantize). Products with a bf16 result, k up to 2^18 and
  *             enough rows t to fill the device with tiles of more than 128 are then
@@ -683,9 +683,9 @@ typedef struct aqtb200_grouped_gemm_desc {
   int64_t out_ld, out_group_stride;
   void* workspace;
   size_t workspace_bytes;
-  const void* far;
-  int64_t far_k_stride, far_stride;
-  int32_t far_padded;
+  const void* note;
+  int64_t note_k_stride, note_stride;
+  int32_t note_padded;
 } aqtb200_grouped_gemm_desc;
 
 size_t aqtb200_grouped_gemm_workspace_bytes(const aqtb200_grouped_gemm_desc* desc);

@@ -283,13 +283,13 @@ def test_abi_gemm_columns_of_groups(lib):
                          a_group_stride=4096)) == -2
 
 
-def test_abi_marks(lib):
-  """Marks are of one matrix with 1 x 128 blocks, eight bytes each."""
+def test_abi_notes_on_scales(lib):
+  """Notes are of one matrix with 1 x 128 blocks, sixteen bytes each."""
   call = lambda d: lib.aqtb200_block_quantize(C.byref(d), None)
-  assert call(_quant_desc(far_row=260)) == -2
-  assert call(_quant_desc(far_row=256, square=1)) == -2
-  d = _quant_desc(far_row=256)
+  assert call(_quant_desc(note_row=264)) == -2
+  assert call(_quant_desc(note_row=256, square=1)) == -2
+  d = _quant_desc(note_row=256)
   d.x.b0 = 2
   assert call(d) == -2
-  d = _gemm_desc(a_dtype=_lib.E4M3, b_dtype=_lib.E4M3, a_scale=256, b_scale=256, far=260)
+  d = _gemm_desc(a_dtype=_lib.E4M3, b_dtype=_lib.E4M3, a_scale=256, b_scale=256, note=264)
   assert lib.aqtb200_grouped_gemm(C.byref(d), None, None) == -1

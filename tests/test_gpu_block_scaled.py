@@ -588,3 +588,42 @@ def test_far_rows_wherever_they_lie(m, n, rows):
     same[at] = False
     assert torch.equal(out[same], base[same]), first
   _done()
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_far_scales_of_transposed_operands(dtype):
+  """Operands read the way they lie: their marks change places with their values."""
+  x, w, g = (_data((300, 384), dtype, 78, 1.0), _data((384, 200), dtype, 79, 0.3),
+             _data((300, 200), dtype, 80, 1.0))
+  x[:130] *= 2.0 ** -70
+  x[130:, :128] *= 2.0 ** 30
+  w[:, :128] *= 2.0 ** -66
+  g[:, 150:] *= 2.0 ** -90
+  cfg = bs.dot_general_make()
+  out, bp = cfg.vjp(x, w, DIMS)
+  want = (out, *bp(g))
+  flip = lambda t: t.t().contiguous().t()
+  out, bp = cfg.vjp(flip(x), flip(w), DIMS)
+  got = (out, *bp(flip(g)))
+  _done()
+  for a, b, (value, mag, kk) in zip(got, want, _want(_f32(x), _f32(w), _f32(g))):
+    assert torch.equal(a, b)
+    ref.assert_close(_f32(a).astype(np.float64), value, mag, kk, HALF[dtype])
+
+
+@pytest.mark.parametrize('g_exponent', [-90, -100, -112])
+def test_small_cotangents(g_exponent):
+  """Scales below what a sum could stand, and sums that are large enough: the
+  products' own results are right and stay, those of columns that cancel are made
+  anew."""
+  m, k, n = 1500, 300, 1750
+  x, w, g = (_data((m, k), torch.float32, 81, 1.0), _data((k, n), torch.float32, 82, 0.3),
+             _data((m, n), torch.float32, 83, 1.0) * 2.0 ** g_exponent)
+  x[::2, 7] = 0   # meets next to nothing of a column's cotangents
+  g[1::2, 11] = 0
+  g[1::2, 11][::9] = 2.0 ** (g_exponent - 13)
+  out, bp = bs.dot_general_make().vjp(x, w, DIMS)
+  dl, dr = bp(g)
+  _done()
+  for got, (want, mag, kk) in zip((out, dl, dr), _want(_f32(x), _f32(w), _f32(g))):
+    ref.assert_close(_f32(got).astype(np.float64), want, mag, kk, 2.0 ** -24)
