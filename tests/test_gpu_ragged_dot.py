@@ -743,3 +743,38 @@ def test_far_rows_wherever_they_lie(m, n, sizes):
       same[at] = False
       assert torch.equal(out[same], base[same]), first
   _done()
+
+
+@pytest.mark.parametrize('q', [False, True])
+def test_captured_training_step_on_torchs_tape(q):
+  """Forward and backward through autograd in one graph: residuals are memory of the
+  graph, and replays follow new operands and sizes."""
+  x, w, g = (_data((130, 136), torch.bfloat16, 102), _data(
+      (3, 136, 77), torch.bfloat16, 103, 0.1), _data((130, 77), torch.bfloat16, 104))
+  sizes = _sizes([70, 0, 55])
+  cfg = bs.dot_general_make() if q else None
+  a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+
+  def step():
+    y = rd.ragged_dot(a, b, sizes, cfg=cfg)
+    return (y.detach(), *torch.autograd.grad(y, (a, b), g))
+
+  side = torch.cuda.Stream()
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    step()
+  torch.cuda.current_stream().wait_stream(side)
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    got = step()
+  for seed, values in ((105, [70, 0, 55]), (106, [1, 100, 29])):
+    with torch.no_grad():
+      a.copy_(_data(x.shape, x.dtype, seed))
+      b.copy_(_data(w.shape, w.dtype, seed + 10, 0.1))
+    sizes.copy_(_sizes(values))
+    graph.replay()
+    out, bp = rd.ragged_dot_vjp(a, b, sizes, cfg=cfg)
+    want = (out, *bp(g))
+    _done()
+    for s, t in zip(got, want):
+      assert torch.equal(s, t)
