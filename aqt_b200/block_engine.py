@@ -124,8 +124,6 @@ class Side:
                 self.kept, memory, self.note and (self.note[0] + shift, *self.note[1:]))
 
 
-def _align(n):
-  return (n + 255) & -256
 
 
 def _scratch(nbytes, device):
@@ -168,23 +166,23 @@ def quantize(x, dtype, row=True, col=False, square=False, po2=False,
   at_q_row = at_s_row = at_q_col = at_s_col = at_n_row = at_n_col = end = 0
   if row:
     ld_row = (c + 15) & -16
-    end = _align(batch * r * ld_row)
+    end = (batch * r * ld_row + 255) & -256
   if square:
     at_s_row = end
-    end += _align(batch * nr * nc * 4)
+    end += (batch * nr * nc * 4 + 255) & -256
   elif row:
     at_s_row = end
-    end += _align(batch * nc * r * 4)
+    end += (batch * nc * r * 4 + 255) & -256
   if col:
     at_q_col = end
     ld_col = (r + 15) & -16 if group_sizes is None else row_blocks * BLOCK
-    end += _align(batch * c * ld_col)
+    end += (batch * c * ld_col + 255) & -256
     if not square:
       at_s_col = end
-      end += _align(batch * row_blocks * c * 4)
+      end += (batch * row_blocks * c * 4 + 255) & -256
   notes = not square and batch == 1
   if notes:
-    nbytes = _align(row_blocks * nc * 16)
+    nbytes = (row_blocks * nc * 16 + 255) & -256
     if row:
       at_n_row = end
       end += nbytes

@@ -393,7 +393,7 @@ __device__ __forceinline__ int share_of(int nkb, int part, int split) {
 //   row scales       the sum times the row's scale, where that lies in ROW_MIN .. ROW_MAX
 // Elements with a block of other scales are computed again, by far_tile, when all is
 // stored. (Nothing of this is in the epilogue's loop or between its tiles: choosing
-// slab by slab cost 2 to 5 %, and a verdict on each tile 1 to 2 %.) 8192 x 4096 x 14336
+// slab by slab cost 2 to 5 %, and a decision on each tile 1 to 2 %.) 8192 x 4096 x 14336
 // with operands of 2^-60 and 2^-62, all of it: 82 ms in place of 0.6; cotangents of
 // 2^-95, where it only looks: 5.0 ms backward in place of 1.3.
 constexpr float GG_ROW_MIN = 0x1p-94f, GG_ROW_MAX = 0x1p89f;

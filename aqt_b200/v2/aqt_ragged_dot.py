@@ -84,7 +84,8 @@ def _check(lhs, rhs, group_sizes, cfg, preferred):
     raise ValueError(f'contracted extents differ: lhs {tuple(lhs.shape)}, rhs '
                      f'{tuple(w.shape)}')
   be.check_group_sizes(group_sizes, w.shape[0])
-  be.check_same_device(lhs, w, group_sizes)
+  if not lhs.device == w.device == group_sizes.device:
+    be.check_same_device(lhs, w, group_sizes)
   return block_scaled._out_dtype(preferred, lhs)  # pylint: disable=protected-access
 
 

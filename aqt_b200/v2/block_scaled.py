@@ -334,7 +334,8 @@ def _dims(lhs, rhs, dimension_numbers):
     be.check_operand(w, 'rhs')
     if lhs.dtype != w.dtype:
       raise TypeError(f'Unmatched lhs and rhs dtype: {lhs.dtype} vs {w.dtype}')
-  be.check_same_device(lhs, w)
+  if lhs.device != w.device:
+    be.check_same_device(lhs, w)
   if w.ndim != 2:
     raise NotImplementedError(f'rhs is a matrix (got {tuple(w.shape)})')
   la, ra = lca[0], rca[0]
