@@ -438,42 +438,47 @@ class Residuals:
   have moved.
   """
 
-  __slots__ = ('lhs', 'rhs', 'stream', 'base')
+  __slots__ = ('lhs', 'rhs', 'stream', 'memory', 'base')
 
   def __init__(self, lhs, rhs):
     self.lhs, self.rhs = lhs, rhs
     self.stream = engine._stream()  # pylint: disable=protected-access
-    self.base = None
-
-  def memory(self):
-    return tuple(s.keep if isinstance(s, Side) else s
-                 for s in (self.lhs, self.rhs))
+    self.memory = (lhs.keep if isinstance(lhs, Side) else lhs,
+                   rhs.keep if isinstance(rhs, Side) else rhs)
 
   def about_to_use(self):
     """Called with the operands' device current."""
     if engine._stream() != self.stream:  # pylint: disable=protected-access
-      for t in self.memory():
+      for t in self.memory:
         if t is not None and t.is_cuda:
           t.record_stream(torch.cuda.current_stream())
 
   def release(self):
-    memory = self.memory()
-    self.base = tuple(t if t is None else t.data_ptr() for t in memory)
-    self.lhs, self.rhs = (s.at(0, None) if isinstance(s, Side) else None
-                          for s in (self.lhs, self.rhs))
+    memory, self.memory = self.memory, None
+    self.base = tuple([t if t is None else t.data_ptr() for t in memory])
+    if isinstance(self.lhs, Side):
+      self.lhs.keep = None
+    else:
+      self.lhs = None
+    if isinstance(self.rhs, Side):
+      self.rhs.keep = None
+    else:
+      self.rhs = None
     return memory
 
-  def regain(self, *memory):
+  def regain(self, lhs, rhs):
     r = object.__new__(Residuals)
-    r.stream, r.base = self.stream, None
-    r.lhs, r.rhs = (_regain(s, base, t) for s, base, t in zip(
-        (self.lhs, self.rhs), self.base, memory))
+    r.stream, r.memory = self.stream, (lhs, rhs)
+    r.lhs = _regain(self.lhs, self.base[0], lhs)
+    r.rhs = _regain(self.rhs, self.base[1], rhs)
     return r
 
 
 def _regain(side, base, t):
   if side is None or t is None:
     return t
-  if t.data_ptr() != base and (t.data_ptr() % 256 or not t.is_contiguous()):
+  if t.data_ptr() == base:
+    return side
+  if t.data_ptr() % 256 or not t.is_contiguous():
     t = t.clone(memory_format=torch.contiguous_format)  # aligned as at first
   return side.at(base, t)
